@@ -293,6 +293,77 @@ int rode_sddmm_f32_ordered(int M, int m1, int m2, int n, int k, long long nnz, c
                            float *out, void *workspace, size_t workspace_bytes, rode_stream_t stream1,
                            rode_stream_t stream2);
 
+/* ------------------------------------------------------------------------------------
+ * Attention on the two sparse patterns of language models, without storing the pattern: scores at the visible (query, key)
+ * pairs, softmax over them and the product with the values in one pass (what SDDMM, a row softmax and SpMM do on a CSR
+ * pattern).  No counterpart in the reference.
+ *
+ *   dtype      of q, k, v, out and the gradients; sums, softmax statistics and partial results are fp32
+ *   dim        head dimension: any multiple of 4 up to 256
+ *   heads      query heads, a multiple of kv_heads; query head h reads key head h / (heads / kv_heads)
+ *   scale      of the scores (usually 1 / sqrt(dim))
+ * Strides are in elements, the last dimension is contiguous.  Bases and strides must be multiples of 4 elements; 16-bit operands
+ * whose bases and strides are multiples of 16 bytes, with dim a multiple of 8 up to 128, run on the tensor cores, which round the softmax weights (and,
+ * backward, the scores' gradients) to dtype before they multiply.  Rows of an operand at most 2^30.
+ *
+ * A query that sees no key gets a zero row.  A non-finite key or value reaches the queries that see it, and may reach other
+ * queries of the same sequence (whose weight for it is 0), never another sequence; nothing behind lengths[b] is read.
+ * Results do not depend on the order in which thread blocks run.
+ */
+enum rode_dtype { RODE_F32 = 0, RODE_F16 = 1, RODE_BF16 = 2 };
+
+/* An operand: element (batch, row, head, d) is data[batch * s.batch + row * s.row + head * s.head + d]. */
+typedef struct {
+    const void *data;
+    long long batch, row, head;
+} rode_heads_t;
+
+/* Sliding window and sinks over packed sequences.  Sequence s owns rows q_offsets[s] .. q_offsets[s+1] of q and
+ * k_offsets[s] .. k_offsets[s+1] of k and v (int32[n_seq+1] on the device, not decreasing; both null: one sequence of all
+ * rows).  Its queries are its last positions: query i stands at p = i + keys - queries and sees key j
+ * when j <= p and (p - j < window or j < sinks).
+ *   q [q_rows, heads, dim], k and v [k_rows, kv_heads, dim]   .batch is not used
+ *   out  [q_rows, heads, dim] contiguous
+ *   lse  float[heads, q_rows], natural logarithm of the softmax sums (-inf for a query that sees no key); may be null
+ *   clear  1: rows of out (of the gradients) that belong to no sequence become zero; 0: they are left as they were
+ */
+int rode_window_attention(int dtype, int n_seq, const int *q_offsets, const int *k_offsets, int q_rows, int k_rows,
+                          int heads, int kv_heads, int dim, int window, int sinks, float scale, int clear,
+                          const rode_heads_t *q, const rode_heads_t *k, const rode_heads_t *v, void *out, float *lse,
+                          rode_stream_t stream);
+
+/* Its gradients: dq [q_rows, heads, dim], dk and dv [k_rows, kv_heads, dim] contiguous, dk and dv both or neither (null).
+ * out and lse are what the forward call wrote.  workspace: rode_window_attention_backward_workspace_bytes() bytes,
+ * 16-byte aligned, not shared by calls that may overlap in time. */
+int rode_window_attention_backward_workspace_bytes(int q_rows, int heads, size_t *bytes);
+int rode_window_attention_backward(int dtype, int n_seq, const int *q_offsets, const int *k_offsets, int q_rows,
+                                   int k_rows, int heads, int kv_heads, int dim, int window, int sinks, float scale,
+                                   int clear, const rode_heads_t *q, const rode_heads_t *k, const rode_heads_t *v,
+                                   const void *out, const float *lse, const rode_heads_t *dout, void *dq, void *dk,
+                                   void *dv, void *workspace, size_t workspace_bytes, rode_stream_t stream);
+
+/* The same pattern for one new token per sequence against a cache: request b's query (q [batch, heads, dim], .row is not
+ * used) stands at position lengths[b] - 1 of its cache (k_cache, v_cache [batch, capacity, kv_heads, dim]), whose rows from
+ * lengths[b] on are not read.  lengths int32[batch] on the device, taken as at least 0 and at most capacity.
+ * out [batch, heads, dim] contiguous.  workspace as above, 0 bytes for some sizes; it depends on the current device. */
+int rode_window_attention_step_workspace_bytes(int batch, int capacity, int heads, int kv_heads, int dim, int window,
+                                               int sinks, size_t *bytes);
+int rode_window_attention_step(int dtype, int batch, int capacity, int heads, int kv_heads, int dim, int window,
+                               int sinks, float scale, const rode_heads_t *q, const rode_heads_t *k_cache,
+                               const rode_heads_t *v_cache, const int *lengths, void *out, void *workspace,
+                               size_t workspace_bytes, rode_stream_t stream);
+
+/* One new token per request behind a prefix that all requests share: request b's query sees all rows of the prefix (prefix_k,
+ * prefix_v [prefix, kv_heads, dim], .batch is not used) and the first lengths[b] rows of its own cache.  The queries of all
+ * requests go through the prefix together, so that it is read once. */
+int rode_shared_prefix_attention_workspace_bytes(int batch, int prefix, int capacity, int heads, int kv_heads, int dim,
+                                                 size_t *bytes);
+int rode_shared_prefix_attention(int dtype, int batch, int prefix, int capacity, int heads, int kv_heads, int dim,
+                                 float scale, const rode_heads_t *q, const rode_heads_t *prefix_k,
+                                 const rode_heads_t *prefix_v, const rode_heads_t *k_cache, const rode_heads_t *v_cache,
+                                 const int *lengths, void *out, void *workspace, size_t workspace_bytes,
+                                 rode_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -17,7 +17,8 @@ ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 INCLUDE = os.path.join(ROOT, "include")
 LIB = os.path.join(PKG, "librode_b200.so")
-SOURCES = ["rode_host.cu", "rode_preprocess.cu", "rode_hot_columns.cu", "rode_spmm.cu", "rode_sddmm.cu"]
+SOURCES = ["rode_host.cu", "rode_preprocess.cu", "rode_hot_columns.cu", "rode_spmm.cu", "rode_sddmm.cu", "rode_attention.cu",
+           "rode_attention_simple.cu"]
 NVCC_FLAGS = [
     "-O3", "-std=c++17", "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo",
     "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=default", "--expt-relaxed-constexpr",
@@ -42,7 +43,7 @@ def build_library(force: bool = False, verbose: bool = False) -> str:
     if not force and _newer(LIB, _deps()):
         return LIB
     nvcc = os.environ.get("NVCC", "nvcc")
-    cmd = [nvcc, *NVCC_FLAGS, "-shared", "-I", INCLUDE, "-I", CSRC]
+    cmd = [nvcc, *NVCC_FLAGS, "--threads", "0", "-shared", "-I", INCLUDE, "-I", CSRC]
     if verbose:
         cmd += ["-Xptxas", "-v"]
     cmd += [os.path.join(CSRC, s) for s in SOURCES] + ["-o", LIB]
@@ -63,8 +64,8 @@ def build_torch_extension(force: bool = False) -> str:
 
     suffix = sysconfig.get_config_var("EXT_SUFFIX") or ".so"
     target = os.path.join(PKG, "rode_sddmm_cuda" + suffix)
-    src = os.path.join(PKG, "torch_ext", "rode_sddmm_cuda.cpp")
-    if not force and _newer(target, [src, LIB] + _deps()):
+    src = [os.path.join(PKG, "torch_ext", f) for f in ("rode_sddmm_cuda.cpp", "rode_attention.cpp")]
+    if not force and _newer(target, [*src, LIB] + _deps()):
         return target
     build_library()
     cuda_home = os.environ.get("CUDA_HOME", "/usr/local/cuda")
@@ -76,7 +77,7 @@ def build_torch_extension(force: bool = False) -> str:
            "-DTORCH_API_INCLUDE_EXTENSION_H", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
     for i in inc:
         cmd += ["-I", i]
-    cmd += [src, "-o", target, "-L", PKG, "-lrode_b200", "-L", torch_lib, "-ltorch", "-ltorch_cpu", "-lc10",
+    cmd += [*src, "-o", target, "-L", PKG, "-lrode_b200", "-L", torch_lib, "-ltorch", "-ltorch_cpu", "-lc10",
             "-ltorch_python", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{torch_lib}"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:

@@ -32,6 +32,9 @@ C_ABI_SYMBOLS = (
     "rode_spmm_f32_hot", "rode_spmm_f64_hot", "rode_spmm_f32_all", "rode_spmm_f64_all",
     "rode_order_verdict", "rode_sddmm_order_pays", "rode_sddmm_workspace_bytes", "rode_sddmm_f32_ordered",
     "rode_spmm_order_pays", "rode_spmm_ordered_workspace_bytes", "rode_spmm_f32_ordered", "rode_spmm_f64_ordered",
+    "rode_window_attention", "rode_window_attention_backward_workspace_bytes", "rode_window_attention_backward",
+    "rode_window_attention_step_workspace_bytes", "rode_window_attention_step",
+    "rode_shared_prefix_attention_workspace_bytes", "rode_shared_prefix_attention",
 )
 # Itanium-ABI names of the C++ entry points declared in RoDeSpmm.h / RoDeSddmm.h /
 # RoDePreprocess.h; identical to the names the reference's own objects export.
@@ -55,6 +58,15 @@ class RodeError(RuntimeError):
 
 
 _lib: Optional[ctypes.CDLL] = None
+
+
+class Heads(ctypes.Structure):
+    """rode_heads_t: an attention operand, strides in elements."""
+
+    _fields_ = [("data", ctypes.c_void_p), ("batch", ctypes.c_longlong), ("row", ctypes.c_longlong), ("head", ctypes.c_longlong)]
+
+
+RODE_F32, RODE_F16, RODE_BF16 = 0, 1, 2
 
 
 def load() -> ctypes.CDLL:
@@ -95,12 +107,24 @@ def load() -> ctypes.CDLL:
     lib.rode_spmm_f64_ordered.argtypes = lib.rode_spmm_f32_ordered.argtypes
     lib.rode_sddmm_workspace_bytes.argtypes = [ci, ci, ctypes.c_longlong, ctypes.POINTER(sz)]
     lib.rode_sddmm_f32_ordered.argtypes = [ci, ci, ci, ci, ci, ctypes.c_longlong] + [vp] * 10 + [sz, vp, vp]
+    cf, heads = ctypes.c_float, ctypes.POINTER(Heads)
+    lib.rode_window_attention.argtypes = [ci, ci, vp, vp] + [ci] * 7 + [cf, ci] + [heads] * 3 + [vp] * 3
+    lib.rode_window_attention_backward_workspace_bytes.argtypes = [ci, ci, ctypes.POINTER(sz)]
+    lib.rode_window_attention_backward.argtypes = ([ci, ci, vp, vp] + [ci] * 7 + [cf, ci] + [heads] * 3 + [vp, vp, heads]
+                                                   + [vp] * 4 + [sz, vp])
+    lib.rode_window_attention_step_workspace_bytes.argtypes = [ci] * 7 + [ctypes.POINTER(sz)]
+    lib.rode_window_attention_step.argtypes = [ci] * 8 + [cf] + [heads] * 3 + [vp] * 3 + [sz, vp]
+    lib.rode_shared_prefix_attention_workspace_bytes.argtypes = [ci] * 6 + [ctypes.POINTER(sz)]
+    lib.rode_shared_prefix_attention.argtypes = [ci] * 7 + [cf] + [heads] * 5 + [vp] * 3 + [sz, vp]
     for name in ("rode_preprocess_workspace_bytes", "rode_preprocess_capacity", "rode_preprocess",
                  "rode_preprocess_noalloc", "rode_preprocess_cpu", "rode_spmm_workspace_bytes", "rode_spmm_f32", "rode_spmm_f64",
                  "rode_sddmm_f32", "rode_hot_columns_workspace_bytes", "rode_hot_columns_words", "rode_hot_columns",
                  "rode_spmm_f32_hot", "rode_spmm_f64_hot", "rode_spmm_f32_all", "rode_spmm_f64_all",
                  "rode_order_verdict", "rode_sddmm_order_pays", "rode_sddmm_workspace_bytes", "rode_sddmm_f32_ordered",
-                 "rode_spmm_order_pays", "rode_spmm_ordered_workspace_bytes", "rode_spmm_f32_ordered", "rode_spmm_f64_ordered"):
+                 "rode_spmm_order_pays", "rode_spmm_ordered_workspace_bytes", "rode_spmm_f32_ordered", "rode_spmm_f64_ordered",
+                 "rode_window_attention", "rode_window_attention_backward_workspace_bytes", "rode_window_attention_backward",
+                 "rode_window_attention_step_workspace_bytes", "rode_window_attention_step",
+                 "rode_shared_prefix_attention_workspace_bytes", "rode_shared_prefix_attention"):
         getattr(lib, name).restype = ci
     _lib = lib
     return lib

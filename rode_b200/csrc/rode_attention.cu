@@ -1,0 +1,297 @@
+// C entry points of the attention operators: argument checks, workspaces, which kernels a call runs on.
+#include "rode_attention.cuh"
+
+namespace rode {
+namespace {
+
+constexpr int kMaxRows = 1 << 30;
+constexpr int kMaxHeads = 65535;  // gridDim.y
+
+int check_shape(const char *what, int dtype, int heads, int kv_heads, int dim, float scale) {
+    if (dtype != RODE_F32 && dtype != RODE_F16 && dtype != RODE_BF16)
+        return fail(RODE_ERR_INVALID_ARGUMENT, "%s: unknown dtype %d", what, dtype);
+    if (heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || heads > kMaxHeads)
+        return fail(RODE_ERR_INVALID_ARGUMENT, "%s: heads = %d must be a positive multiple of kv_heads = %d, at most %d", what,
+                    heads, kv_heads, kMaxHeads);
+    if (dim <= 0 || dim % 4 != 0 || dim > 256)
+        return fail(RODE_ERR_INVALID_ARGUMENT, "%s: dim = %d must be a multiple of 4, at most 256", what, dim);
+    if (!(scale > -INFINITY && scale < INFINITY)) return fail(RODE_ERR_INVALID_ARGUMENT, "%s: scale must be finite", what);
+    return RODE_OK;
+}
+
+int check_window(const char *what, int window, int sinks) {
+    if (window <= 0 || sinks < 0)
+        return fail(RODE_ERR_INVALID_ARGUMENT, "%s: window = %d must be positive, sinks = %d must not be negative", what, window,
+                    sinks);
+    return RODE_OK;
+}
+
+size_t element_bytes(int dtype) { return dtype == RODE_F32 ? 4 : 2; }
+
+// Elements (of a power of two) that the base and all strides are multiples of, at most `most`.
+bool aligned_heads(const rode_heads_t &x, int dtype, long long elements) {
+    return aligned_to(x.data, elements * element_bytes(dtype)) && x.batch % elements == 0 && x.row % elements == 0 &&
+           x.head % elements == 0;
+}
+
+int check_operand(const char *what, const char *name, const rode_heads_t *x, int dtype, bool read) {
+    if (!read) return RODE_OK;
+    if (x == nullptr || x->data == nullptr) return fail(RODE_ERR_INVALID_ARGUMENT, "%s: null pointer %s", what, name);
+    if (x->batch < 0 || x->row < 0 || x->head < 0)
+        return fail(RODE_ERR_INVALID_ARGUMENT, "%s: %s has a negative stride", what, name);
+    if (!aligned_heads(*x, dtype, 4))
+        return fail(RODE_ERR_INVALID_ARGUMENT, "%s: base and strides of %s must be aligned to 4 elements", what, name);
+    return RODE_OK;
+}
+
+int check_result(const char *what, const char *name, const void *x, bool written) {
+    if (written && x == nullptr) return fail(RODE_ERR_INVALID_ARGUMENT, "%s: null pointer %s", what, name);
+    if (written && !aligned_to(x, 16)) return fail(RODE_ERR_INVALID_ARGUMENT, "%s: %s must be 16-byte aligned", what, name);
+    return RODE_OK;
+}
+
+int check_workspace(const char *what, const void *ws, size_t have, size_t need) {
+    if (need == 0) return RODE_OK;
+    if (ws == nullptr || have < need)
+        return fail(RODE_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, got %zu", what, need, ws == nullptr ? 0 : have);
+    if (!aligned_to(ws, 16)) return fail(RODE_ERR_WORKSPACE, "%s: workspace must be 16-byte aligned", what);
+    return RODE_OK;
+}
+
+int check_packed(const char *what, int n_seq, const int *q_offsets, const int *k_offsets, int q_rows, int k_rows) {
+    if (q_rows < 0 || k_rows < 0 || q_rows > kMaxRows || k_rows > kMaxRows)
+        return fail(RODE_ERR_INVALID_ARGUMENT, "%s: q_rows = %d and k_rows = %d must be 0 to 2^30", what, q_rows, k_rows);
+    if ((q_offsets == nullptr) != (k_offsets == nullptr))
+        return fail(RODE_ERR_INVALID_ARGUMENT, "%s: offsets of queries and keys, or neither", what);
+    if (q_offsets == nullptr ? n_seq != 1 : (n_seq < 0 || n_seq > kMaxRows))
+        return fail(RODE_ERR_INVALID_ARGUMENT, "%s: bad number of sequences %d", what, n_seq);
+    return RODE_OK;
+}
+
+#define RODE_TRY(expr)                            \
+    do {                                          \
+        if (const int rode_e_ = (expr)) return rode_e_; \
+    } while (0)
+
+// Into how many parts the keys of a call with few rows are cut: enough for about four CTAs of the single-token kernel per SM, none
+// of fewer than 256 keys.
+int parts_of(long long ctas, long long keys) {
+    const long long want = (4ll * sm_count() + ctas - 1) / ctas, most = (keys + 255) / 256;
+    const long long n = want < most ? want : most;
+    return static_cast<int>(n < 1 ? 1 : n > 128 ? 128 : n);
+}
+
+struct Parts {
+    int prefix, own;
+    size_t bytes;
+};
+
+Parts plan_parts(int batch, int prefix, long long seen, int heads, int kv_heads, int dim) {
+    Parts p = {0, 0, 0};
+    if (batch == 0) return p;
+    const int group = heads / kv_heads;
+    p.own = parts_of(static_cast<long long>(batch) * kv_heads * ((group + 7) / 8), seen);
+    if (prefix > 0) p.prefix = parts_of((static_cast<long long>(batch) * group + 63) / 64 * kv_heads, prefix);
+    const int n = p.prefix + p.own;
+    if (n > 1) p.bytes = static_cast<size_t>(n) * batch * heads * (dim + 1) * sizeof(float);
+    return p;
+}
+
+int run_cached(const char *what, int dtype, Cached c, const Parts &parts, void *workspace, size_t workspace_bytes,
+               cudaStream_t stream) {
+    RODE_TRY(check_workspace(what, workspace, workspace_bytes, parts.bytes));
+    const int n = parts.prefix + parts.own;
+    if (n > 1) {
+        c.part_out = static_cast<float *>(workspace);
+        c.part_lse = c.part_out + static_cast<size_t>(n) * c.batch * c.win.heads * c.win.dim;
+    }
+    if (parts.prefix > 0) RODE_TRY(simple_shared(dtype, c, 0, parts.prefix, stream));
+    RODE_TRY(simple_step(dtype, c, parts.prefix, parts.own, stream));
+    if (n > 1) RODE_TRY(join_parts(dtype, c, n, stream));
+    return RODE_OK;
+}
+
+}  // namespace
+}  // namespace rode
+
+using namespace rode;
+
+extern "C" {
+
+int rode_window_attention(int dtype, int n_seq, const int *q_offsets, const int *k_offsets, int q_rows, int k_rows,
+                          int heads, int kv_heads, int dim, int window, int sinks, float scale, int clear,
+                          const rode_heads_t *q, const rode_heads_t *k, const rode_heads_t *v, void *out, float *lse,
+                          rode_stream_t stream) {
+    const char *what = "rode_window_attention";
+    RODE_TRY(check_shape(what, dtype, heads, kv_heads, dim, scale));
+    RODE_TRY(check_window(what, window, sinks));
+    RODE_TRY(check_packed(what, n_seq, q_offsets, k_offsets, q_rows, k_rows));
+    RODE_TRY(check_operand(what, "q", q, dtype, q_rows > 0));
+    RODE_TRY(check_operand(what, "k", k, dtype, q_rows > 0 && k_rows > 0));
+    RODE_TRY(check_operand(what, "v", v, dtype, q_rows > 0 && k_rows > 0));
+    RODE_TRY(check_result(what, "out", out, q_rows > 0));
+    if (q_rows == 0) return RODE_OK;
+    Prompt p = {};
+    p.seqs = {q_offsets, k_offsets, n_seq, q_rows, k_rows};
+    p.win = {window, sinks, heads, kv_heads, dim, scale};
+    p.q = *q;
+    if (k_rows > 0) {
+        p.k = *k;
+        p.v = *v;
+    }
+    p.out = out;
+    p.lse = lse;
+    p.clear = clear != 0;
+    return simple_prompt(dtype, p, stream);
+}
+
+int rode_window_attention_backward_workspace_bytes(int q_rows, int heads, size_t *bytes) {
+    if (q_rows < 0 || q_rows > kMaxRows || heads <= 0 || heads > kMaxHeads || bytes == nullptr)
+        return fail(RODE_ERR_INVALID_ARGUMENT, "rode_window_attention_backward_workspace_bytes: bad argument");
+    *bytes = static_cast<size_t>(q_rows) * heads * sizeof(float);
+    return RODE_OK;
+}
+
+int rode_window_attention_backward(int dtype, int n_seq, const int *q_offsets, const int *k_offsets, int q_rows,
+                                   int k_rows, int heads, int kv_heads, int dim, int window, int sinks, float scale,
+                                   int clear, const rode_heads_t *q, const rode_heads_t *k, const rode_heads_t *v,
+                                   const void *out, const float *lse, const rode_heads_t *dout, void *dq, void *dk,
+                                   void *dv, void *workspace, size_t workspace_bytes, rode_stream_t stream) {
+    const char *what = "rode_window_attention_backward";
+    RODE_TRY(check_shape(what, dtype, heads, kv_heads, dim, scale));
+    RODE_TRY(check_window(what, window, sinks));
+    RODE_TRY(check_packed(what, n_seq, q_offsets, k_offsets, q_rows, k_rows));
+    const bool both = q_rows > 0 && k_rows > 0, keys = dk != nullptr || dv != nullptr;
+    RODE_TRY(check_operand(what, "q", q, dtype, q_rows > 0));
+    RODE_TRY(check_operand(what, "k", k, dtype, both));
+    RODE_TRY(check_operand(what, "v", v, dtype, both));
+    RODE_TRY(check_operand(what, "dout", dout, dtype, q_rows > 0));
+    RODE_TRY(check_result(what, "out", out, q_rows > 0));
+    RODE_TRY(check_result(what, "dq", dq, q_rows > 0));
+    RODE_TRY(check_result(what, "dk", dk, keys && k_rows > 0));
+    RODE_TRY(check_result(what, "dv", dv, keys && k_rows > 0));
+    if (q_rows > 0 && lse == nullptr) return fail(RODE_ERR_INVALID_ARGUMENT, "%s: null pointer lse", what);
+    size_t need = 0;
+    RODE_TRY(rode_window_attention_backward_workspace_bytes(q_rows, heads, &need));
+    RODE_TRY(check_workspace(what, workspace, workspace_bytes, need));
+    if (q_rows == 0 && (k_rows == 0 || !keys)) return RODE_OK;
+    Prompt p = {};
+    p.seqs = {q_offsets, k_offsets, n_seq, q_rows, k_rows};
+    p.win = {window, sinks, heads, kv_heads, dim, scale};
+    if (q_rows > 0) {
+        p.q = *q;
+        p.dout = *dout;
+    }
+    if (k_rows > 0 && k != nullptr && v != nullptr) {
+        p.k = *k;
+        p.v = *v;
+    }
+    p.out = const_cast<void *>(out);
+    p.lse = const_cast<float *>(lse);
+    p.dq = dq;
+    p.dk = dk;
+    p.dv = dv;
+    p.delta = static_cast<float *>(workspace);
+    p.clear = clear != 0;
+    return simple_prompt_backward(dtype, p, stream);
+}
+
+static int check_cached_sizes(const char *what, int batch, int prefix, int capacity) {
+    if (batch < 0 || batch > kMaxRows || prefix < 0 || prefix > kMaxRows || capacity < 0 || capacity > kMaxRows)
+        return fail(RODE_ERR_INVALID_ARGUMENT, "%s: batch = %d, prefix = %d and capacity = %d must be 0 to 2^30", what, batch, prefix,
+                    capacity);
+    return RODE_OK;
+}
+
+static long long seen_at_most(int capacity, int window, int sinks) {
+    const long long seen = static_cast<long long>(window) + sinks;
+    return seen < capacity ? seen : capacity;
+}
+
+int rode_window_attention_step_workspace_bytes(int batch, int capacity, int heads, int kv_heads, int dim, int window,
+                                               int sinks, size_t *bytes) {
+    const char *what = "rode_window_attention_step_workspace_bytes";
+    if (bytes == nullptr) return fail(RODE_ERR_INVALID_ARGUMENT, "%s: null pointer bytes", what);
+    RODE_TRY(check_shape(what, RODE_F32, heads, kv_heads, dim, 1.f));
+    RODE_TRY(check_window(what, window, sinks));
+    RODE_TRY(check_cached_sizes(what, batch, 0, capacity));
+    *bytes = plan_parts(batch, 0, seen_at_most(capacity, window, sinks), heads, kv_heads, dim).bytes;
+    return RODE_OK;
+}
+
+int rode_window_attention_step(int dtype, int batch, int capacity, int heads, int kv_heads, int dim, int window,
+                               int sinks, float scale, const rode_heads_t *q, const rode_heads_t *k_cache,
+                               const rode_heads_t *v_cache, const int *lengths, void *out, void *workspace,
+                               size_t workspace_bytes, rode_stream_t stream) {
+    const char *what = "rode_window_attention_step";
+    RODE_TRY(check_shape(what, dtype, heads, kv_heads, dim, scale));
+    RODE_TRY(check_window(what, window, sinks));
+    RODE_TRY(check_cached_sizes(what, batch, 0, capacity));
+    RODE_TRY(check_operand(what, "q", q, dtype, batch > 0));
+    RODE_TRY(check_operand(what, "k_cache", k_cache, dtype, batch > 0 && capacity > 0));
+    RODE_TRY(check_operand(what, "v_cache", v_cache, dtype, batch > 0 && capacity > 0));
+    RODE_TRY(check_result(what, "out", out, batch > 0));
+    if (batch > 0 && lengths == nullptr) return fail(RODE_ERR_INVALID_ARGUMENT, "%s: null pointer lengths", what);
+    if (batch == 0) return RODE_OK;
+    Cached c = {};
+    c.batch = batch;
+    c.capacity = capacity;
+    c.win = {window, sinks, heads, kv_heads, dim, scale};
+    c.q = *q;
+    if (capacity > 0) {
+        c.k = *k_cache;
+        c.v = *v_cache;
+    }
+    c.lengths = lengths;
+    c.out = out;
+    return run_cached(what, dtype, c, plan_parts(batch, 0, seen_at_most(capacity, window, sinks), heads, kv_heads, dim), workspace,
+                      workspace_bytes, stream);
+}
+
+int rode_shared_prefix_attention_workspace_bytes(int batch, int prefix, int capacity, int heads, int kv_heads, int dim,
+                                                 size_t *bytes) {
+    const char *what = "rode_shared_prefix_attention_workspace_bytes";
+    if (bytes == nullptr) return fail(RODE_ERR_INVALID_ARGUMENT, "%s: null pointer bytes", what);
+    RODE_TRY(check_shape(what, RODE_F32, heads, kv_heads, dim, 1.f));
+    RODE_TRY(check_cached_sizes(what, batch, prefix, capacity));
+    *bytes = plan_parts(batch, prefix, capacity, heads, kv_heads, dim).bytes;
+    return RODE_OK;
+}
+
+int rode_shared_prefix_attention(int dtype, int batch, int prefix, int capacity, int heads, int kv_heads, int dim,
+                                 float scale, const rode_heads_t *q, const rode_heads_t *prefix_k,
+                                 const rode_heads_t *prefix_v, const rode_heads_t *k_cache, const rode_heads_t *v_cache,
+                                 const int *lengths, void *out, void *workspace, size_t workspace_bytes,
+                                 rode_stream_t stream) {
+    const char *what = "rode_shared_prefix_attention";
+    RODE_TRY(check_shape(what, dtype, heads, kv_heads, dim, scale));
+    RODE_TRY(check_cached_sizes(what, batch, prefix, capacity));
+    RODE_TRY(check_operand(what, "q", q, dtype, batch > 0));
+    RODE_TRY(check_operand(what, "prefix_k", prefix_k, dtype, batch > 0 && prefix > 0));
+    RODE_TRY(check_operand(what, "prefix_v", prefix_v, dtype, batch > 0 && prefix > 0));
+    RODE_TRY(check_operand(what, "k_cache", k_cache, dtype, batch > 0 && capacity > 0));
+    RODE_TRY(check_operand(what, "v_cache", v_cache, dtype, batch > 0 && capacity > 0));
+    RODE_TRY(check_result(what, "out", out, batch > 0));
+    if (batch > 0 && lengths == nullptr) return fail(RODE_ERR_INVALID_ARGUMENT, "%s: null pointer lengths", what);
+    if (batch == 0) return RODE_OK;
+    Cached c = {};
+    c.batch = batch;
+    c.capacity = capacity;
+    c.prefix = prefix;
+    // every row of the own cache up to the length
+    c.win = {kMaxRows, 0, heads, kv_heads, dim, scale};
+    c.q = *q;
+    if (prefix > 0) {
+        c.pk = *prefix_k;
+        c.pv = *prefix_v;
+    }
+    if (capacity > 0) {
+        c.k = *k_cache;
+        c.v = *v_cache;
+    }
+    c.lengths = lengths;
+    c.out = out;
+    return run_cached(what, dtype, c, plan_parts(batch, prefix, capacity, heads, kv_heads, dim), workspace, workspace_bytes, stream);
+}
+
+}  // extern "C"

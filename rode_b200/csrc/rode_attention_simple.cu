@@ -1,0 +1,669 @@
+// Attention on the window-and-sinks and shared-prefix patterns by fused multiply-adds in 32 bits: every type and every head
+// dimension that is a multiple of 4 up to 256.  What 16-bit operands of common shapes run on is in rode_attention_tiles.cu
+// and rode_attention_step.cu; single precision stays here, because a tensor core would round its operands to 11 bits.
+//
+// One pass over the keys with the running maximum m and sum l of the softmax: scores of a tile in base 2 (scale * log2 e
+// folded into the queries' products), m' = max(m, max s), the accumulator times 2^(m - m'), plus 2^(s - m') V.
+//
+// A CTA of 256 threads works on 64 rows x 64 keys (32 x 32 at head dimensions above 128, where the operands' tiles would not fit
+// the shared memory); a thread holds 4 x 4 scores and 4 rows x dim / 16 columns of the result, so that eight 16-byte
+// loads from shared memory feed 64 FMAs.  Rows of shared memory are 4 floats longer than the tile: eight threads that read one
+// column of eight keys hit different banks.
+#include "rode_attention.cuh"
+
+namespace rode {
+namespace {
+
+constexpr int kThreads = 256;
+
+template <int kDim>
+constexpr int tile_rows() {
+    return kDim <= 128 ? 64 : 32;
+}
+
+// rows x kDim floats, columns beyond dim and rows beyond `have` zero.
+template <typename T, int kDim>
+__device__ __forceinline__ void fetch_tile(float *dst, const T *src, long long stride, int have, int dim) {
+    constexpr int kRows = tile_rows<kDim>();
+    for (int i = threadIdx.x; i < kRows * (kDim / 4); i += kThreads) {
+        const int r = i / (kDim / 4), c = i % (kDim / 4) * 4;
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (r < have && c < dim) x = load4(src + r * stride + c);
+        *reinterpret_cast<float4 *>(dst + r * (kDim + 4) + c) = x;
+    }
+}
+
+// acc[i][j] = a[row i] . b[row j] for rows ty * R + i and tx + 16 * j
+template <int kDim, int R>
+__device__ __forceinline__ void dot_tile(const float *a, const float *b, int dim, float (&acc)[R][R]) {
+    const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+        for (int j = 0; j < R; ++j) acc[i][j] = 0.f;
+    for (int d = 0; d < dim; d += 4) {
+        float4 x[R], y[R];
+#pragma unroll
+        for (int i = 0; i < R; ++i) x[i] = *reinterpret_cast<const float4 *>(a + (ty * R + i) * (kDim + 4) + d);
+#pragma unroll
+        for (int j = 0; j < R; ++j) y[j] = *reinterpret_cast<const float4 *>(b + (tx + 16 * j) * (kDim + 4) + d);
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+#pragma unroll
+            for (int j = 0; j < R; ++j) {
+                acc[i][j] = fmaf(x[i].x, y[j].x, acc[i][j]);
+                acc[i][j] = fmaf(x[i].y, y[j].y, acc[i][j]);
+                acc[i][j] = fmaf(x[i].z, y[j].z, acc[i][j]);
+                acc[i][j] = fmaf(x[i].w, y[j].w, acc[i][j]);
+            }
+    }
+}
+
+// acc[i][c] += sum over n of w[ty * R + i][n] * x[n][(tx + 16 * c) * 4 ..]; w has rows of kRows + 4 floats
+template <int kDim, int R>
+__device__ __forceinline__ void weigh_rows(const float *w, const float *x, float4 (&acc)[R][kDim / 64]) {
+    constexpr int kRows = tile_rows<kDim>();
+    const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
+    for (int n = 0; n < kRows; n += 4) {
+        float4 p[R];
+#pragma unroll
+        for (int i = 0; i < R; ++i) p[i] = *reinterpret_cast<const float4 *>(w + (ty * R + i) * (kRows + 4) + n);
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int c = 0; c < kDim / 64; ++c) {
+                const float4 y = *reinterpret_cast<const float4 *>(x + (n + u) * (kDim + 4) + (tx + 16 * c) * 4);
+#pragma unroll
+                for (int i = 0; i < R; ++i) vfma(acc[i][c], reinterpret_cast<const float *>(&p[i])[u], y);
+            }
+    }
+}
+
+// Maximum and sum over the 16 threads that share a row.
+__device__ __forceinline__ float row_max(float x) {
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+    return x;
+}
+__device__ __forceinline__ float row_sum(float x) {
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+    return x;
+}
+
+// The running softmax of one tile's scores: s becomes the weights, which go to `weights` for weigh_rows.
+template <int kDim, int R>
+__device__ __forceinline__ void softmax_tile(float (&s)[R][R], float (&m)[R], float (&l)[R], float4 (&acc)[R][kDim / 64],
+                                             float *weights) {
+    constexpr int kRows = tile_rows<kDim>();
+    const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        float top = s[i][0];
+#pragma unroll
+        for (int j = 1; j < R; ++j) top = fmaxf(top, s[i][j]);
+        const float next = fmaxf(m[i], row_max(top));
+        const float base = next == -INFINITY ? 0.f : next;  // a row that has seen no key: all weights 0, not NaN
+        const float keep = exp2f(m[i] - base);
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+            s[i][j] = exp2f(s[i][j] - base);
+            sum += s[i][j];
+            weights[(ty * R + i) * (kRows + 4) + tx + 16 * j] = s[i][j];
+        }
+        l[i] = l[i] * keep + row_sum(sum);
+        m[i] = next;
+#pragma unroll
+        for (int c = 0; c < kDim / 64; ++c) {
+            acc[i][c].x *= keep;
+            acc[i][c].y *= keep;
+            acc[i][c].z *= keep;
+            acc[i][c].w *= keep;
+        }
+    }
+}
+
+template <int kDim>
+constexpr int forward_shared() {
+    return 4 * (3 * tile_rows<kDim>() * (kDim + 4) + tile_rows<kDim>() * (tile_rows<kDim>() + 4));
+}
+
+// One tile of a sequence's queries, one head.
+template <typename T, int kDim>
+__global__ void __launch_bounds__(kThreads) prompt_rows(Prompt p) {
+    constexpr int kRows = tile_rows<kDim>(), R = kRows / 16;
+    extern __shared__ float4 shared4[];
+    float *qs = reinterpret_cast<float *>(shared4), *ks = qs + kRows * (kDim + 4), *vs = ks + kRows * (kDim + 4),
+          *ws = vs + kRows * (kDim + 4);
+    const Window &w = p.win;
+    const int head = blockIdx.y, kv = head / (w.heads / w.kv_heads);
+    const Tile t = find_tile(p.seqs.q_offsets, p.seqs.n_seq, p.seqs.q_rows, blockIdx.x, kRows);
+    if (t.first < 0 || t.first >= t.rows || (t.seq < 0 && !p.clear)) return;
+    const int2 keys = t.seq < 0 ? make_int2(0, 0) : sequence_rows(p.seqs.k_offsets, p.seqs.k_rows, t.seq);
+    const int have = min(kRows, t.rows - t.first);
+    const long long row0 = static_cast<long long>(t.row0) + t.first;
+    const int pos0 = t.first + keys.y - t.rows;  // position of the tile's first query
+    fetch_tile<T, kDim>(qs, row_of<T>(p.q, 0, row0, head), p.q.row, have, w.dim);
+
+    float m[R], l[R];
+    float4 acc[R][kDim / 64];
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        m[i] = -INFINITY;
+        l[i] = 0.f;
+#pragma unroll
+        for (int c = 0; c < kDim / 64; ++c) acc[i][c] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
+    const KeyBlocks blocks(pos0, pos0 + have, w.window, w.sinks, kRows);
+    for (int b = 0; b < blocks.n; ++b) {
+        const int k0 = blocks.at(b) * kRows, n = min(kRows, keys.y - k0);
+        __syncthreads();
+        fetch_tile<T, kDim>(ks, row_of<T>(p.k, 0, keys.x + k0, kv), p.k.row, n, w.dim);
+        fetch_tile<T, kDim>(vs, row_of<T>(p.v, 0, keys.x + k0, kv), p.v.row, n, w.dim);
+        __syncthreads();
+        float s[R][R];
+        dot_tile<kDim, R>(qs, ks, w.dim, s);
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+#pragma unroll
+            for (int j = 0; j < R; ++j)
+                s[i][j] = sees(pos0 + ty * R + i, k0 + tx + 16 * j, w.window, w.sinks) ? s[i][j] * (w.scale * kLog2e) : -INFINITY;
+        softmax_tile<kDim, R>(s, m, l, acc, ws);
+        __syncthreads();
+        weigh_rows<kDim, R>(ws, vs, acc);
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        const int r = ty * R + i;
+        if (r >= have) continue;
+        const float inv = l[i] > 0.f || l[i] != l[i] ? 1.f / l[i] : 0.f;
+        T *out = static_cast<T *>(p.out) + ((row0 + r) * w.heads + head) * w.dim;
+#pragma unroll
+        for (int c = 0; c < kDim / 64; ++c) {
+            const int d = (tx + 16 * c) * 4;
+            if (d < w.dim)
+                store4(out + d, make_float4(acc[i][c].x * inv, acc[i][c].y * inv, acc[i][c].z * inv, acc[i][c].w * inv));
+        }
+        if (tx == 0 && p.lse != nullptr)
+            p.lse[static_cast<long long>(head) * p.seqs.q_rows + row0 + r] = m[i] == -INFINITY ? -INFINITY : (m[i] + log2f(l[i])) * kLn2;
+    }
+}
+
+// Queries of all requests that share a key head, row r = request r / group, head r % group of the group, against a part of the prefix.
+template <typename T, int kDim>
+__global__ void __launch_bounds__(kThreads) shared_rows(Cached c, int first_split, int splits) {
+    constexpr int kRows = tile_rows<kDim>(), R = kRows / 16;
+    extern __shared__ float4 shared4[];
+    float *qs = reinterpret_cast<float *>(shared4), *ks = qs + kRows * (kDim + 4), *vs = ks + kRows * (kDim + 4),
+          *ws = vs + kRows * (kDim + 4);
+    const Window &w = c.win;
+    const int kv = blockIdx.y, group = w.heads / w.kv_heads, split = blockIdx.z;
+    const int row0 = blockIdx.x * kRows, have = min(kRows, c.batch * group - row0);
+    for (int i = threadIdx.x; i < kRows * (kDim / 4); i += kThreads) {
+        const int r = i / (kDim / 4), d = i % (kDim / 4) * 4;
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (r < have && d < w.dim) x = load4(row_of<T>(c.q, (row0 + r) / group, 0, kv * group + (row0 + r) % group) + d);
+        *reinterpret_cast<float4 *>(qs + r * (kDim + 4) + d) = x;
+    }
+    float m[R], l[R];
+    float4 acc[R][kDim / 64];
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        m[i] = -INFINITY;
+        l[i] = 0.f;
+#pragma unroll
+        for (int d = 0; d < kDim / 64; ++d) acc[i][d] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
+    const int blocks = (c.prefix + kRows - 1) / kRows;
+    const int b1 = static_cast<int>(static_cast<long long>(blocks) * (split + 1) / splits);
+    for (int b = static_cast<int>(static_cast<long long>(blocks) * split / splits); b < b1; ++b) {
+        const int k0 = b * kRows, n = min(kRows, c.prefix - k0);
+        __syncthreads();
+        fetch_tile<T, kDim>(ks, row_of<T>(c.pk, 0, k0, kv), c.pk.row, n, w.dim);
+        fetch_tile<T, kDim>(vs, row_of<T>(c.pv, 0, k0, kv), c.pv.row, n, w.dim);
+        __syncthreads();
+        float s[R][R];
+        dot_tile<kDim, R>(qs, ks, w.dim, s);
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+#pragma unroll
+            for (int j = 0; j < R; ++j) s[i][j] = tx + 16 * j < n ? s[i][j] * (w.scale * kLog2e) : -INFINITY;
+        softmax_tile<kDim, R>(s, m, l, acc, ws);
+        __syncthreads();
+        weigh_rows<kDim, R>(ws, vs, acc);
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        const int r = row0 + ty * R + i;
+        if (ty * R + i >= have) continue;
+        const float inv = l[i] > 0.f || l[i] != l[i] ? 1.f / l[i] : 0.f;
+        const long long at = (static_cast<long long>(first_split + split) * c.batch + r / group) * w.heads + kv * group + r % group;
+#pragma unroll
+        for (int d4 = 0; d4 < kDim / 64; ++d4) {
+            const int d = (tx + 16 * d4) * 4;
+            if (d < w.dim)
+                store4(c.part_out + at * w.dim + d,
+                       make_float4(acc[i][d4].x * inv, acc[i][d4].y * inv, acc[i][d4].z * inv, acc[i][d4].w * inv));
+        }
+        if (tx == 0) c.part_lse[at] = m[i] == -INFINITY ? -INFINITY : m[i] + log2f(l[i]);
+    }
+}
+
+template <int kDim>
+constexpr int backward_shared() {
+    return 4 * (4 * tile_rows<kDim>() * (kDim + 4) + 2 * tile_rows<kDim>() * (tile_rows<kDim>() + 4) + 2 * tile_rows<kDim>());
+}
+
+// Weights P and score gradients dS = P (dP - delta) of a tile from s = q.k and dp = do.v.  Rows that saw no key have lse = -inf, but
+// no visible key either.
+template <int R>
+__device__ __forceinline__ void score_gradients(float (&s)[R][R], float (&dp)[R][R], const float *lse2, const float *delta, int pos0,
+                                                int have, int k0, const Window &w) {
+    const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+            const int r = ty * R + i;
+            const bool on = r < have && sees(pos0 + r, k0 + tx + 16 * j, w.window, w.sinks);
+            s[i][j] = on ? exp2f(s[i][j] * (w.scale * kLog2e) - lse2[r]) : 0.f;
+            dp[i][j] = on ? s[i][j] * (dp[i][j] - delta[r]) : 0.f;
+        }
+}
+
+// Gradient of one tile of queries, one head; also delta = do . o of its rows, for key_gradients.
+template <typename T, int kDim>
+__global__ void __launch_bounds__(kThreads) query_gradients(Prompt p) {
+    constexpr int kRows = tile_rows<kDim>(), R = kRows / 16, kTile = kRows * (kDim + 4);
+    extern __shared__ float4 shared4[];
+    float *qs = reinterpret_cast<float *>(shared4), *gs = qs + kTile, *ks = gs + kTile, *vs = ks + kTile, *ds = vs + kTile,
+          *lse2 = ds + 2 * kRows * (kRows + 4), *delta = lse2 + kRows;
+    const Window &w = p.win;
+    const int head = blockIdx.y, kv = head / (w.heads / w.kv_heads);
+    const Tile t = find_tile(p.seqs.q_offsets, p.seqs.n_seq, p.seqs.q_rows, blockIdx.x, kRows);
+    if (t.first < 0 || t.first >= t.rows || (t.seq < 0 && !p.clear)) return;
+    const int2 keys = t.seq < 0 ? make_int2(0, 0) : sequence_rows(p.seqs.k_offsets, p.seqs.k_rows, t.seq);
+    const int have = min(kRows, t.rows - t.first);
+    const long long row0 = static_cast<long long>(t.row0) + t.first;
+    const int pos0 = t.first + keys.y - t.rows;
+    const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
+    fetch_tile<T, kDim>(qs, row_of<T>(p.q, 0, row0, head), p.q.row, have, w.dim);
+    fetch_tile<T, kDim>(gs, row_of<T>(p.dout, 0, row0, head), p.dout.row, have, w.dim);
+    __syncthreads();
+    for (int r = ty; r < kRows; r += 16) {
+        float sum = 0.f;
+        if (r < have) {
+            const T *o = static_cast<const T *>(p.out) + ((row0 + r) * w.heads + head) * w.dim;
+            for (int d = tx * 4; d < w.dim; d += 64) {
+                const float4 x = load4(o + d), g = *reinterpret_cast<const float4 *>(gs + r * (kDim + 4) + d);
+                sum += x.x * g.x + x.y * g.y + x.z * g.z + x.w * g.w;
+            }
+        }
+        sum = row_sum(sum);
+        if (tx == 0) {
+            const long long at = static_cast<long long>(head) * p.seqs.q_rows + row0 + r;
+            delta[r] = sum;
+            lse2[r] = r < have ? p.lse[at] * kLog2e : 0.f;
+            if (r < have) p.delta[at] = sum;
+        }
+    }
+    float4 acc[R][kDim / 64];
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+        for (int c = 0; c < kDim / 64; ++c) acc[i][c] = make_float4(0.f, 0.f, 0.f, 0.f);
+    const KeyBlocks blocks(pos0, pos0 + have, w.window, w.sinks, kRows);
+    for (int b = 0; b < blocks.n; ++b) {
+        const int k0 = blocks.at(b) * kRows, n = min(kRows, keys.y - k0);
+        __syncthreads();
+        fetch_tile<T, kDim>(ks, row_of<T>(p.k, 0, keys.x + k0, kv), p.k.row, n, w.dim);
+        fetch_tile<T, kDim>(vs, row_of<T>(p.v, 0, keys.x + k0, kv), p.v.row, n, w.dim);
+        __syncthreads();
+        float s[R][R], dp[R][R];
+        dot_tile<kDim, R>(qs, ks, w.dim, s);
+        dot_tile<kDim, R>(gs, vs, w.dim, dp);
+        score_gradients<R>(s, dp, lse2, delta, pos0, have, k0, w);
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+#pragma unroll
+            for (int j = 0; j < R; ++j) ds[(ty * R + i) * (kRows + 4) + tx + 16 * j] = dp[i][j];
+        __syncthreads();
+        weigh_rows<kDim, R>(ds, ks, acc);
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        const int r = ty * R + i;
+        if (r >= have) continue;
+        T *out = static_cast<T *>(p.dq) + ((row0 + r) * w.heads + head) * w.dim;
+#pragma unroll
+        for (int c = 0; c < kDim / 64; ++c) {
+            const int d = (tx + 16 * c) * 4;
+            if (d < w.dim)
+                store4(out + d, make_float4(acc[i][c].x * w.scale, acc[i][c].y * w.scale, acc[i][c].z * w.scale,
+                                            acc[i][c].w * w.scale));
+        }
+    }
+}
+
+// Gradients of one tile of keys and values, one key head: the queries of all its heads, one after the other, so that the sum
+// over a group has one order.
+template <typename T, int kDim>
+__global__ void __launch_bounds__(kThreads) key_gradients(Prompt p) {
+    constexpr int kRows = tile_rows<kDim>(), R = kRows / 16, kTile = kRows * (kDim + 4);
+    extern __shared__ float4 shared4[];
+    float *qs = reinterpret_cast<float *>(shared4), *gs = qs + kTile, *ks = gs + kTile, *vs = ks + kTile, *pt = vs + kTile,
+          *dt = pt + kRows * (kRows + 4), *lse2 = dt + kRows * (kRows + 4), *delta = lse2 + kRows;
+    const Window &w = p.win;
+    const int kv = blockIdx.y, group = w.heads / w.kv_heads;
+    const int *offsets = p.seqs.k_offsets;
+    const Tile t = find_tile(offsets, p.seqs.n_seq, p.seqs.k_rows, blockIdx.x, kRows);
+    if (t.first < 0 || t.first >= t.rows || (t.seq < 0 && !p.clear)) return;
+    const int2 queries = t.seq < 0 ? make_int2(0, 0) : sequence_rows(p.seqs.q_offsets, p.seqs.q_rows, t.seq);
+    const int have = min(kRows, t.rows - t.first);
+    const long long row0 = static_cast<long long>(t.row0) + t.first;
+    const int shift = t.rows - queries.y;  // position of the first query
+    const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
+    fetch_tile<T, kDim>(ks, row_of<T>(p.k, 0, row0, kv), p.k.row, have, w.dim);
+    fetch_tile<T, kDim>(vs, row_of<T>(p.v, 0, row0, kv), p.v.row, have, w.dim);
+    float4 dk[R][kDim / 64], dv[R][kDim / 64];
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+        for (int c = 0; c < kDim / 64; ++c) dk[i][c] = dv[i][c] = make_float4(0.f, 0.f, 0.f, 0.f);
+    // queries at positions from the tile's first key to the end of its last key's window (sinks: to the end)
+    const int last = t.first < w.sinks || w.window >= t.rows - (t.first + have - 1) ? t.rows : t.first + have - 1 + w.window;
+    const int i0 = max(t.first - shift, 0) / kRows * kRows, i1 = min(last - shift, queries.y);
+    for (int h = kv * group; h < (kv + 1) * group; ++h)
+        for (int i = i0; i < i1; i += kRows) {
+            const int n = min(kRows, queries.y - i);
+            const long long q0 = static_cast<long long>(queries.x) + i;
+            __syncthreads();
+            fetch_tile<T, kDim>(qs, row_of<T>(p.q, 0, q0, h), p.q.row, n, w.dim);
+            fetch_tile<T, kDim>(gs, row_of<T>(p.dout, 0, q0, h), p.dout.row, n, w.dim);
+            if (threadIdx.x < kRows) {
+                const long long at = static_cast<long long>(h) * p.seqs.q_rows + q0 + threadIdx.x;
+                const bool in = static_cast<int>(threadIdx.x) < n;
+                lse2[threadIdx.x] = in ? p.lse[at] * kLog2e : 0.f;
+                delta[threadIdx.x] = in ? p.delta[at] : 0.f;
+            }
+            __syncthreads();
+            float s[R][R], dp[R][R];
+            dot_tile<kDim, R>(qs, ks, w.dim, s);
+            dot_tile<kDim, R>(gs, vs, w.dim, dp);
+            score_gradients<R>(s, dp, lse2, delta, shift + i, n, t.first, w);
+#pragma unroll
+            for (int a = 0; a < R; ++a)
+#pragma unroll
+                for (int j = 0; j < R; ++j) {
+                    pt[(tx + 16 * j) * (kRows + 4) + ty * R + a] = s[a][j];
+                    dt[(tx + 16 * j) * (kRows + 4) + ty * R + a] = dp[a][j];
+                }
+            __syncthreads();
+            weigh_rows<kDim, R>(pt, gs, dv);
+            weigh_rows<kDim, R>(dt, qs, dk);
+        }
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        const int r = ty * R + i;
+        if (r >= have) continue;
+        const long long at = ((row0 + r) * w.kv_heads + kv) * w.dim;
+#pragma unroll
+        for (int c = 0; c < kDim / 64; ++c) {
+            const int d = (tx + 16 * c) * 4;
+            if (d >= w.dim) continue;
+            store4(static_cast<T *>(p.dk) + at + d,
+                   make_float4(dk[i][c].x * w.scale, dk[i][c].y * w.scale, dk[i][c].z * w.scale, dk[i][c].w * w.scale));
+            store4(static_cast<T *>(p.dv) + at + d, dv[i][c]);
+        }
+    }
+}
+
+// --- single tokens -------------------------------------------------------------------------------------------------------------
+
+// One request's queries of a key head (eight of them at a time) against a part of the keys that they see, which is the same for
+// all of them: key i of the list is key i of the cache for the sinks, then the window's.
+constexpr int kStepThreads = 128, kStepKeys = 32, kStepQueries = 8;
+
+template <typename T, int kDim>
+__global__ void __launch_bounds__(kStepThreads) step_rows(Cached c, int first_split, int splits) {
+    constexpr int kQuads = kDim / 4, kGroups = kStepThreads / kQuads, kPer = kStepQueries / kGroups;
+    extern __shared__ float4 shared4[];
+    float *ks = reinterpret_cast<float *>(shared4), *vs = ks + kStepKeys * (kDim + 4), *qs = vs + kStepKeys * (kDim + 4),
+          *ws = qs + kStepQueries * (kDim + 4), *keeps = ws + kStepQueries * kStepKeys, *sums = keeps + kStepQueries;
+    const Window &w = c.win;
+    const int b = blockIdx.x, split = blockIdx.z, group = w.heads / w.kv_heads;
+    const int chunks = (group + kStepQueries - 1) / kStepQueries, kv = blockIdx.y / chunks;
+    const int g0 = blockIdx.y % chunks * kStepQueries, have = min(kStepQueries, group - g0), head0 = kv * group + g0;
+    const int n = min(max(__ldg(c.lengths + b), 0), c.capacity);
+    const int lo = max(n - w.window, 0), sinks = min(w.sinks, lo), seen = sinks + n - lo;
+    const int part = ((seen + splits - 1) / splits + kStepKeys - 1) / kStepKeys * kStepKeys;
+    const int begin = static_cast<int>(min(static_cast<long long>(part) * split, static_cast<long long>(seen)));
+    const int end = min(begin + part, seen);
+    const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+    for (int i = tid; i < kStepQueries * kQuads; i += kStepThreads) {
+        const int r = i / kQuads, d = i % kQuads * 4;
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (r < have && d < w.dim) x = load4(row_of<T>(c.q, b, 0, head0 + r) + d);
+        *reinterpret_cast<float4 *>(qs + r * (kDim + 4) + d) = x;
+    }
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};  // of queries 2 * warp and 2 * warp + 1, in every lane
+    float4 acc[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    const int d0 = tid % kQuads * 4, r0 = tid / kQuads * kPer;
+    for (int k0 = begin; k0 < end; k0 += kStepKeys) {
+        const int keys = min(kStepKeys, end - k0);
+        __syncthreads();
+        for (int i = tid; i < kStepKeys * kQuads; i += kStepThreads) {
+            const int r = i / kQuads, d = i % kQuads * 4;
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
+            if (r < keys && d < w.dim) {
+                const int j = k0 + r < sinks ? k0 + r : k0 + r - sinks + lo;
+                x = load4(row_of<T>(c.k, b, j, kv) + d);
+                y = load4(row_of<T>(c.v, b, j, kv) + d);
+            }
+            *reinterpret_cast<float4 *>(ks + r * (kDim + 4) + d) = x;
+            *reinterpret_cast<float4 *>(vs + r * (kDim + 4) + d) = y;
+        }
+        __syncthreads();
+        {
+            const int key = tid / 4, r = tid % 4 * 2;
+            float s0 = 0.f, s1 = 0.f;
+            for (int d = 0; d < w.dim; d += 4) {
+                const float4 x = *reinterpret_cast<const float4 *>(ks + key * (kDim + 4) + d);
+                const float4 y = *reinterpret_cast<const float4 *>(qs + r * (kDim + 4) + d);
+                const float4 z = *reinterpret_cast<const float4 *>(qs + (r + 1) * (kDim + 4) + d);
+                s0 = fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, fmaf(x.w, y.w, s0))));
+                s1 = fmaf(x.x, z.x, fmaf(x.y, z.y, fmaf(x.z, z.z, fmaf(x.w, z.w, s1))));
+            }
+            const bool in = key < keys;
+            ws[r * kStepKeys + key] = in ? s0 * (w.scale * kLog2e) : -INFINITY;
+            ws[(r + 1) * kStepKeys + key] = in ? s1 * (w.scale * kLog2e) : -INFINITY;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int r = 2 * warp + u;
+            const float s = ws[r * kStepKeys + lane];
+            float top = s;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            const float next = fmaxf(m[u], top), base = next == -INFINITY ? 0.f : next;
+            const float keep = exp2f(m[u] - base), e = exp2f(s - base);
+            float sum = e;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            l[u] = l[u] * keep + sum;
+            m[u] = next;
+            ws[r * kStepKeys + lane] = e;
+            if (lane == 0) keeps[r] = keep;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const float keep = keeps[r0 + i];
+            acc[i].x *= keep;
+            acc[i].y *= keep;
+            acc[i].z *= keep;
+            acc[i].w *= keep;
+        }
+        for (int key = 0; key < kStepKeys; ++key) {
+            const float4 y = *reinterpret_cast<const float4 *>(vs + key * (kDim + 4) + d0);
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) vfma(acc[i], ws[(r0 + i) * kStepKeys + key], y);
+        }
+    }
+    if (lane == 0) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int r = 2 * warp + u;
+            sums[r] = l[u];
+            if (c.part_out != nullptr && r < have)
+                c.part_lse[(static_cast<long long>(first_split + split) * c.batch + b) * w.heads + head0 + r] =
+                    m[u] == -INFINITY ? -INFINITY : m[u] + log2f(l[u]);
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int r = r0 + i;
+        if (r >= have || d0 >= w.dim) continue;
+        const float inv = sums[r] > 0.f || sums[r] != sums[r] ? 1.f / sums[r] : 0.f;
+        const float4 x = make_float4(acc[i].x * inv, acc[i].y * inv, acc[i].z * inv, acc[i].w * inv);
+        const long long at = static_cast<long long>(b) * w.heads + head0 + r;
+        if (c.part_out != nullptr)
+            store4(c.part_out + (static_cast<long long>(first_split + split) * c.batch * w.heads + at) * w.dim + d0, x);
+        else
+            store4(static_cast<T *>(c.out) + at * w.dim + d0, x);
+    }
+}
+
+template <int kDim>
+constexpr int step_shared() {
+    return 4 * ((2 * kStepKeys + kStepQueries) * (kDim + 4) + kStepQueries * kStepKeys + 2 * kStepQueries);
+}
+
+// Joins the parts of every row: weights 2^(lse - max lse).  A warp per row.
+template <typename T>
+__global__ void __launch_bounds__(128) join_rows(Cached c, int splits) {
+    const long long rows = static_cast<long long>(c.batch) * c.win.heads, row = blockIdx.x * 4ll + threadIdx.x / 32;
+    if (row >= rows) return;
+    const int lane = threadIdx.x % 32, dim = c.win.dim;
+    const float *lse = c.part_lse + row;
+    const float *part = c.part_out + row * dim;
+    float top = -INFINITY, sum = 0.f;
+    for (int s = lane; s < splits; s += 32) top = fmaxf(top, lse[s * rows]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (top == -INFINITY) top = 0.f;
+    for (int s = lane; s < splits; s += 32) sum += exp2f(lse[s * rows] - top);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+    for (int d = lane * 4; d < dim; d += 128) {
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int s = 0; s < splits; ++s) {
+            const float x = exp2f(lse[s * rows] - top);
+            // (a part without keys has no weight, whatever its rows hold)
+            if (x != 0.f) vfma(acc, x * inv, *reinterpret_cast<const float4 *>(part + s * rows * dim + d));
+        }
+        store4(static_cast<T *>(c.out) + row * dim + d, acc);
+    }
+}
+
+template <typename F>
+int by_type(int dtype, F &&f) {
+    if (dtype == RODE_F32) return f(static_cast<float *>(nullptr));
+    if (dtype == RODE_F16) return f(static_cast<__half *>(nullptr));
+    return f(static_cast<__nv_bfloat16 *>(nullptr));
+}
+template <typename F>
+int by_dim(int dim, F &&f) {
+    if (dim <= 64) return f(std::integral_constant<int, 64>());
+    if (dim <= 128) return f(std::integral_constant<int, 128>());
+    return f(std::integral_constant<int, 256>());
+}
+
+}  // namespace
+
+int simple_prompt(int dtype, const Prompt &p, cudaStream_t stream) {
+    return by_type(dtype, [&](auto *type) {
+        return by_dim(p.win.dim, [&](auto dim) {
+            using T = std::remove_pointer_t<decltype(type)>;
+            constexpr int kDim = decltype(dim)::value;
+            auto *kernel = &prompt_rows<T, kDim>;
+            if (const int e = allow_shared(kernel, forward_shared<kDim>())) return e;
+            const int slots = tile_slots(p.seqs.q_offsets, p.seqs.n_seq, p.seqs.q_rows, tile_rows<kDim>());
+            kernel<<<dim3(slots, p.win.heads), kThreads, forward_shared<kDim>(), stream>>>(p);
+            RODE_CHECK_LAUNCH("prompt_rows");
+            return static_cast<int>(RODE_OK);
+        });
+    });
+}
+
+int simple_prompt_backward(int dtype, const Prompt &p, cudaStream_t stream) {
+    return by_type(dtype, [&](auto *type) {
+        return by_dim(p.win.dim, [&](auto dim) {
+            using T = std::remove_pointer_t<decltype(type)>;
+            constexpr int kDim = decltype(dim)::value;
+            auto *kernel = &query_gradients<T, kDim>;
+            auto *kernel2 = &key_gradients<T, kDim>;
+            if (const int e = allow_shared(kernel, backward_shared<kDim>())) return e;
+            if (const int e = allow_shared(kernel2, backward_shared<kDim>())) return e;
+            const int slots = tile_slots(p.seqs.q_offsets, p.seqs.n_seq, p.seqs.q_rows, tile_rows<kDim>());
+            if (slots > 0) kernel<<<dim3(slots, p.win.heads), kThreads, backward_shared<kDim>(), stream>>>(p);
+            RODE_CHECK_LAUNCH("query_gradients");
+            const int k_slots = tile_slots(p.seqs.k_offsets, p.seqs.n_seq, p.seqs.k_rows, tile_rows<kDim>());
+            if (p.dk != nullptr && k_slots > 0) kernel2<<<dim3(k_slots, p.win.kv_heads), kThreads, backward_shared<kDim>(), stream>>>(p);
+            RODE_CHECK_LAUNCH("key_gradients");
+            return static_cast<int>(RODE_OK);
+        });
+    });
+}
+
+int simple_shared(int dtype, const Cached &c, int first_split, int splits, cudaStream_t stream) {
+    return by_type(dtype, [&](auto *type) {
+        return by_dim(c.win.dim, [&](auto dim) {
+            using T = std::remove_pointer_t<decltype(type)>;
+            constexpr int kDim = decltype(dim)::value;
+            auto *kernel = &shared_rows<T, kDim>;
+            if (const int e = allow_shared(kernel, forward_shared<kDim>())) return e;
+            const long long rows = static_cast<long long>(c.batch) * (c.win.heads / c.win.kv_heads);
+            const int tiles = static_cast<int>((rows + tile_rows<kDim>() - 1) / tile_rows<kDim>());
+            kernel<<<dim3(tiles, c.win.kv_heads, splits), kThreads, forward_shared<kDim>(), stream>>>(c, first_split, splits);
+            RODE_CHECK_LAUNCH("shared_rows");
+            return static_cast<int>(RODE_OK);
+        });
+    });
+}
+
+int simple_step(int dtype, const Cached &c, int first_split, int splits, cudaStream_t stream) {
+    return by_type(dtype, [&](auto *type) {
+        return by_dim(c.win.dim, [&](auto dim) {
+            using T = std::remove_pointer_t<decltype(type)>;
+            constexpr int kDim = decltype(dim)::value;
+            auto *kernel = &step_rows<T, kDim>;
+            if (const int e = allow_shared(kernel, step_shared<kDim>())) return e;
+            const int chunks = (c.win.heads / c.win.kv_heads + kStepQueries - 1) / kStepQueries;
+            kernel<<<dim3(c.batch, c.win.kv_heads * chunks, splits), kStepThreads, step_shared<kDim>(), stream>>>(c, first_split,
+                                                                                                                  splits);
+            RODE_CHECK_LAUNCH("step_rows");
+            return static_cast<int>(RODE_OK);
+        });
+    });
+}
+
+int join_parts(int dtype, const Cached &c, int splits, cudaStream_t stream) {
+    return by_type(dtype, [&](auto *type) {
+        using T = std::remove_pointer_t<decltype(type)>;
+        const long long rows = static_cast<long long>(c.batch) * c.win.heads;
+        join_rows<T><<<static_cast<unsigned>((rows + 3) / 4), 128, 0, stream>>>(c, splits);
+        RODE_CHECK_LAUNCH("join_rows");
+        return static_cast<int>(RODE_OK);
+    });
+}
+
+}  // namespace rode

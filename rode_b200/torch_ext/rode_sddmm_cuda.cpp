@@ -30,6 +30,8 @@
 
 #include "rode_b200.h"
 
+void bind_attention(pybind11::module_ &m);  // rode_attention.cpp
+
 namespace {
 
 #define RODE_CHECK_CUDA(x) TORCH_CHECK((x).device().is_cuda(), #x " must be a CUDA tensor")
@@ -287,4 +289,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           py::arg("hot_columns") = py::none(), py::arg("ordered") = false);
     m.def("hot_columns", &py_hot_columns, "Column popularity bitmap for spmm_forward, or None (CUDA)",
           py::arg("column_indices"), py::arg("n_cols"), py::arg("dense_row_bytes"), py::arg("budget_bytes") = 0);
+    bind_attention(m);
 }
