@@ -364,6 +364,11 @@ int rode_shared_prefix_attention(int dtype, int batch, int prefix, int capacity,
                                  const int *lengths, void *out, void *workspace, size_t workspace_bytes,
                                  rode_stream_t stream);
 
+/* The tensor-core kernels give up a wait between their warps after some seconds instead of hanging.  *failed (host) becomes 1 if that
+ * ever happened on the current device (an error of this library; the results of that call are wrong), else 0.  Synchronises the
+ * device. */
+int rode_attention_waits_failed(int *failed);
+
 #ifdef __cplusplus
 }
 #endif

@@ -35,6 +35,7 @@ C_ABI_SYMBOLS = (
     "rode_window_attention", "rode_window_attention_backward_workspace_bytes", "rode_window_attention_backward",
     "rode_window_attention_step_workspace_bytes", "rode_window_attention_step",
     "rode_shared_prefix_attention_workspace_bytes", "rode_shared_prefix_attention",
+    "rode_attention_waits_failed",
 )
 # Itanium-ABI names of the C++ entry points declared in RoDeSpmm.h / RoDeSddmm.h /
 # RoDePreprocess.h; identical to the names the reference's own objects export.
@@ -116,6 +117,7 @@ def load() -> ctypes.CDLL:
     lib.rode_window_attention_step.argtypes = [ci] * 8 + [cf] + [heads] * 3 + [vp] * 3 + [sz, vp]
     lib.rode_shared_prefix_attention_workspace_bytes.argtypes = [ci] * 6 + [ctypes.POINTER(sz)]
     lib.rode_shared_prefix_attention.argtypes = [ci] * 7 + [cf] + [heads] * 5 + [vp] * 3 + [sz, vp]
+    lib.rode_attention_waits_failed.argtypes = [ctypes.POINTER(ci)]
     for name in ("rode_preprocess_workspace_bytes", "rode_preprocess_capacity", "rode_preprocess",
                  "rode_preprocess_noalloc", "rode_preprocess_cpu", "rode_spmm_workspace_bytes", "rode_spmm_f32", "rode_spmm_f64",
                  "rode_sddmm_f32", "rode_hot_columns_workspace_bytes", "rode_hot_columns_words", "rode_hot_columns",
@@ -124,7 +126,7 @@ def load() -> ctypes.CDLL:
                  "rode_spmm_order_pays", "rode_spmm_ordered_workspace_bytes", "rode_spmm_f32_ordered", "rode_spmm_f64_ordered",
                  "rode_window_attention", "rode_window_attention_backward_workspace_bytes", "rode_window_attention_backward",
                  "rode_window_attention_step_workspace_bytes", "rode_window_attention_step",
-                 "rode_shared_prefix_attention_workspace_bytes", "rode_shared_prefix_attention"):
+                 "rode_shared_prefix_attention_workspace_bytes", "rode_shared_prefix_attention", "rode_attention_waits_failed"):
         getattr(lib, name).restype = ci
     _lib = lib
     return lib

@@ -1,4 +1,6 @@
 // C entry points of the attention operators: argument checks, workspaces, which kernels a call runs on.
+#include <algorithm>
+
 #include "rode_attention.cuh"
 
 namespace rode {
@@ -91,7 +93,12 @@ Parts plan_parts(int batch, int prefix, long long seen, int heads, int kv_heads,
     if (batch == 0) return p;
     const int group = heads / kv_heads;
     p.own = parts_of(static_cast<long long>(batch) * kv_heads * ((group + 7) / 8), seen);
-    if (prefix > 0) p.prefix = parts_of((static_cast<long long>(batch) * group + 63) / 64 * kv_heads, prefix);
+    if (prefix > 0) {
+        // one CTA per SM: 256 rows of queries each, as the tensor-core kernel takes them
+        const int per_cta = group <= 128 ? 2 * (128 / group) : 1;
+        const long long ctas = (static_cast<long long>(batch) + per_cta - 1) / per_cta * kv_heads, blocks = (prefix + 127ll) / 128;
+        p.prefix = static_cast<int>(std::max(1ll, std::min(sm_count() / ctas, (blocks + 1) / 2)));
+    }
     const int n = p.prefix + p.own;
     if (n > 1) p.bytes = static_cast<size_t>(n) * batch * heads * (dim + 1) * sizeof(float);
     return p;
@@ -105,7 +112,9 @@ int run_cached(const char *what, int dtype, Cached c, const Parts &parts, void *
         c.part_out = static_cast<float *>(workspace);
         c.part_lse = c.part_out + static_cast<size_t>(n) * c.batch * c.win.heads * c.win.dim;
     }
-    if (parts.prefix > 0) RODE_TRY(simple_shared(dtype, c, 0, parts.prefix, stream));
+    if (parts.prefix > 0)
+        RODE_TRY(tiles_take_shared(dtype, c) ? tiles_shared(dtype, c, 0, parts.prefix, stream)
+                                             : simple_shared(dtype, c, 0, parts.prefix, stream));
     RODE_TRY(simple_step(dtype, c, parts.prefix, parts.own, stream));
     if (n > 1) RODE_TRY(join_parts(dtype, c, n, stream));
     return RODE_OK;
@@ -142,7 +151,7 @@ int rode_window_attention(int dtype, int n_seq, const int *q_offsets, const int 
     p.out = out;
     p.lse = lse;
     p.clear = clear != 0;
-    return simple_prompt(dtype, p, stream);
+    return tiles_take_prompt(dtype, p) ? tiles_prompt(dtype, p, stream) : simple_prompt(dtype, p, stream);
 }
 
 int rode_window_attention_backward_workspace_bytes(int q_rows, int heads, size_t *bytes) {
@@ -292,6 +301,11 @@ int rode_shared_prefix_attention(int dtype, int batch, int prefix, int capacity,
     c.lengths = lengths;
     c.out = out;
     return run_cached(what, dtype, c, plan_parts(batch, prefix, capacity, heads, kv_heads, dim), workspace, workspace_bytes, stream);
+}
+
+int rode_attention_waits_failed(int *failed) {
+    if (failed == nullptr) return fail(RODE_ERR_INVALID_ARGUMENT, "rode_attention_waits_failed: null pointer failed");
+    return tiles_waits_failed(failed);
 }
 
 }  // extern "C"

@@ -61,6 +61,14 @@ int simple_prompt(int dtype, const Prompt &p, cudaStream_t stream);
 int simple_prompt_backward(int dtype, const Prompt &p, cudaStream_t stream);
 int simple_shared(int dtype, const Cached &c, int first_split, int splits, cudaStream_t stream);
 int simple_step(int dtype, const Cached &c, int first_split, int splits, cudaStream_t stream);
+
+// On the tensor cores, where *_take_* says so.
+bool tiles_take_prompt(int dtype, const Prompt &p);
+bool tiles_take_shared(int dtype, const Cached &c);
+int tiles_prompt(int dtype, const Prompt &p, cudaStream_t stream);
+int tiles_shared(int dtype, const Cached &c, int first_split, int splits, cudaStream_t stream);
+int tiles_waits_failed(int *failed);
+
 int join_parts(int dtype, const Cached &c, int splits, cudaStream_t stream);
 
 #ifdef __CUDACC__

@@ -1,0 +1,484 @@
+// Attention of 16-bit operands on the tensor cores (tcgen05): prompts and shared prefixes, head dimensions that are multiples of 8
+// up to 128, 16-byte aligned operands.
+//
+// Rows of a tile are (query, head of the group) pairs, the heads innermost: all heads that read one key head share its key and
+// value tiles, and a tile spans few positions, so that few keys of its blocks are out of its window.  128 / group queries per
+// tile, two tiles per CTA.
+//
+// Forward, per block of 128 keys and tile: S = Q K^T into tensor memory, each thread of a warpgroup takes one row of S into
+// registers (maximum and sum need no exchange), writes the weights P back over S in 16 bits, O += P V with P read
+// from tensor memory.  One warpgroup per tile, so that while one tile is in its softmax the tensor cores work on the other; one
+// warp issues the products, one the copies.
+// O stays in tensor memory.  The running maximum is taken over only when it grows by more than 8 (in base 2): weights may then be as large
+// as 2^8, which costs no precision (the sum has the same factor), and the multiplication of O by 2^(old - new) is rare.
+// P is rounded to the operands' type (the products take 16-bit operands); the sum is that of the unrounded weights.
+#include <type_traits>
+
+#include "rode_attention.cuh"
+#include "rode_tensor_cores.cuh"
+
+namespace rode {
+
+// Waits that were given up (never, unless a kernel has an error), per GPU.
+__device__ int waits_failed;
+
+namespace {
+
+constexpr int kRows = 128;                  // rows and keys of a tile
+constexpr int kPanel = kRows * 128;         // bytes of a panel of 64 columns
+constexpr float kLazy = 8.f;
+
+// The last part of a sequence's keys, queries, ...: rows from `have` on of a tile of `panels` panels become zero (they belong to
+// another sequence, or to nobody, and 0 x NaN is NaN).  One warp.
+__device__ __forceinline__ void clear_rows(uint32_t tile, int panels, int have) {
+    const int lane = threadIdx.x % 32;
+    for (int p = 0; p < panels; ++p)
+        for (int i = have * 8 + lane; i < kRows * 8; i += 32)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(tile + p * kPanel + i * 16), "r"(0) : "memory");
+    fence_async_proxy();
+    __syncwarp();
+}
+
+// What a CTA works on: two tiles of rows, the blocks of keys that any of them sees.
+struct Work {
+    long long row0;     // first query (of the packed operand, or first request)
+    int n_queries;      // queries of this CTA that exist
+    int pos0;           // position of the first one
+    long long key0;     // first key of the sequence
+    int keys;           // its keys
+    int blocks, n_sink, first;
+    __device__ __forceinline__ int key_of(int i) const { return (i < n_sink ? i : first + i - n_sink) * kRows; }
+};
+
+struct TileMaps {
+    CUtensorMap q, k, v;
+};
+
+template <int kDim>
+constexpr int forward_stages() {
+    return kDim == 64 ? 4 : 2;
+}
+template <int kDim>
+constexpr int forward_bytes() {
+    return 1024 + kDim / 64 * kPanel * (2 + 2 * forward_stages<kDim>()) + 512;
+}
+
+// Two warpgroups of softmax, one whose first warp issues the products and whose second one issues the copies.  The registers of a
+// launch (384 x 168) are dealt out anew: 2 x 128 x 216 + 128 x 72 is the same number.
+constexpr int kTileThreads = 384;
+__device__ __forceinline__ void take_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 216;"); }
+__device__ __forceinline__ void give_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 72;"); }
+
+// kShared: rows are requests, keys a part of the prefix, results go to the parts; else prompts.
+template <typename T, int kDim, bool kShared>
+__global__ void __launch_bounds__(kTileThreads, 1)
+    forward_tiles(const __grid_constant__ TileMaps maps, const Prompt p, const Cached c, int first_split, int splits) {
+    constexpr int kPanels = kDim / 64, kStages = forward_stages<kDim>(), kTile = kPanels * kPanel;
+    extern __shared__ char shared_raw[];
+    const Window &w = kShared ? c.win : p.win;
+    const int group = w.heads / w.kv_heads, per_tile = kRows / group, kv = blockIdx.y;
+
+    Work wk;
+    if constexpr (kShared) {
+        wk.row0 = static_cast<long long>(blockIdx.x) * 2 * per_tile;
+        wk.n_queries = static_cast<int>(min(static_cast<long long>(2 * per_tile), c.batch - wk.row0));
+        wk.pos0 = 0;
+        wk.key0 = 0;
+        wk.keys = c.prefix;
+        const long long all = (c.prefix + kRows - 1) / kRows;
+        wk.n_sink = 0;
+        wk.first = static_cast<int>(all * blockIdx.z / splits);
+        wk.blocks = static_cast<int>(all * (blockIdx.z + 1) / splits) - wk.first;
+    } else {
+        const Tile t = find_tile(p.seqs.q_offsets, p.seqs.n_seq, p.seqs.q_rows, blockIdx.x, 2 * per_tile);
+        if (t.first < 0 || t.first >= t.rows || (t.seq < 0 && !p.clear)) return;
+        const int2 keys = t.seq < 0 ? make_int2(0, 0) : sequence_rows(p.seqs.k_offsets, p.seqs.k_rows, t.seq);
+        wk.row0 = static_cast<long long>(t.row0) + t.first;
+        wk.n_queries = min(2 * per_tile, t.rows - t.first);
+        wk.pos0 = t.first + keys.y - t.rows;
+        wk.key0 = keys.x;
+        wk.keys = keys.y;
+        const KeyBlocks b(wk.pos0, wk.pos0 + wk.n_queries, w.window, w.sinks, kRows);
+        wk.blocks = b.n;
+        wk.n_sink = b.n_sink;
+        wk.first = b.first;
+    }
+    // Queries of tile t, and whether it sees any key of the block from k0 on.
+    const auto queries_of = [&](int t) { return min(per_tile, wk.n_queries - t * per_tile); };
+    const auto sees_block = [&](int t, int k0) {
+        const int n = queries_of(t);
+        if (n <= 0) return false;
+        if constexpr (kShared) return true;
+        const int a = wk.pos0 + t * per_tile, b = a + n - 1;  // positions
+        return k0 <= b && (k0 + kRows - 1 > a - w.window || k0 < w.sinks);
+    };
+
+    const uint32_t base = (shared_address(shared_raw) + 1023) & ~1023u;
+    const uint32_t qs = base, ks = qs + 2 * kTile, vs = ks + kStages * kTile, bars = vs + kStages * kTile;
+    const uint32_t q_full = bars, v_raw = bars + 8, s_full = bars + 16, p_full = bars + 32, o_done = bars + 48, k_full = bars + 64,
+                   k_empty = k_full + 8 * kStages, v_full = k_empty + 8 * kStages, v_empty = v_full + 8 * kStages,
+                   tmem_at = v_empty + 8 * kStages;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    if (warp == 8) {
+        tmem_alloc(tmem_at, 512);
+        if (lane == 0) {
+            barrier_init(q_full, 1);
+            barrier_init(v_raw, 1);
+            for (int t = 0; t < 2; ++t) {
+                barrier_init(s_full + 8 * t, 1);
+                barrier_init(p_full + 8 * t, 128);
+                barrier_init(o_done + 8 * t, 1);
+            }
+            for (int i = 0; i < kStages; ++i) {
+                barrier_init(k_full + 8 * i, 1);
+                barrier_init(k_empty + 8 * i, 1);
+                barrier_init(v_full + 8 * i, 1);
+                barrier_init(v_empty + 8 * i, 1);
+            }
+            barrier_init_done();
+        }
+        __syncwarp();
+        tmem_fence_before();
+    }
+    __syncthreads();
+    tmem_fence_after();
+    uint32_t tmem;
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem) : "r"(tmem_at));
+    bool ok = true;  // (a wait that was given up ends the CTA's work; it took seconds, so that no copy is in flight any more)
+
+    if (warp >= 8) give_registers();
+    if (warp == 9) {
+        // copies
+        if (lane == 0 && wk.blocks > 0) {
+            const int tiles = queries_of(1) > 0 ? 2 : 1;
+            barrier_expect(q_full, tiles * kPanels * per_tile * group * 128);
+            for (int t = 0; t < tiles; ++t)
+                for (int x = 0; x < kPanels; ++x)
+                    copy_box(qs + t * kTile + x * kPanel, &maps.q, x * 64, kv * group, static_cast<int>(wk.row0) + t * per_tile, q_full);
+        }
+        int raw = 0;
+        for (int i = 0; i < wk.blocks && ok; ++i) {
+            const int st = i % kStages, k0 = wk.key_of(i), have = wk.keys - k0;
+            const uint32_t free = (i / kStages & 1) ^ 1;
+            const int y = static_cast<int>(wk.key0) + k0;
+            ok = barrier_wait(k_empty + 8 * st, free);
+            if (ok && lane == 0) {
+                barrier_expect(k_full + 8 * st, kTile);
+                for (int x = 0; x < kPanels; ++x) copy_box(ks + st * kTile + x * kPanel, &maps.k, x * 64, kv, y, k_full + 8 * st);
+            }
+            ok = ok && barrier_wait(v_empty + 8 * st, free);
+            if (!ok) break;
+            const uint32_t bar = have < kRows ? v_raw : v_full + 8 * st;
+            if (lane == 0) {
+                barrier_expect(bar, kTile);
+                for (int x = 0; x < kPanels; ++x) copy_box(vs + st * kTile + x * kPanel, &maps.v, x * 64, kv, y, bar);
+            }
+            __syncwarp();
+            if (have < kRows) {
+                ok = barrier_wait(v_raw, raw & 1);
+                ++raw;
+                clear_rows(vs + st * kTile, kPanels, have);
+                if (lane == 0) barrier_arrive(v_full + 8 * st);
+            }
+        }
+    } else if (warp == 8) {
+        // products
+        const uint32_t scores = product_descriptor<T>(kRows, false), values = product_descriptor<T>((w.dim + 15) / 16 * 16, true);
+        const int steps = (w.dim + 15) / 16;
+        int waiting[2] = {0, 0}, issued[2] = {0, 0}, weights[2] = {0, 0};
+        const auto issue_scores = [&](int t, int st) {
+            if (lane == 0) {
+                for (int s = 0; s < steps; ++s) {
+                    const uint32_t at = s / 4 * kPanel + s % 4 * 32;
+                    product(tmem + t * kRows, tile_descriptor(qs + t * kTile + at, 16), tile_descriptor(ks + st * kTile + at, 16), scores,
+                            s > 0);
+                }
+                products_arrive(s_full + 8 * t);
+            }
+        };
+        if (wk.blocks > 0) {
+            ok = barrier_wait(q_full, 0) && barrier_wait(k_full, 0);
+            tmem_fence_after();
+            if (ok) {
+                for (int t = 0; t < 2; ++t)
+                    if (sees_block(t, wk.key_of(0))) issue_scores(t, 0);
+                if (lane == 0) products_arrive(k_empty);
+            }
+        }
+        for (int i = 0; i < wk.blocks && ok; ++i) {
+            const int st = i % kStages, k0 = wk.key_of(i);
+            const bool more = i + 1 < wk.blocks;
+            const int next = (i + 1) % kStages, k1 = more ? wk.key_of(i + 1) : 0;
+            ok = barrier_wait(v_full + 8 * st, i / kStages & 1) && (!more || barrier_wait(k_full + 8 * next, (i + 1) / kStages & 1));
+            for (int t = 0; t < 2 && ok; ++t) {
+                if (sees_block(t, k0)) {
+                    ok = barrier_wait(p_full + 8 * t, weights[t]++ & 1);
+                    if (!ok) break;
+                    tmem_fence_after();
+                    if (lane == 0) {
+                        for (int s = 0; s < kRows / 16; ++s)
+                            product_from_tmem(tmem + 256 + t * kDim, tmem + t * kRows + s * 8,
+                                              tile_descriptor(vs + st * kTile + s * 2048, kPanel), values, issued[t] > 0 || s > 0);
+                        products_arrive(o_done + 8 * t);
+                    }
+                    ++issued[t];
+                }
+                if (more && sees_block(t, k1)) {
+                    // the next scores go where the weights were
+                    if (waiting[t] < issued[t]) {
+                        waiting[t] = issued[t];
+                        ok = barrier_wait(o_done + 8 * t, (issued[t] - 1) & 1);
+                        if (!ok) break;
+                    }
+                    issue_scores(t, next);
+                }
+            }
+            if (ok && lane == 0) {
+                products_arrive(v_empty + 8 * st);
+                if (more) products_arrive(k_empty + 8 * next);
+            }
+            __syncwarp();
+        }
+    } else if (warp < 8) {
+        // softmax: one row per thread
+        take_registers();
+        const int t = warp / 4, r = threadIdx.x % 128;
+        const uint32_t lanes = static_cast<uint32_t>(warp % 4 * 32) << 16;
+        const uint32_t s_at = tmem + lanes + t * kRows, o_at = tmem + lanes + 256 + t * kDim;
+        const int n = queries_of(t), query = r / group, head = kv * group + r % group;
+        const bool mine = query < n;
+        const int a = wk.pos0 + t * per_tile, pos = a + query;
+        const float s2 = w.scale * kLog2e;
+        float m = -INFINITY, l = 0.f;
+        int done = 0;
+        for (int i = 0; i < wk.blocks; ++i) {
+            const int k0 = wk.key_of(i);
+            if (!sees_block(t, k0)) continue;
+            ok = barrier_wait(s_full + 8 * t, done & 1);
+            if (!ok) break;
+            tmem_fence_after();
+            uint32_t s[128];
+            tmem_load32<0>(s_at, s);
+            tmem_load32<32>(s_at + 32, s);
+            tmem_load32<64>(s_at + 64, s);
+            tmem_load32<96>(s_at + 96, s);
+            tmem_wait_load32<0>(s);
+            tmem_wait_load32<32>(s);
+            tmem_wait_load32<64>(s);
+            tmem_wait_load32<96>(s);
+            bool whole;
+            if constexpr (kShared)
+                whole = k0 + kRows <= wk.keys;
+            else
+                whole = k0 + kRows - 1 <= a && (a + n - 1 - k0 < w.window || k0 + kRows <= w.sinks);
+            if (!whole) {
+                const int last = kShared ? wk.keys - 1 - k0 : pos - k0;                  // columns up to this one
+                const int from = kShared ? 0 : pos - w.window + 1 - k0, sink = kShared ? 0 : w.sinks - k0;
+#pragma unroll
+                for (int j = 0; j < 128; ++j)
+                    if (j > last || (j < from && j >= sink)) s[j] = 0xff800000u;  // -infinity
+            }
+            float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int j = 0; j < 128; ++j) top[j % 4] = fmaxf(top[j % 4], __uint_as_float(s[j]));
+            const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+            const bool grows = (high - m) * s2 > kLazy;
+            if (__any_sync(0xffffffffu, grows)) {
+                const float next = grows ? high : m;
+                const float keep = grows ? exp2f((m - next) * s2) : 1.f;
+                m = next;
+                l *= keep;
+                if (done > 0) {
+#pragma unroll
+                    for (int x = 0; x < kDim; x += 32) {
+                        uint32_t o[32];
+                        tmem_load32<0>(o_at + x, o);
+                        tmem_wait_load32<0>(o);
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * keep);
+                        tmem_store32<0>(o_at + x, o);
+                    }
+                }
+            }
+            const float off = m == -INFINITY ? 0.f : -m * s2;
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < 128; j += 2) {
+                float x = fmaf(__uint_as_float(s[j]), s2, off), y = fmaf(__uint_as_float(s[j + 1]), s2, off);
+                asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(x));
+                asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(y));
+                sum[j / 2 % 2 * 2] += x;
+                sum[j / 2 % 2 * 2 + 1] += y;
+                s[j / 2] = pack2<T>(x, y);
+            }
+            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            tmem_store32<0>(s_at, s);
+            tmem_store32<32>(s_at + 32, s);
+            tmem_wait_store();
+            tmem_fence_before();
+            barrier_arrive(p_full + 8 * t);
+            ++done;
+        }
+        if (ok && done > 0) {
+            ok = barrier_wait(o_done + 8 * t, (done - 1) & 1);
+            tmem_fence_after();
+        }
+        const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+        const float lse2 = m == -INFINITY ? -INFINITY : m * s2 + log2f(l);
+        if (kShared) {
+            const long long at = ((first_split + blockIdx.z) * static_cast<long long>(c.batch) + wk.row0 + t * per_tile + query) * w.heads + head;
+            if (mine) c.part_lse[at] = lse2;
+#pragma unroll
+            for (int x = 0; x < kDim; x += 32) {
+                uint32_t o[32];
+                tmem_load32<0>(o_at + x, o);
+                tmem_wait_load32<0>(o);
+#pragma unroll
+                for (int j = 0; j < 32; j += 4)
+                    if (mine && x + j < w.dim)
+                        store4(c.part_out + at * w.dim + x + j,
+                               done > 0 ? make_float4(__uint_as_float(o[j]) * inv, __uint_as_float(o[j + 1]) * inv,
+                                                      __uint_as_float(o[j + 2]) * inv, __uint_as_float(o[j + 3]) * inv)
+                                        : make_float4(0.f, 0.f, 0.f, 0.f));
+            }
+        } else {
+            const long long row = wk.row0 + t * per_tile + query;
+            if (mine && p.lse != nullptr)
+                p.lse[static_cast<long long>(head) * p.seqs.q_rows + row] = lse2 == -INFINITY ? -INFINITY : lse2 * kLn2;
+            T *out = static_cast<T *>(p.out) + (row * w.heads + head) * w.dim;
+#pragma unroll
+            for (int x = 0; x < kDim; x += 32) {
+                uint32_t o[32];
+                tmem_load32<0>(o_at + x, o);
+                tmem_wait_load32<0>(o);
+#pragma unroll
+                for (int j = 0; j < 32; j += 8) {
+                    uint4 y = make_uint4(0, 0, 0, 0);
+                    if (done > 0) {
+                        y.x = pack2<T>(__uint_as_float(o[j]) * inv, __uint_as_float(o[j + 1]) * inv);
+                        y.y = pack2<T>(__uint_as_float(o[j + 2]) * inv, __uint_as_float(o[j + 3]) * inv);
+                        y.z = pack2<T>(__uint_as_float(o[j + 4]) * inv, __uint_as_float(o[j + 5]) * inv);
+                        y.w = pack2<T>(__uint_as_float(o[j + 6]) * inv, __uint_as_float(o[j + 7]) * inv);
+                    }
+                    if (mine && x + j < w.dim) *reinterpret_cast<uint4 *>(out + x + j) = y;
+                }
+            }
+        }
+    }
+    if (!ok) waits_failed = 1;
+    tmem_fence_before();
+    __syncthreads();
+    tmem_fence_after();
+    if (warp == 8) tmem_free(tmem, 512);
+}
+
+// --- host -----------------------------------------------------------------------------------------------------------------------
+
+using EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                                 const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
+                                 CUtensorMapFloatOOBfill);
+
+EncodeTiled encoder() {
+    static const EncodeTiled fn = [] {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found) != cudaSuccess ||
+            found != cudaDriverEntryPointSuccess) {
+            (void)cudaGetLastError();
+            return static_cast<EncodeTiled>(nullptr);
+        }
+        return reinterpret_cast<EncodeTiled>(p);
+    }();
+    return fn;
+}
+
+// [rows][heads][dim] in boxes of 64 columns x box_heads x box_rows; outer is x.row or x.batch.
+int encode(CUtensorMap *map, int dtype, const rode_heads_t &x, long long outer, int rows, int heads, int dim, int box_heads, int box_rows) {
+    const EncodeTiled fn = encoder();
+    if (fn == nullptr) return fail(RODE_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
+    const cuuint64_t line = static_cast<cuuint64_t>(dim) * 2;
+    const cuuint64_t size[3] = {static_cast<cuuint64_t>(dim), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(rows)};
+    // (the strides of dimensions of one element are never used)
+    const cuuint64_t strides[2] = {heads > 1 ? static_cast<cuuint64_t>(x.head) * 2 : line, rows > 1 ? static_cast<cuuint64_t>(outer) * 2 : line};
+    const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(box_heads), static_cast<cuuint32_t>(box_rows)}, step[3] = {1, 1, 1};
+    const CUresult e = fn(map, dtype == RODE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                          const_cast<void *>(x.data), size, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (e != CUDA_SUCCESS) return fail(RODE_ERR_CUDA, "cuTensorMapEncodeTiled failed: %d", static_cast<int>(e));
+    return RODE_OK;
+}
+
+// Base and strides are whole 16-byte units, as a tensor copy wants them, and no dimension repeats.
+bool copyable(const rode_heads_t &x, long long outer, int rows, int heads) {
+    const auto fits = [](long long stride, int n) { return n <= 1 || (stride > 0 && stride % 8 == 0 && stride < (1ll << 39)); };
+    return aligned_to(x.data, 16) && fits(x.head, heads) && fits(outer, rows);
+}
+
+template <typename F>
+int by_half(int dtype, int dim, F &&f) {
+    const auto g = [&](auto *type) {
+        return dim <= 64 ? f(type, std::integral_constant<int, 64>()) : f(type, std::integral_constant<int, 128>());
+    };
+    return dtype == RODE_F16 ? g(static_cast<__half *>(nullptr)) : g(static_cast<__nv_bfloat16 *>(nullptr));
+}
+
+}  // namespace
+
+bool tiles_take(int dtype, const Window &w) {
+    return dtype != RODE_F32 && w.dim % 8 == 0 && w.dim <= 128 && w.heads / w.kv_heads <= kRows && w.scale > 0.f;
+}
+
+bool tiles_take_prompt(int dtype, const Prompt &p) {
+    return tiles_take(dtype, p.win) && p.seqs.k_rows > 0 && copyable(p.q, p.q.row, p.seqs.q_rows, p.win.heads) &&
+           copyable(p.k, p.k.row, p.seqs.k_rows, p.win.kv_heads) && copyable(p.v, p.v.row, p.seqs.k_rows, p.win.kv_heads);
+}
+
+bool tiles_take_shared(int dtype, const Cached &c) {
+    return tiles_take(dtype, c.win) && copyable(c.q, c.q.batch, c.batch, c.win.heads) &&
+           copyable(c.pk, c.pk.row, c.prefix, c.win.kv_heads) && copyable(c.pv, c.pv.row, c.prefix, c.win.kv_heads);
+}
+
+int tiles_prompt(int dtype, const Prompt &p, cudaStream_t stream) {
+    const Window &w = p.win;
+    const int group = w.heads / w.kv_heads, per_tile = kRows / group;
+    TileMaps maps;
+    if (const int e = encode(&maps.q, dtype, p.q, p.q.row, p.seqs.q_rows, w.heads, w.dim, group, per_tile)) return e;
+    if (const int e = encode(&maps.k, dtype, p.k, p.k.row, p.seqs.k_rows, w.kv_heads, w.dim, 1, kRows)) return e;
+    if (const int e = encode(&maps.v, dtype, p.v, p.v.row, p.seqs.k_rows, w.kv_heads, w.dim, 1, kRows)) return e;
+    return by_half(dtype, w.dim, [&](auto *type, auto dim) {
+        using T = std::remove_pointer_t<decltype(type)>;
+        constexpr int kDim = decltype(dim)::value;
+        auto *kernel = &forward_tiles<T, kDim, false>;
+        if (const int e = allow_shared(kernel, forward_bytes<kDim>())) return e;
+        const int slots = tile_slots(p.seqs.q_offsets, p.seqs.n_seq, p.seqs.q_rows, 2 * per_tile);
+        kernel<<<dim3(slots, w.kv_heads), kTileThreads, forward_bytes<kDim>(), stream>>>(maps, p, Cached{}, 0, 1);
+        RODE_CHECK_LAUNCH("forward_tiles");
+        return static_cast<int>(RODE_OK);
+    });
+}
+
+int tiles_shared(int dtype, const Cached &c, int first_split, int splits, cudaStream_t stream) {
+    const Window &w = c.win;
+    const int group = w.heads / w.kv_heads, per_tile = kRows / group;
+    TileMaps maps;
+    if (const int e = encode(&maps.q, dtype, c.q, c.q.batch, c.batch, w.heads, w.dim, group, per_tile)) return e;
+    if (const int e = encode(&maps.k, dtype, c.pk, c.pk.row, c.prefix, w.kv_heads, w.dim, 1, kRows)) return e;
+    if (const int e = encode(&maps.v, dtype, c.pv, c.pv.row, c.prefix, w.kv_heads, w.dim, 1, kRows)) return e;
+    return by_half(dtype, w.dim, [&](auto *type, auto dim) {
+        using T = std::remove_pointer_t<decltype(type)>;
+        constexpr int kDim = decltype(dim)::value;
+        auto *kernel = &forward_tiles<T, kDim, true>;
+        if (const int e = allow_shared(kernel, forward_bytes<kDim>())) return e;
+        const int tiles = (c.batch + 2 * per_tile - 1) / (2 * per_tile);
+        kernel<<<dim3(tiles, w.kv_heads, splits), kTileThreads, forward_bytes<kDim>(), stream>>>(maps, Prompt{}, c, first_split, splits);
+        RODE_CHECK_LAUNCH("forward_tiles");
+        return static_cast<int>(RODE_OK);
+    });
+}
+
+int tiles_waits_failed(int *failed) {
+    RODE_CUDA_TRY(cudaMemcpyFromSymbol(failed, waits_failed, sizeof(int)));
+    return RODE_OK;
+}
+
+}  // namespace rode

@@ -7,6 +7,21 @@ import torch
 import attention_reference as R
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def no_wait_given_up():
+    """No kernel's warps gave up waiting for one another."""
+    import ctypes
+
+    from rode_b200 import capi
+
+    yield
+    failed = ctypes.c_int(-1)
+    capi.check(capi.load().rode_attention_waits_failed(ctypes.byref(failed)))
+    assert failed.value == 0
+
+
 TYPES = [torch.float32, torch.float16, torch.bfloat16]
 
 
