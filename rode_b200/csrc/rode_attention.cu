@@ -202,7 +202,7 @@ int rode_window_attention_backward(int dtype, int n_seq, const int *q_offsets, c
     p.dv = dv;
     p.delta = static_cast<float *>(workspace);
     p.clear = clear != 0;
-    return simple_prompt_backward(dtype, p, stream);
+    return tiles_take_backward(dtype, p) ? tiles_backward(dtype, p, stream) : simple_prompt_backward(dtype, p, stream);
 }
 
 static int check_cached_sizes(const char *what, int batch, int prefix, int capacity) {

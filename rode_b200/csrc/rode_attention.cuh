@@ -66,6 +66,8 @@ int simple_step(int dtype, const Cached &c, int first_split, int splits, cudaStr
 bool tiles_take_prompt(int dtype, const Prompt &p);
 bool tiles_take_shared(int dtype, const Cached &c);
 int tiles_prompt(int dtype, const Prompt &p, cudaStream_t stream);
+bool tiles_take_backward(int dtype, const Prompt &p);
+int tiles_backward(int dtype, const Prompt &p, cudaStream_t stream);
 int tiles_shared(int dtype, const Cached &c, int first_split, int splits, cudaStream_t stream);
 int tiles_waits_failed(int *failed);
 

@@ -372,6 +372,518 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     if (warp == 8) tmem_free(tmem, 512);
 }
 
+// --- gradients ------------------------------------------------------------------------------------------------------------------
+//
+// dS = P (dP - delta) with P = 2^(scale log2e S - lse) and dP = dO V^T again from the operands, delta = dO . O per row.  Two kernels, so that
+// every sum has one owner and one order: one CTA per tile of queries adds up dQ = dS K, one per tile of keys dV = P^T dO and dK = dS^T Q
+// (7 products instead of the 5 that one kernel with atomic additions would need).  The first takes rows of queries as the rows of S, the
+// second computes S^T and dP^T, so that in both the 16-bit factor that the threads compute (dS, P^T, dS^T) is the operand from tensor
+// memory, over the columns it was computed from, and no tile is transposed.  P and dS are rounded to the operands' type for that.
+// Two warpgroups share a tile, each 64 columns.
+
+template <int kDim>
+constexpr int backward_stages() {
+    return kDim == 64 ? 4 : 2;
+}
+template <int kDim>
+constexpr int backward_bytes() {
+    return 1024 + kDim / 64 * kPanel * (2 + 2 * backward_stages<kDim>()) + backward_stages<kDim>() * 2 * kRows * 4 + 512;
+}
+
+struct GradientMaps {
+    CUtensorMap q, dout, k, v;
+};
+
+// Columns [64 half, 64 half + 64) of a tile's P and dS from S and dP in registers; columns out of [from, to) (or below sink) see nothing.
+struct Range {
+    int from, to, sink;  // sees column j when j < to and (j >= from or j < sink)
+};
+
+__device__ __forceinline__ void hide(uint32_t (&x)[64], const Range &r, uint32_t value) {
+#pragma unroll
+    for (int j = 0; j < 64; ++j)
+        if (j >= r.to || (j < r.from && j >= r.sink)) x[j] = value;
+}
+
+// 16-byte pieces of a row: sum of products.
+template <typename T>
+__device__ __forceinline__ float dot_row(const T *a, const T *b, int dim) {
+    float sum = 0.f;
+    for (int d = 0; d < dim; d += 8) {
+        const uint4 x = __ldg(reinterpret_cast<const uint4 *>(a + d)), y = __ldg(reinterpret_cast<const uint4 *>(b + d));
+        const T *s = reinterpret_cast<const T *>(&x), *t = reinterpret_cast<const T *>(&y);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum = fmaf(to_float(s[i]), to_float(t[i]), sum);
+    }
+    return sum;
+}
+
+// Columns x .. x + 31 of an accumulator row, times factor, to 32 elements of a row of `dim`.
+template <typename T>
+__device__ __forceinline__ void store_columns(T *row, uint32_t at, int x, int dim, float factor, bool mine, bool any) {
+    uint32_t o[32];
+    tmem_load32<0>(at + x, o);
+    tmem_wait_load32<0>(o);
+#pragma unroll
+    for (int j = 0; j < 32; j += 8) {
+        uint4 y = make_uint4(0, 0, 0, 0);
+        if (any) {
+            y.x = pack2<T>(__uint_as_float(o[j]) * factor, __uint_as_float(o[j + 1]) * factor);
+            y.y = pack2<T>(__uint_as_float(o[j + 2]) * factor, __uint_as_float(o[j + 3]) * factor);
+            y.z = pack2<T>(__uint_as_float(o[j + 4]) * factor, __uint_as_float(o[j + 5]) * factor);
+            y.w = pack2<T>(__uint_as_float(o[j + 6]) * factor, __uint_as_float(o[j + 7]) * factor);
+        }
+        if (mine && x + j < dim) *reinterpret_cast<uint4 *>(row + x + j) = y;
+    }
+}
+
+// dQ of one tile of rows, and delta.  Tensor memory: S twice (dS over it), dP, dQ.  The products of block i + 1 that need no dS (S, then
+// dP) run while the threads work on block i.
+template <typename T, int kDim>
+__global__ void __launch_bounds__(kTileThreads, 1) query_gradient_tiles(const __grid_constant__ GradientMaps maps, const Prompt p) {
+    constexpr int kPanels = kDim / 64, kStages = backward_stages<kDim>(), kTile = kPanels * kPanel;
+    extern __shared__ char shared_raw[];
+    const Window &w = p.win;
+    const int group = w.heads / w.kv_heads, per_tile = kRows / group, kv = blockIdx.y;
+    const Tile t = find_tile(p.seqs.q_offsets, p.seqs.n_seq, p.seqs.q_rows, blockIdx.x, per_tile);
+    if (t.first < 0 || t.first >= t.rows || (t.seq < 0 && !p.clear)) return;
+    const int2 keys = t.seq < 0 ? make_int2(0, 0) : sequence_rows(p.seqs.k_offsets, p.seqs.k_rows, t.seq);
+    const long long row0 = static_cast<long long>(t.row0) + t.first;
+    const int n = min(per_tile, t.rows - t.first), pos0 = t.first + keys.y - t.rows;
+    const KeyBlocks blocks(pos0, pos0 + n, w.window, w.sinks, kRows);
+
+    const uint32_t base = (shared_address(shared_raw) + 1023) & ~1023u;
+    const uint32_t qs = base, gs = qs + kTile, ks = gs + kTile, vs = ks + kStages * kTile, bars = vs + kStages * kTile;
+    const uint32_t q_full = bars, k_raw = bars + 8, s_full = bars + 16, dp_full = bars + 32, ds_full = bars + 40, dq_done = bars + 48,
+                   k_full = bars + 64, k_empty = k_full + 8 * kStages, v_full = k_empty + 8 * kStages, v_empty = v_full + 8 * kStages,
+                   tmem_at = v_empty + 8 * kStages;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    if (warp == 8) {
+        tmem_alloc(tmem_at, 512);
+        if (lane == 0) {
+            barrier_init(q_full, 1);
+            barrier_init(k_raw, 1);
+            barrier_init(s_full, 1);
+            barrier_init(s_full + 8, 1);
+            barrier_init(dp_full, 1);
+            barrier_init(ds_full, 256);
+            barrier_init(dq_done, 1);
+            for (int i = 0; i < kStages; ++i) {
+                barrier_init(k_full + 8 * i, 1);
+                barrier_init(k_empty + 8 * i, 1);
+                barrier_init(v_full + 8 * i, 1);
+                barrier_init(v_empty + 8 * i, 1);
+            }
+            barrier_init_done();
+        }
+        __syncwarp();
+        tmem_fence_before();
+    }
+    __syncthreads();
+    tmem_fence_after();
+    uint32_t tmem;
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem) : "r"(tmem_at));
+    const uint32_t dp_at = tmem + 256, dq_at = tmem + 384;
+    bool ok = true;
+
+    if (warp >= 8) give_registers();
+    if (warp == 9) {
+        if (lane == 0 && blocks.n > 0) {
+            barrier_expect(q_full, 2 * kPanels * per_tile * group * 128);
+            for (int x = 0; x < kPanels; ++x) {
+                copy_box(qs + x * kPanel, &maps.q, x * 64, kv * group, static_cast<int>(row0), q_full);
+                copy_box(gs + x * kPanel, &maps.dout, x * 64, kv * group, static_cast<int>(row0), q_full);
+            }
+        }
+        int raw = 0;
+        for (int i = 0; i < blocks.n && ok; ++i) {
+            const int st = i % kStages, k0 = blocks.at(i) * kRows, have = keys.y - k0, y = keys.x + k0;
+            const uint32_t free = (i / kStages & 1) ^ 1;
+            ok = barrier_wait(k_empty + 8 * st, free);
+            const uint32_t bar = have < kRows ? k_raw : k_full + 8 * st;
+            if (ok && lane == 0) {
+                barrier_expect(bar, kTile);
+                for (int x = 0; x < kPanels; ++x) copy_box(ks + st * kTile + x * kPanel, &maps.k, x * 64, kv, y, bar);
+            }
+            __syncwarp();
+            if (ok && have < kRows) {
+                ok = barrier_wait(k_raw, raw++ & 1);
+                clear_rows(ks + st * kTile, kPanels, have);
+                if (lane == 0) barrier_arrive(k_full + 8 * st);
+            }
+            ok = ok && barrier_wait(v_empty + 8 * st, free);
+            if (ok && lane == 0) {
+                barrier_expect(v_full + 8 * st, kTile);
+                for (int x = 0; x < kPanels; ++x) copy_box(vs + st * kTile + x * kPanel, &maps.v, x * 64, kv, y, v_full + 8 * st);
+            }
+            __syncwarp();
+        }
+    } else if (warp == 8) {
+        const uint32_t scores = product_descriptor<T>(kRows, false), sums = product_descriptor<T>((w.dim + 15) / 16 * 16, true);
+        const int steps = (w.dim + 15) / 16;
+        const auto issue = [&](uint32_t d, uint32_t a, uint32_t b, uint32_t bar) {
+            if (lane == 0) {
+                for (int s = 0; s < steps; ++s) {
+                    const uint32_t at = s / 4 * kPanel + s % 4 * 32;
+                    product(d, tile_descriptor(a + at, 16), tile_descriptor(b + at, 16), scores, s > 0);
+                }
+                products_arrive(bar);
+            }
+        };
+        if (blocks.n > 0) {
+            ok = barrier_wait(q_full, 0) && barrier_wait(k_full, 0) && barrier_wait(v_full, 0);
+            tmem_fence_after();
+            if (ok) {
+                issue(tmem, qs, ks, s_full);
+                issue(dp_at, gs, vs, dp_full);
+                if (lane == 0) products_arrive(v_empty);
+            }
+        }
+        for (int i = 0; i < blocks.n && ok; ++i) {
+            const int st = i % kStages, next = (i + 1) % kStages, buf = i & 1;
+            const uint32_t next_full = (i + 1) / kStages & 1;
+            const bool more = i + 1 < blocks.n;
+            // (every phase of dq_done is waited for here, so that the threads' wait for the last one cannot be a phase early)
+            ok = i == 0 || barrier_wait(dq_done, (i - 1) & 1);
+            if (!ok) break;
+            if (more) {
+                // S of the next block where dS of the last one was
+                ok = barrier_wait(k_full + 8 * next, next_full);
+                if (!ok) break;
+                tmem_fence_after();
+                issue(tmem + (buf ^ 1) * kRows, qs, ks + next * kTile, s_full + 8 * (buf ^ 1));
+            }
+            ok = barrier_wait(ds_full, i & 1);
+            if (!ok) break;
+            tmem_fence_after();
+            if (lane == 0) {
+                for (int s = 0; s < kRows / 16; ++s)
+                    product_from_tmem(dq_at, tmem + buf * kRows + s / 4 * 64 + s % 4 * 8, tile_descriptor(ks + st * kTile + s * 2048, kPanel),
+                                      sums, i > 0 || s > 0);
+                products_arrive(dq_done);
+                products_arrive(k_empty + 8 * st);
+            }
+            if (more) {
+                ok = barrier_wait(v_full + 8 * next, next_full);
+                if (!ok) break;
+                issue(dp_at, gs, vs + next * kTile, dp_full);
+                if (lane == 0) products_arrive(v_empty + 8 * next);
+            }
+            __syncwarp();
+        }
+    } else if (warp < 8) {
+        take_registers();
+        const int half = warp / 4, r = threadIdx.x % 128;
+        const uint32_t lanes = static_cast<uint32_t>(warp % 4 * 32) << 16;
+        const int query = r / group, head = kv * group + r % group, pos = pos0 + query;
+        const bool mine = query < n;
+        const long long row = row0 + query, at = static_cast<long long>(head) * p.seqs.q_rows + row;
+        float delta = 0.f, off = 0.f;
+        if (mine) {
+            delta = dot_row(row_of<T>(p.dout, 0, row, head), static_cast<const T *>(p.out) + (row * w.heads + head) * w.dim, w.dim);
+            const float lse = p.lse[at];
+            if (half == 0) p.delta[at] = delta;
+            off = lse == -INFINITY ? 0.f : -lse * kLog2e;
+        }
+        const float s2 = w.scale * kLog2e;
+        for (int i = 0; i < blocks.n; ++i) {
+            const int k0 = blocks.at(i) * kRows, buf = i & 1, c0 = k0 + half * 64;
+            const uint32_t s_at = tmem + lanes + buf * kRows + half * 64;
+            const bool whole = k0 + kRows - 1 <= pos0 && (pos0 + n - 1 - k0 < w.window || k0 + kRows <= w.sinks);
+            const Range range = {pos - w.window + 1 - c0, pos + 1 - c0, w.sinks - c0};
+            ok = barrier_wait(s_full + 8 * buf, i / 2 & 1);
+            if (!ok) break;
+            tmem_fence_after();
+            uint32_t s[64], d[64];
+            tmem_load32<0>(s_at, s);
+            tmem_load32<32>(s_at + 32, s);
+            tmem_wait_load32<0>(s);
+            tmem_wait_load32<32>(s);
+            if (!whole) hide(s, range, 0xff800000u);
+#pragma unroll
+            for (int j = 0; j < 64; ++j) {
+                float x = fmaf(__uint_as_float(s[j]), s2, off);
+                asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(x));
+                s[j] = __float_as_uint(x);
+            }
+            ok = barrier_wait(dp_full, i & 1);
+            if (!ok) break;
+            tmem_fence_after();
+            tmem_load32<0>(dp_at + lanes + half * 64, d);
+            tmem_load32<32>(dp_at + lanes + half * 64 + 32, d);
+            tmem_wait_load32<0>(d);
+            tmem_wait_load32<32>(d);
+            if (!whole) hide(d, range, 0u);
+#pragma unroll
+            for (int j = 0; j < 64; j += 2)
+                s[j / 2] = pack2<T>(__uint_as_float(s[j]) * (__uint_as_float(d[j]) - delta),
+                                    __uint_as_float(s[j + 1]) * (__uint_as_float(d[j + 1]) - delta));
+            tmem_store32<0>(s_at, s);
+            tmem_wait_store();
+            tmem_fence_before();
+            barrier_arrive(ds_full);
+        }
+        if (ok && blocks.n > 0) {
+            ok = barrier_wait(dq_done, (blocks.n - 1) & 1);
+            tmem_fence_after();
+        }
+        T *out = static_cast<T *>(p.dq) + (row * w.heads + head) * w.dim;
+#pragma unroll
+        for (int x = 0; x < kDim / 2; x += 32)
+            store_columns(out, dq_at + lanes, half * (kDim / 2) + x, w.dim, w.scale, mine, blocks.n > 0);
+    }
+    if (!ok) waits_failed = 1;
+    tmem_fence_before();
+    __syncthreads();
+    tmem_fence_after();
+    if (warp == 8) tmem_free(tmem, 512);
+}
+
+// dK and dV of one tile of 128 keys: all rows of queries that see any of them, 128 at a time.  Tensor memory: S^T (P^T over it), dP^T
+// (dS^T over it), dV, dK.  Per tile of queries the products run in the order dV, next S^T, dK, next dP^T: while the threads make dS of this tile
+// the tensor cores work on dV and the next S^T, while they make the next P on dK and the next dP^T.
+template <typename T, int kDim>
+__global__ void __launch_bounds__(kTileThreads, 1) key_gradient_tiles(const __grid_constant__ GradientMaps maps, const Prompt p) {
+    constexpr int kPanels = kDim / 64, kStages = backward_stages<kDim>(), kTile = kPanels * kPanel;
+    extern __shared__ char shared_raw[];
+    const Window &w = p.win;
+    const int group = w.heads / w.kv_heads, per_tile = kRows / group, kv = blockIdx.y;
+    const Tile t = find_tile(p.seqs.k_offsets, p.seqs.n_seq, p.seqs.k_rows, blockIdx.x, kRows);
+    if (t.first < 0 || t.first >= t.rows || (t.seq < 0 && !p.clear)) return;
+    const int2 queries = t.seq < 0 ? make_int2(0, 0) : sequence_rows(p.seqs.q_offsets, p.seqs.q_rows, t.seq);
+    const long long row0 = static_cast<long long>(t.row0) + t.first;
+    const int have = min(kRows, t.rows - t.first), shift = t.rows - queries.y;
+    // queries from the tile's first key to the end of its last key's window (sinks: to the end)
+    const int last = t.first < w.sinks || w.window >= t.rows - (t.first + have - 1) ? t.rows : t.first + have - 1 + w.window;
+    const int i0 = max(t.first - shift, 0), i1 = max(min(last - shift, queries.y), i0), tiles = (i1 - i0 + per_tile - 1) / per_tile;
+
+    const uint32_t base = (shared_address(shared_raw) + 1023) & ~1023u;
+    const uint32_t ks = base, vs = ks + kTile, qs = vs + kTile, gs = qs + kStages * kTile, rows_at = gs + kStages * kTile,
+                   bars = rows_at + kStages * 2 * kRows * 4;
+    const uint32_t k_full = bars, raw = bars + 8, s_full = bars + 16, p_full = bars + 24, dp_full = bars + 32, ds_full = bars + 40,
+                   dv_done = bars + 48, dk_done = bars + 56, q_full = bars + 64, q_empty = q_full + 8 * kStages, g_full = q_empty + 8 * kStages,
+                   g_empty = g_full + 8 * kStages, rows_full = g_empty + 8 * kStages, tmem_at = rows_full + 8 * kStages;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    if (warp == 8) {
+        tmem_alloc(tmem_at, 512);
+        if (lane == 0) {
+            barrier_init(k_full, 1);
+            barrier_init(raw, 1);
+            barrier_init(s_full, 1);
+            barrier_init(p_full, 256);
+            barrier_init(dp_full, 1);
+            barrier_init(ds_full, 256);
+            barrier_init(dv_done, 1);
+            barrier_init(dk_done, 1);
+            for (int i = 0; i < kStages; ++i) {
+                barrier_init(q_full + 8 * i, 1);
+                barrier_init(q_empty + 8 * i, 1);
+                barrier_init(g_full + 8 * i, 1);
+                barrier_init(g_empty + 8 * i, 1);
+                barrier_init(rows_full + 8 * i, 32);
+            }
+            barrier_init_done();
+        }
+        __syncwarp();
+        tmem_fence_before();
+    }
+    __syncthreads();
+    tmem_fence_after();
+    uint32_t tmem;
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem) : "r"(tmem_at));
+    const uint32_t dp_at = tmem + 128, dv_at = tmem + 256, dk_at = tmem + 384;
+    bool ok = true;
+
+    if (warp >= 8) give_registers();
+    if (warp == 9) {
+        if (lane == 0 && tiles > 0) {
+            barrier_expect(k_full, 2 * kTile);
+            for (int x = 0; x < kPanels; ++x) {
+                copy_box(ks + x * kPanel, &maps.k, x * 64, kv, static_cast<int>(row0), k_full);
+                copy_box(vs + x * kPanel, &maps.v, x * 64, kv, static_cast<int>(row0), k_full);
+            }
+        }
+        // rows that no copy writes, where the group does not divide 128
+        const int full = per_tile * group;
+        if (full < kRows)
+            for (int i = 0; i < kStages; ++i) {
+                clear_rows(qs + i * kTile, kPanels, full);
+                clear_rows(gs + i * kTile, kPanels, full);
+            }
+        int cleared = 0;
+        for (int i = 0; i < tiles && ok; ++i) {
+            const int st = i % kStages, n = min(per_tile, queries.y - i0 - i * per_tile), y = queries.x + i0 + i * per_tile;
+            const uint32_t free = (i / kStages & 1) ^ 1;
+            for (int u = 0; u < 2 && ok; ++u) {  // queries, then gradients of the results
+                const uint32_t tile = (u ? gs : qs) + st * kTile, done = (u ? g_full : q_full) + 8 * st, bar = n < per_tile ? raw : done;
+                ok = barrier_wait((u ? g_empty : q_empty) + 8 * st, free);
+                if (ok && lane == 0) {
+                    barrier_expect(bar, kPanels * full * 128);
+                    for (int x = 0; x < kPanels; ++x) copy_box(tile + x * kPanel, u ? &maps.dout : &maps.q, x * 64, kv * group, y, bar);
+                }
+                __syncwarp();
+                if (ok && n < per_tile) {
+                    ok = barrier_wait(raw, cleared++ & 1);
+                    clear_rows(tile, kPanels, n * group);
+                    if (lane == 0) barrier_arrive(done);
+                }
+            }
+        }
+    } else if (warp == 10) {
+        // lse and delta of the tiles' rows
+        for (int i = 0; i < tiles && ok; ++i) {
+            const int st = i % kStages, n = min(per_tile, queries.y - i0 - i * per_tile);
+            const long long first = static_cast<long long>(queries.x) + i0 + i * per_tile;
+            // (free when the queries of the stage are: their last product comes behind ds_full)
+            ok = barrier_wait(q_empty + 8 * st, (i / kStages & 1) ^ 1);
+            if (!ok) break;
+            for (int r = lane; r < kRows; r += 32) {
+                float lse = 0.f, delta = 0.f;
+                if (r / group < n) {
+                    const long long at = static_cast<long long>(kv * group + r % group) * p.seqs.q_rows + first + r / group;
+                    lse = __ldg(p.lse + at);
+                    lse = lse == -INFINITY ? 0.f : -lse * kLog2e;
+                    delta = __ldg(p.delta + at);
+                }
+                asm volatile("st.shared.b32 [%0], %1;" ::"r"(rows_at + (st * 2 * kRows + r) * 4), "f"(lse) : "memory");
+                asm volatile("st.shared.b32 [%0], %1;" ::"r"(rows_at + (st * 2 * kRows + kRows + r) * 4), "f"(delta) : "memory");
+            }
+            barrier_arrive(rows_full + 8 * st);
+        }
+    } else if (warp == 8) {
+        const uint32_t scores = product_descriptor<T>(kRows, false), sums = product_descriptor<T>((w.dim + 15) / 16 * 16, true);
+        const int steps = (w.dim + 15) / 16;
+        const auto issue = [&](uint32_t d, uint32_t a, uint32_t b, uint32_t bar) {
+            if (lane == 0) {
+                for (int s = 0; s < steps; ++s) {
+                    const uint32_t at = s / 4 * kPanel + s % 4 * 32;
+                    product(d, tile_descriptor(a + at, 16), tile_descriptor(b + at, 16), scores, s > 0);
+                }
+                products_arrive(bar);
+            }
+        };
+        const auto add_up = [&](uint32_t d, uint32_t a, uint32_t b, bool add, uint32_t bar, uint32_t free) {
+            if (lane == 0) {
+                for (int s = 0; s < kRows / 16; ++s)
+                    product_from_tmem(d, a + s / 4 * 64 + s % 4 * 8, tile_descriptor(b + s * 2048, kPanel), sums, add || s > 0);
+                products_arrive(bar);
+                products_arrive(free);
+            }
+        };
+        if (tiles > 0) {
+            ok = barrier_wait(k_full, 0) && barrier_wait(q_full, 0) && barrier_wait(g_full, 0);
+            tmem_fence_after();
+            if (ok) {
+                issue(tmem, ks, qs, s_full);
+                issue(dp_at, vs, gs, dp_full);
+            }
+        }
+        for (int i = 0; i < tiles && ok; ++i) {
+            const int st = i % kStages, next = (i + 1) % kStages;
+            const uint32_t next_full = (i + 1) / kStages & 1;
+            const bool more = i + 1 < tiles;
+            ok = barrier_wait(p_full, i & 1);
+            if (!ok) break;
+            tmem_fence_after();
+            add_up(dv_at, tmem, gs + st * kTile, i > 0, dv_done, g_empty + 8 * st);
+            if (more) {
+                ok = barrier_wait(q_full + 8 * next, next_full) && barrier_wait(dv_done, i & 1);
+                if (!ok) break;
+                issue(tmem, ks, qs + next * kTile, s_full);
+            }
+            ok = barrier_wait(ds_full, i & 1);
+            if (!ok) break;
+            tmem_fence_after();
+            add_up(dk_at, dp_at, qs + st * kTile, i > 0, dk_done, q_empty + 8 * st);
+            if (more) {
+                ok = barrier_wait(g_full + 8 * next, next_full) && barrier_wait(dk_done, i & 1);
+                if (!ok) break;
+                issue(dp_at, vs, gs + next * kTile, dp_full);
+            }
+            __syncwarp();
+        }
+    } else if (warp < 8) {
+        take_registers();
+        const int half = warp / 4, r = threadIdx.x % 128, key = t.first + r;
+        const uint32_t lanes = static_cast<uint32_t>(warp % 4 * 32) << 16;
+        const uint32_t s_at = tmem + lanes + half * 64, d_at = dp_at + lanes + half * 64;
+        const float s2 = w.scale * kLog2e;
+        for (int i = 0; i < tiles; ++i) {
+            const int st = i % kStages, q0 = i0 + i * per_tile, n = min(per_tile, queries.y - q0), pos0 = q0 + shift;
+            // columns are (query, head): the queries that see this thread's key are a range of them
+            const bool whole = n * group == kRows && pos0 >= t.first + have - 1 && (pos0 + n - 1 - t.first < w.window || t.first + have <= w.sinks);
+            const int a = min(max(key - pos0, 0), n), b = key < w.sinks ? n : max(min(n, key - pos0 + w.window), 0);
+            const Range range = {a * group - half * 64, b * group - half * 64, 0};
+            const uint32_t off_at = rows_at + (st * 2 * kRows + half * 64) * 4, delta_at = off_at + kRows * 4;
+            ok = barrier_wait(rows_full + 8 * st, i / kStages & 1) && barrier_wait(s_full, i & 1);
+            if (!ok) break;
+            tmem_fence_after();
+            uint32_t s[64], d[64];
+            tmem_load32<0>(s_at, s);
+            tmem_load32<32>(s_at + 32, s);
+            tmem_wait_load32<0>(s);
+            tmem_wait_load32<32>(s);
+            if (!whole) hide(s, range, 0xff800000u);
+#pragma unroll
+            for (int j = 0; j < 64; j += 4) {
+                float o[4];
+                asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(o[0]), "=f"(o[1]), "=f"(o[2]), "=f"(o[3]) : "r"(off_at + j * 4));
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    float x = fmaf(__uint_as_float(s[j + u]), s2, o[u]);
+                    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(x));
+                    s[j + u] = __float_as_uint(x);
+                }
+            }
+            {
+                uint32_t packed[32];
+#pragma unroll
+                for (int j = 0; j < 64; j += 2) packed[j / 2] = pack2<T>(__uint_as_float(s[j]), __uint_as_float(s[j + 1]));
+                tmem_store32<0>(s_at, packed);
+                tmem_wait_store();
+                tmem_fence_before();
+                barrier_arrive(p_full);
+            }
+            ok = barrier_wait(dp_full, i & 1);
+            if (!ok) break;
+            tmem_fence_after();
+            tmem_load32<0>(d_at, d);
+            tmem_load32<32>(d_at + 32, d);
+            tmem_wait_load32<0>(d);
+            tmem_wait_load32<32>(d);
+            if (!whole) hide(d, range, 0u);
+#pragma unroll
+            for (int j = 0; j < 64; j += 4) {
+                float o[4];
+                asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(o[0]), "=f"(o[1]), "=f"(o[2]), "=f"(o[3]) : "r"(delta_at + j * 4));
+                float x[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) x[u] = __uint_as_float(s[j + u]) * (__uint_as_float(d[j + u]) - o[u]);
+                s[j / 2] = pack2<T>(x[0], x[1]);
+                s[j / 2 + 1] = pack2<T>(x[2], x[3]);
+            }
+            tmem_store32<0>(d_at, s);
+            tmem_wait_store();
+            tmem_fence_before();
+            barrier_arrive(ds_full);
+        }
+        if (ok && tiles > 0) {
+            ok = barrier_wait(dk_done, (tiles - 1) & 1) && barrier_wait(dv_done, (tiles - 1) & 1);
+            tmem_fence_after();
+        }
+        const long long at = ((row0 + r) * w.kv_heads + kv) * w.dim;
+        T *out = static_cast<T *>(half == 0 ? p.dv : p.dk) + at;
+#pragma unroll
+        for (int x = 0; x < kDim; x += 32)
+            store_columns(out, (half == 0 ? dv_at : dk_at) + lanes, x, w.dim, half == 0 ? 1.f : w.scale, r < have, tiles > 0);
+    }
+    if (!ok) waits_failed = 1;
+    tmem_fence_before();
+    __syncthreads();
+    tmem_fence_after();
+    if (warp == 8) tmem_free(tmem, 512);
+}
+
 // --- host -----------------------------------------------------------------------------------------------------------------------
 
 using EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
@@ -433,6 +945,10 @@ bool tiles_take_prompt(int dtype, const Prompt &p) {
            copyable(p.k, p.k.row, p.seqs.k_rows, p.win.kv_heads) && copyable(p.v, p.v.row, p.seqs.k_rows, p.win.kv_heads);
 }
 
+bool tiles_take_backward(int dtype, const Prompt &p) {
+    return tiles_take_prompt(dtype, p) && p.seqs.q_rows > 0 && copyable(p.dout, p.dout.row, p.seqs.q_rows, p.win.heads);
+}
+
 bool tiles_take_shared(int dtype, const Cached &c) {
     return tiles_take(dtype, c.win) && copyable(c.q, c.q.batch, c.batch, c.win.heads) &&
            copyable(c.pk, c.pk.row, c.prefix, c.win.kv_heads) && copyable(c.pv, c.pv.row, c.prefix, c.win.kv_heads);
@@ -453,6 +969,32 @@ int tiles_prompt(int dtype, const Prompt &p, cudaStream_t stream) {
         const int slots = tile_slots(p.seqs.q_offsets, p.seqs.n_seq, p.seqs.q_rows, 2 * per_tile);
         kernel<<<dim3(slots, w.kv_heads), kTileThreads, forward_bytes<kDim>(), stream>>>(maps, p, Cached{}, 0, 1);
         RODE_CHECK_LAUNCH("forward_tiles");
+        return static_cast<int>(RODE_OK);
+    });
+}
+
+int tiles_backward(int dtype, const Prompt &p, cudaStream_t stream) {
+    const Window &w = p.win;
+    const int group = w.heads / w.kv_heads, per_tile = kRows / group;
+    GradientMaps maps;
+    if (const int e = encode(&maps.q, dtype, p.q, p.q.row, p.seqs.q_rows, w.heads, w.dim, group, per_tile)) return e;
+    if (const int e = encode(&maps.dout, dtype, p.dout, p.dout.row, p.seqs.q_rows, w.heads, w.dim, group, per_tile)) return e;
+    if (const int e = encode(&maps.k, dtype, p.k, p.k.row, p.seqs.k_rows, w.kv_heads, w.dim, 1, kRows)) return e;
+    if (const int e = encode(&maps.v, dtype, p.v, p.v.row, p.seqs.k_rows, w.kv_heads, w.dim, 1, kRows)) return e;
+    return by_half(dtype, w.dim, [&](auto *type, auto dim) {
+        using T = std::remove_pointer_t<decltype(type)>;
+        constexpr int kDim = decltype(dim)::value;
+        auto *rows = &query_gradient_tiles<T, kDim>;
+        auto *keys = &key_gradient_tiles<T, kDim>;
+        if (const int e = allow_shared(rows, backward_bytes<kDim>())) return e;
+        if (const int e = allow_shared(keys, backward_bytes<kDim>())) return e;
+        const int slots = tile_slots(p.seqs.q_offsets, p.seqs.n_seq, p.seqs.q_rows, per_tile);
+        rows<<<dim3(slots, w.kv_heads), kTileThreads, backward_bytes<kDim>(), stream>>>(maps, p);
+        RODE_CHECK_LAUNCH("query_gradient_tiles");
+        if (p.dk == nullptr) return static_cast<int>(RODE_OK);
+        const int k_slots = tile_slots(p.seqs.k_offsets, p.seqs.n_seq, p.seqs.k_rows, kRows);
+        keys<<<dim3(k_slots, w.kv_heads), kTileThreads, backward_bytes<kDim>(), stream>>>(maps, p);
+        RODE_CHECK_LAUNCH("key_gradient_tiles");
         return static_cast<int>(RODE_OK);
     });
 }
