@@ -115,7 +115,8 @@ int run_cached(const char *what, int dtype, Cached c, const Parts &parts, void *
     if (parts.prefix > 0)
         RODE_TRY(tiles_take_shared(dtype, c) ? tiles_shared(dtype, c, 0, parts.prefix, stream)
                                              : simple_shared(dtype, c, 0, parts.prefix, stream));
-    RODE_TRY(simple_step(dtype, c, parts.prefix, parts.own, stream));
+    RODE_TRY(step_takes(dtype, c) ? step_on_tensor_cores(dtype, c, parts.prefix, parts.own, stream)
+                                  : simple_step(dtype, c, parts.prefix, parts.own, stream));
     if (n > 1) RODE_TRY(join_parts(dtype, c, n, stream));
     return RODE_OK;
 }

@@ -69,6 +69,8 @@ int tiles_prompt(int dtype, const Prompt &p, cudaStream_t stream);
 bool tiles_take_backward(int dtype, const Prompt &p);
 int tiles_backward(int dtype, const Prompt &p, cudaStream_t stream);
 int tiles_shared(int dtype, const Cached &c, int first_split, int splits, cudaStream_t stream);
+bool step_takes(int dtype, const Cached &c);
+int step_on_tensor_cores(int dtype, const Cached &c, int first_split, int splits, cudaStream_t stream);
 int tiles_waits_failed(int *failed);
 
 int join_parts(int dtype, const Cached &c, int splits, cudaStream_t stream);
