@@ -904,6 +904,8 @@ EncodeTiled encoder() {
     return fn;
 }
 
+// (A call of the driver, for which the thread must have a context: it has one behind allow_shared, a call of the runtime.  Autograd's
+// threads may come here without.)
 // [rows][heads][dim] in boxes of 64 columns x box_heads x box_rows; outer is x.row or x.batch.
 int encode(CUtensorMap *map, int dtype, const rode_heads_t &x, long long outer, int rows, int heads, int dim, int box_heads, int box_rows) {
     const EncodeTiled fn = encoder();
@@ -958,14 +960,14 @@ int tiles_prompt(int dtype, const Prompt &p, cudaStream_t stream) {
     const Window &w = p.win;
     const int group = w.heads / w.kv_heads, per_tile = kRows / group;
     TileMaps maps;
-    if (const int e = encode(&maps.q, dtype, p.q, p.q.row, p.seqs.q_rows, w.heads, w.dim, group, per_tile)) return e;
-    if (const int e = encode(&maps.k, dtype, p.k, p.k.row, p.seqs.k_rows, w.kv_heads, w.dim, 1, kRows)) return e;
-    if (const int e = encode(&maps.v, dtype, p.v, p.v.row, p.seqs.k_rows, w.kv_heads, w.dim, 1, kRows)) return e;
     return by_half(dtype, w.dim, [&](auto *type, auto dim) {
         using T = std::remove_pointer_t<decltype(type)>;
         constexpr int kDim = decltype(dim)::value;
         auto *kernel = &forward_tiles<T, kDim, false>;
         if (const int e = allow_shared(kernel, forward_bytes<kDim>())) return e;
+        if (const int e = encode(&maps.q, dtype, p.q, p.q.row, p.seqs.q_rows, w.heads, w.dim, group, per_tile)) return e;
+        if (const int e = encode(&maps.k, dtype, p.k, p.k.row, p.seqs.k_rows, w.kv_heads, w.dim, 1, kRows)) return e;
+        if (const int e = encode(&maps.v, dtype, p.v, p.v.row, p.seqs.k_rows, w.kv_heads, w.dim, 1, kRows)) return e;
         const int slots = tile_slots(p.seqs.q_offsets, p.seqs.n_seq, p.seqs.q_rows, 2 * per_tile);
         kernel<<<dim3(slots, w.kv_heads), kTileThreads, forward_bytes<kDim>(), stream>>>(maps, p, Cached{}, 0, 1);
         RODE_CHECK_LAUNCH("forward_tiles");
@@ -977,10 +979,6 @@ int tiles_backward(int dtype, const Prompt &p, cudaStream_t stream) {
     const Window &w = p.win;
     const int group = w.heads / w.kv_heads, per_tile = kRows / group;
     GradientMaps maps;
-    if (const int e = encode(&maps.q, dtype, p.q, p.q.row, p.seqs.q_rows, w.heads, w.dim, group, per_tile)) return e;
-    if (const int e = encode(&maps.dout, dtype, p.dout, p.dout.row, p.seqs.q_rows, w.heads, w.dim, group, per_tile)) return e;
-    if (const int e = encode(&maps.k, dtype, p.k, p.k.row, p.seqs.k_rows, w.kv_heads, w.dim, 1, kRows)) return e;
-    if (const int e = encode(&maps.v, dtype, p.v, p.v.row, p.seqs.k_rows, w.kv_heads, w.dim, 1, kRows)) return e;
     return by_half(dtype, w.dim, [&](auto *type, auto dim) {
         using T = std::remove_pointer_t<decltype(type)>;
         constexpr int kDim = decltype(dim)::value;
@@ -988,6 +986,10 @@ int tiles_backward(int dtype, const Prompt &p, cudaStream_t stream) {
         auto *keys = &key_gradient_tiles<T, kDim>;
         if (const int e = allow_shared(rows, backward_bytes<kDim>())) return e;
         if (const int e = allow_shared(keys, backward_bytes<kDim>())) return e;
+        if (const int e = encode(&maps.q, dtype, p.q, p.q.row, p.seqs.q_rows, w.heads, w.dim, group, per_tile)) return e;
+        if (const int e = encode(&maps.dout, dtype, p.dout, p.dout.row, p.seqs.q_rows, w.heads, w.dim, group, per_tile)) return e;
+        if (const int e = encode(&maps.k, dtype, p.k, p.k.row, p.seqs.k_rows, w.kv_heads, w.dim, 1, kRows)) return e;
+        if (const int e = encode(&maps.v, dtype, p.v, p.v.row, p.seqs.k_rows, w.kv_heads, w.dim, 1, kRows)) return e;
         const int slots = tile_slots(p.seqs.q_offsets, p.seqs.n_seq, p.seqs.q_rows, per_tile);
         rows<<<dim3(slots, w.kv_heads), kTileThreads, backward_bytes<kDim>(), stream>>>(maps, p);
         RODE_CHECK_LAUNCH("query_gradient_tiles");
@@ -1003,14 +1005,14 @@ int tiles_shared(int dtype, const Cached &c, int first_split, int splits, cudaSt
     const Window &w = c.win;
     const int group = w.heads / w.kv_heads, per_tile = kRows / group;
     TileMaps maps;
-    if (const int e = encode(&maps.q, dtype, c.q, c.q.batch, c.batch, w.heads, w.dim, group, per_tile)) return e;
-    if (const int e = encode(&maps.k, dtype, c.pk, c.pk.row, c.prefix, w.kv_heads, w.dim, 1, kRows)) return e;
-    if (const int e = encode(&maps.v, dtype, c.pv, c.pv.row, c.prefix, w.kv_heads, w.dim, 1, kRows)) return e;
     return by_half(dtype, w.dim, [&](auto *type, auto dim) {
         using T = std::remove_pointer_t<decltype(type)>;
         constexpr int kDim = decltype(dim)::value;
         auto *kernel = &forward_tiles<T, kDim, true>;
         if (const int e = allow_shared(kernel, forward_bytes<kDim>())) return e;
+        if (const int e = encode(&maps.q, dtype, c.q, c.q.batch, c.batch, w.heads, w.dim, group, per_tile)) return e;
+        if (const int e = encode(&maps.k, dtype, c.pk, c.pk.row, c.prefix, w.kv_heads, w.dim, 1, kRows)) return e;
+        if (const int e = encode(&maps.v, dtype, c.pv, c.pv.row, c.prefix, w.kv_heads, w.dim, 1, kRows)) return e;
         const int tiles = (c.batch + 2 * per_tile - 1) / (2 * per_tile);
         kernel<<<dim3(tiles, w.kv_heads, splits), kTileThreads, forward_bytes<kDim>(), stream>>>(maps, Prompt{}, c, first_split, splits);
         RODE_CHECK_LAUNCH("forward_tiles");

@@ -278,3 +278,24 @@ def test_refusals():
     big = torch.zeros(4, 2, 260, device="cuda")
     with pytest.raises(ValueError, match="multiple of 4, at most 256"):
         f(big, big, big, 3)
+
+
+def test_from_a_thread_without_a_context():
+    """A host thread whose first call of CUDA is ours (its memory comes from what the allocator holds already)."""
+    import threading
+
+    from rode_b200.rode_attention import rode_window_attention
+
+    q, k, v, dout = _make([100], [100], 4, 2, 64, torch.bfloat16, seed=11)
+    want = _run(q, k, v, dout, 30, 2)
+    got = []
+
+    def work():
+        got.append(rode_window_attention(q, k, v, 30, 2))
+
+    for _ in range(2):
+        t = threading.Thread(target=work)
+        t.start()
+        t.join()
+    torch.cuda.synchronize()
+    assert len(got) == 2 and all(torch.equal(x, want["out"]) for x in got)
