@@ -39,6 +39,27 @@ __device__ __forceinline__ void clear_rows(uint32_t tile, int panels, int have) 
     __syncwarp();
 }
 
+// The columns of a tile that a row sees: column j when j < to and (j >= from or j < sink).
+struct Range {
+    int from, to, sink;
+};
+
+__device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1; }
+
+// Columns that are not seen become `value`.  By words of 32 bits, whose tests cost two instructions per column; the empty statement keeps
+// the compiler from running them, predicated off, for blocks that are seen whole too (1040 clocks of a block's 5000).
+template <int n>
+__device__ __forceinline__ void hide(uint32_t (&x)[n], const Range &r, uint32_t value) {
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int c = 0; c < n; c += 32) {
+        const uint32_t seen = bits_below(r.to - c) & (~bits_below(r.from - c) | bits_below(r.sink - c));
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+            if (!(seen >> j & 1)) x[c + j] = value;
+    }
+}
+
 // What a CTA works on: two tiles of rows, the blocks of keys that any of them sees.
 struct Work {
     long long row0;     // first query (of the packed operand, or first request)
@@ -113,12 +134,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         return k0 <= b && (k0 + kRows - 1 > a - w.window || k0 < w.sinks);
     };
 
-    const uint32_t base = (shared_address(shared_raw) + 1023) & ~1023u;
+    const uint32_t base = uniform((shared_address(shared_raw) + 1023) & ~1023u);
     const uint32_t qs = base, ks = qs + 2 * kTile, vs = ks + kStages * kTile, bars = vs + kStages * kTile;
-    const uint32_t q_full = bars, v_raw = bars + 8, s_full = bars + 16, p_full = bars + 32, o_done = bars + 48, k_full = bars + 64,
+    const uint32_t q_full = bars, v_raw = bars + 8, s_full = bars + 16, o_done = bars + 32, p_full = bars + 48, k_full = bars + 80,
                    k_empty = k_full + 8 * kStages, v_full = k_empty + 8 * kStages, v_empty = v_full + 8 * kStages,
                    tmem_at = v_empty + 8 * kStages;
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int warp = uniform(threadIdx.x / 32), lane = threadIdx.x % 32;
     if (warp == 8) {
         tmem_alloc(tmem_at, 512);
         if (lane == 0) {
@@ -126,14 +147,15 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             barrier_init(v_raw, 1);
             for (int t = 0; t < 2; ++t) {
                 barrier_init(s_full + 8 * t, 1);
-                barrier_init(p_full + 8 * t, 128);
+                barrier_init(p_full + 16 * t, 128);
+                barrier_init(p_full + 16 * t + 8, 128);
                 barrier_init(o_done + 8 * t, 1);
             }
             for (int i = 0; i < kStages; ++i) {
                 barrier_init(k_full + 8 * i, 1);
-                barrier_init(k_empty + 8 * i, 1);
+                barrier_init(k_empty + 8 * i, 2);
                 barrier_init(v_full + 8 * i, 1);
-                barrier_init(v_empty + 8 * i, 1);
+                barrier_init(v_empty + 8 * i, 2);
             }
             barrier_init_done();
         }
@@ -144,6 +166,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     tmem_fence_after();
     uint32_t tmem;
     asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem) : "r"(tmem_at));
+    tmem = uniform(tmem);
     bool ok = true;  // (a wait that was given up ends the CTA's work; it took seconds, so that no copy is in flight any more)
 
     if (warp >= 8) give_registers();
@@ -181,63 +204,64 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 if (lane == 0) barrier_arrive(v_full + 8 * st);
             }
         }
-    } else if (warp == 8) {
-        // products
+    } else if (warp == 8 || warp == 10) {
+        // products, one warp per tile, so that a wait for one tile holds up nothing of the other
+        const int t = warp == 8 ? 0 : 1;
         const uint32_t scores = product_descriptor<T>(kRows, false), values = product_descriptor<T>((w.dim + 15) / 16 * 16, true);
+        const uint32_t one = elect_one();
         const int steps = (w.dim + 15) / 16;
-        int waiting[2] = {0, 0}, issued[2] = {0, 0}, weights[2] = {0, 0};
-        const auto issue_scores = [&](int t, int st) {
-            if (lane == 0) {
-                for (int s = 0; s < steps; ++s) {
-                    const uint32_t at = s / 4 * kPanel + s % 4 * 32;
-                    product(tmem + t * kRows, tile_descriptor(qs + t * kTile + at, 16), tile_descriptor(ks + st * kTile + at, 16), scores,
-                            s > 0);
-                }
-                products_arrive(s_full + 8 * t);
-            }
-        };
-        if (wk.blocks > 0) {
-            ok = barrier_wait(q_full, 0) && barrier_wait(k_full, 0);
-            tmem_fence_after();
-            if (ok) {
-                for (int t = 0; t < 2; ++t)
-                    if (sees_block(t, wk.key_of(0))) issue_scores(t, 0);
-                if (lane == 0) products_arrive(k_empty);
-            }
-        }
-        for (int i = 0; i < wk.blocks && ok; ++i) {
-            const int st = i % kStages, k0 = wk.key_of(i);
-            const bool more = i + 1 < wk.blocks;
-            const int next = (i + 1) % kStages, k1 = more ? wk.key_of(i + 1) : 0;
-            ok = barrier_wait(v_full + 8 * st, i / kStages & 1) && (!more || barrier_wait(k_full + 8 * next, (i + 1) / kStages & 1));
-            for (int t = 0; t < 2 && ok; ++t) {
-                if (sees_block(t, k0)) {
-                    ok = barrier_wait(p_full + 8 * t, weights[t]++ & 1);
-                    if (!ok) break;
-                    tmem_fence_after();
-                    if (lane == 0) {
-                        for (int s = 0; s < kRows / 16; ++s)
-                            product_from_tmem(tmem + 256 + t * kDim, tmem + t * kRows + s * 8,
-                                              tile_descriptor(vs + st * kTile + s * 2048, kPanel), values, issued[t] > 0 || s > 0);
-                        products_arrive(o_done + 8 * t);
+        const uint32_t s_at = tmem + t * kRows, o_at = tmem + 256 + t * kDim;
+        const auto issue_scores = [&](int i) {  // of block i, and its keys' stage is done with
+            const int st = i % kStages;
+            ok = barrier_wait(k_full + 8 * st, i / kStages & 1);
+            if (!ok) return;
+            if (sees_block(t, wk.key_of(i))) {
+                tmem_fence_after();
+                const uint64_t a = tile_descriptor(qs + t * kTile, 16), b = tile_descriptor(ks + st * kTile, 16);
+#pragma unroll
+                for (int s = 0; s < kDim / 16; ++s)
+                    if (s < steps) {
+                        const uint32_t at = (s / 4 * kPanel + s % 4 * 32) >> 4;
+                        product(one, s_at, a + at, b + at, scores, s > 0);
                     }
-                    ++issued[t];
-                }
-                if (more && sees_block(t, k1)) {
-                    // the next scores go where the weights were
-                    if (waiting[t] < issued[t]) {
-                        waiting[t] = issued[t];
-                        ok = barrier_wait(o_done + 8 * t, (issued[t] - 1) & 1);
-                        if (!ok) break;
-                    }
-                    issue_scores(t, next);
-                }
-            }
-            if (ok && lane == 0) {
-                products_arrive(v_empty + 8 * st);
-                if (more) products_arrive(k_empty + 8 * next);
+                products_arrive(one, s_full + 8 * t);
+                products_arrive(one, k_empty + 8 * st);
+            } else if (one) {
+                barrier_arrive(k_empty + 8 * st);
             }
             __syncwarp();
+        };
+        int issued = 0;
+        if (wk.blocks > 0) {
+            ok = barrier_wait(q_full, 0);
+            if (ok) issue_scores(0);
+        }
+        for (int i = 0; i < wk.blocks && ok; ++i) {
+            const int st = i % kStages;
+            ok = barrier_wait(v_full + 8 * st, i / kStages & 1);
+            if (!ok) break;
+            if (sees_block(t, wk.key_of(i))) {
+                const uint64_t b = tile_descriptor(vs + st * kTile, kPanel);
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    ok = ok && barrier_wait(p_full + 16 * t + 8 * half, issued & 1);
+                    tmem_fence_after();
+                    if (ok)
+#pragma unroll
+                        for (int s = 4 * half; s < 4 * half + 4; ++s)
+                            product_from_tmem(one, o_at, s_at + s * 8, b + s * 128, values, issued > 0 || s > 0);
+                }
+                if (!ok) break;
+                products_arrive(one, o_done + 8 * t);
+                products_arrive(one, v_empty + 8 * st);
+                // the next scores go where the weights were
+                ok = barrier_wait(o_done + 8 * t, issued & 1);
+                ++issued;
+            } else if (one) {
+                barrier_arrive(v_empty + 8 * st);
+            }
+            __syncwarp();
+            if (ok && i + 1 < wk.blocks) issue_scores(i + 1);
         }
     } else if (warp < 8) {
         // softmax: one row per thread
@@ -272,11 +296,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             else
                 whole = k0 + kRows - 1 <= a && (a + n - 1 - k0 < w.window || k0 + kRows <= w.sinks);
             if (!whole) {
-                const int last = kShared ? wk.keys - 1 - k0 : pos - k0;                  // columns up to this one
-                const int from = kShared ? 0 : pos - w.window + 1 - k0, sink = kShared ? 0 : w.sinks - k0;
-#pragma unroll
-                for (int j = 0; j < 128; ++j)
-                    if (j > last || (j < from && j >= sink)) s[j] = 0xff800000u;  // -infinity
+                if constexpr (kShared)
+                    hide(s, {0, wk.keys - k0, 0}, 0xff800000u);  // -infinity
+                else
+                    hide(s, {pos - w.window + 1 - k0, pos + 1 - k0, w.sinks - k0}, 0xff800000u);
             }
             float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -303,20 +326,25 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             const float off = m == -INFINITY ? 0.f : -m * s2;
             float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int j = 0; j < 128; j += 2) {
-                float x = fmaf(__uint_as_float(s[j]), s2, off), y = fmaf(__uint_as_float(s[j + 1]), s2, off);
-                asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(x));
-                asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(y));
-                sum[j / 2 % 2 * 2] += x;
-                sum[j / 2 % 2 * 2 + 1] += y;
-                s[j / 2] = pack2<T>(x, y);
+            for (int half = 0; half < 2; ++half) {  // the first half's products run during the second half's exponentials
+#pragma unroll
+                for (int j = 64 * half; j < 64 * half + 64; j += 2) {
+                    float x = fmaf(__uint_as_float(s[j]), s2, off), y = fmaf(__uint_as_float(s[j + 1]), s2, off);
+                    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(x));
+                    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(y));
+                    sum[j / 2 % 2 * 2] += x;
+                    sum[j / 2 % 2 * 2 + 1] += y;
+                    s[j / 2] = pack2<T>(x, y);
+                }
+                if (half == 0)
+                    tmem_store32<0>(s_at, s);
+                else
+                    tmem_store32<32>(s_at + 32, s);
+                tmem_wait_store();
+                tmem_fence_before();
+                barrier_arrive(p_full + 16 * t + 8 * half);
             }
             l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-            tmem_store32<0>(s_at, s);
-            tmem_store32<32>(s_at + 32, s);
-            tmem_wait_store();
-            tmem_fence_before();
-            barrier_arrive(p_full + 8 * t);
             ++done;
         }
         if (ok && done > 0) {
@@ -394,17 +422,6 @@ struct GradientMaps {
     CUtensorMap q, dout, k, v;
 };
 
-// Columns [64 half, 64 half + 64) of a tile's P and dS from S and dP in registers; columns out of [from, to) (or below sink) see nothing.
-struct Range {
-    int from, to, sink;  // sees column j when j < to and (j >= from or j < sink)
-};
-
-__device__ __forceinline__ void hide(uint32_t (&x)[64], const Range &r, uint32_t value) {
-#pragma unroll
-    for (int j = 0; j < 64; ++j)
-        if (j >= r.to || (j < r.from && j >= r.sink)) x[j] = value;
-}
-
 // 16-byte pieces of a row: sum of products.
 template <typename T>
 __device__ __forceinline__ float dot_row(const T *a, const T *b, int dim) {
@@ -452,12 +469,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) query_gradient_tiles(const __
     const int n = min(per_tile, t.rows - t.first), pos0 = t.first + keys.y - t.rows;
     const KeyBlocks blocks(pos0, pos0 + n, w.window, w.sinks, kRows);
 
-    const uint32_t base = (shared_address(shared_raw) + 1023) & ~1023u;
+    const uint32_t base = uniform((shared_address(shared_raw) + 1023) & ~1023u);
     const uint32_t qs = base, gs = qs + kTile, ks = gs + kTile, vs = ks + kStages * kTile, bars = vs + kStages * kTile;
     const uint32_t q_full = bars, k_raw = bars + 8, s_full = bars + 16, dp_full = bars + 32, ds_full = bars + 40, dq_done = bars + 48,
                    k_full = bars + 64, k_empty = k_full + 8 * kStages, v_full = k_empty + 8 * kStages, v_empty = v_full + 8 * kStages,
                    tmem_at = v_empty + 8 * kStages;
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int warp = uniform(threadIdx.x / 32), lane = threadIdx.x % 32;
     if (warp == 8) {
         tmem_alloc(tmem_at, 512);
         if (lane == 0) {
@@ -483,6 +500,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) query_gradient_tiles(const __
     tmem_fence_after();
     uint32_t tmem;
     asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem) : "r"(tmem_at));
+    tmem = uniform(tmem);
     const uint32_t dp_at = tmem + 256, dq_at = tmem + 384;
     bool ok = true;
 
@@ -521,14 +539,16 @@ __global__ void __launch_bounds__(kTileThreads, 1) query_gradient_tiles(const __
     } else if (warp == 8) {
         const uint32_t scores = product_descriptor<T>(kRows, false), sums = product_descriptor<T>((w.dim + 15) / 16 * 16, true);
         const int steps = (w.dim + 15) / 16;
+        const uint32_t one = elect_one();
         const auto issue = [&](uint32_t d, uint32_t a, uint32_t b, uint32_t bar) {
-            if (lane == 0) {
-                for (int s = 0; s < steps; ++s) {
-                    const uint32_t at = s / 4 * kPanel + s % 4 * 32;
-                    product(d, tile_descriptor(a + at, 16), tile_descriptor(b + at, 16), scores, s > 0);
+            const uint64_t x = tile_descriptor(a, 16), y = tile_descriptor(b, 16);
+#pragma unroll
+            for (int s = 0; s < kDim / 16; ++s)
+                if (s < steps) {
+                    const uint32_t at = (s / 4 * kPanel + s % 4 * 32) >> 4;
+                    product(one, d, x + at, y + at, scores, s > 0);
                 }
-                products_arrive(bar);
-            }
+            products_arrive(one, bar);
         };
         if (blocks.n > 0) {
             ok = barrier_wait(q_full, 0) && barrier_wait(k_full, 0) && barrier_wait(v_full, 0);
@@ -536,7 +556,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) query_gradient_tiles(const __
             if (ok) {
                 issue(tmem, qs, ks, s_full);
                 issue(dp_at, gs, vs, dp_full);
-                if (lane == 0) products_arrive(v_empty);
+                products_arrive(one, v_empty);
             }
         }
         for (int i = 0; i < blocks.n && ok; ++i) {
@@ -556,18 +576,17 @@ __global__ void __launch_bounds__(kTileThreads, 1) query_gradient_tiles(const __
             ok = barrier_wait(ds_full, i & 1);
             if (!ok) break;
             tmem_fence_after();
-            if (lane == 0) {
-                for (int s = 0; s < kRows / 16; ++s)
-                    product_from_tmem(dq_at, tmem + buf * kRows + s / 4 * 64 + s % 4 * 8, tile_descriptor(ks + st * kTile + s * 2048, kPanel),
-                                      sums, i > 0 || s > 0);
-                products_arrive(dq_done);
-                products_arrive(k_empty + 8 * st);
-            }
+            const uint64_t keys_of_block = tile_descriptor(ks + st * kTile, kPanel);
+#pragma unroll
+            for (int s = 0; s < kRows / 16; ++s)
+                product_from_tmem(one, dq_at, tmem + buf * kRows + s / 4 * 64 + s % 4 * 8, keys_of_block + s * 128, sums, i > 0 || s > 0);
+            products_arrive(one, dq_done);
+            products_arrive(one, k_empty + 8 * st);
             if (more) {
                 ok = barrier_wait(v_full + 8 * next, next_full);
                 if (!ok) break;
                 issue(dp_at, gs, vs + next * kTile, dp_full);
-                if (lane == 0) products_arrive(v_empty + 8 * next);
+                products_arrive(one, v_empty + 8 * next);
             }
             __syncwarp();
         }
@@ -657,13 +676,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) key_gradient_tiles(const __gr
     const int last = t.first < w.sinks || w.window >= t.rows - (t.first + have - 1) ? t.rows : t.first + have - 1 + w.window;
     const int i0 = max(t.first - shift, 0), i1 = max(min(last - shift, queries.y), i0), tiles = (i1 - i0 + per_tile - 1) / per_tile;
 
-    const uint32_t base = (shared_address(shared_raw) + 1023) & ~1023u;
+    const uint32_t base = uniform((shared_address(shared_raw) + 1023) & ~1023u);
     const uint32_t ks = base, vs = ks + kTile, qs = vs + kTile, gs = qs + kStages * kTile, rows_at = gs + kStages * kTile,
                    bars = rows_at + kStages * 2 * kRows * 4;
     const uint32_t k_full = bars, raw = bars + 8, s_full = bars + 16, p_full = bars + 24, dp_full = bars + 32, ds_full = bars + 40,
                    dv_done = bars + 48, dk_done = bars + 56, q_full = bars + 64, q_empty = q_full + 8 * kStages, g_full = q_empty + 8 * kStages,
                    g_empty = g_full + 8 * kStages, rows_full = g_empty + 8 * kStages, tmem_at = rows_full + 8 * kStages;
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int warp = uniform(threadIdx.x / 32), lane = threadIdx.x % 32;
     if (warp == 8) {
         tmem_alloc(tmem_at, 512);
         if (lane == 0) {
@@ -691,6 +710,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) key_gradient_tiles(const __gr
     tmem_fence_after();
     uint32_t tmem;
     asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem) : "r"(tmem_at));
+    tmem = uniform(tmem);
     const uint32_t dp_at = tmem + 128, dv_at = tmem + 256, dk_at = tmem + 384;
     bool ok = true;
 
@@ -753,22 +773,24 @@ __global__ void __launch_bounds__(kTileThreads, 1) key_gradient_tiles(const __gr
     } else if (warp == 8) {
         const uint32_t scores = product_descriptor<T>(kRows, false), sums = product_descriptor<T>((w.dim + 15) / 16 * 16, true);
         const int steps = (w.dim + 15) / 16;
+        const uint32_t one = elect_one();
         const auto issue = [&](uint32_t d, uint32_t a, uint32_t b, uint32_t bar) {
-            if (lane == 0) {
-                for (int s = 0; s < steps; ++s) {
-                    const uint32_t at = s / 4 * kPanel + s % 4 * 32;
-                    product(d, tile_descriptor(a + at, 16), tile_descriptor(b + at, 16), scores, s > 0);
+            const uint64_t x = tile_descriptor(a, 16), y = tile_descriptor(b, 16);
+#pragma unroll
+            for (int s = 0; s < kDim / 16; ++s)
+                if (s < steps) {
+                    const uint32_t at = (s / 4 * kPanel + s % 4 * 32) >> 4;
+                    product(one, d, x + at, y + at, scores, s > 0);
                 }
-                products_arrive(bar);
-            }
+            products_arrive(one, bar);
         };
         const auto add_up = [&](uint32_t d, uint32_t a, uint32_t b, bool add, uint32_t bar, uint32_t free) {
-            if (lane == 0) {
-                for (int s = 0; s < kRows / 16; ++s)
-                    product_from_tmem(d, a + s / 4 * 64 + s % 4 * 8, tile_descriptor(b + s * 2048, kPanel), sums, add || s > 0);
-                products_arrive(bar);
-                products_arrive(free);
-            }
+            const uint64_t y = tile_descriptor(b, kPanel);
+#pragma unroll
+            for (int s = 0; s < kRows / 16; ++s)
+                product_from_tmem(one, d, a + s / 4 * 64 + s % 4 * 8, y + s * 128, sums, add || s > 0);
+            products_arrive(one, bar);
+            products_arrive(one, free);
         };
         if (tiles > 0) {
             ok = barrier_wait(k_full, 0) && barrier_wait(q_full, 0) && barrier_wait(g_full, 0);

@@ -140,23 +140,38 @@ __device__ __forceinline__ uint32_t product_descriptor(int n, bool b_rows) {
     return 1u << 4 | type << 7 | type << 10 | (b_rows ? 1u << 16 : 0u) | static_cast<uint32_t>(n >> 3) << 17 | (128u >> 4) << 24;
 }
 
-// d (+)= a b over 16 summands; a in shared memory, or in tensor memory (two elements per column).  One thread issues.
-__device__ __forceinline__ void product(uint32_t d, uint64_t a, uint64_t b, uint32_t shape, bool add) {
+// One thread of a warp issues products and their arrivals.  The whole warp runs the code, with its operands in uniform registers, and the
+// instruction is predicated on the elected thread: 64 clocks per 128 x 128 x 16 product, the tensor core's own time, where code
+// behind a branch on the lane took 70 (128 x 64: 37 instead of 72).
+__device__ __forceinline__ uint32_t elect_one() {
+    uint32_t one;
+    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(one));
+    return one;
+}
+// d (+)= a b over 16 summands; a in shared memory, or in tensor memory (two elements per column).
+__device__ __forceinline__ void product(uint32_t one, uint32_t d, uint64_t a, uint64_t b, uint32_t shape, bool add) {
     asm volatile(
-        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a), "l"(b),
-        "r"(shape), "r"(static_cast<uint32_t>(add))
+        "{\n.reg .pred p, q;\nsetp.ne.b32 p, %4, 0;\nsetp.ne.b32 q, %5, 0;\n@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(
+            d),
+        "l"(a), "l"(b), "r"(shape), "r"(static_cast<uint32_t>(add)), "r"(one)
         : "memory");
 }
-__device__ __forceinline__ void product_from_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t shape, bool add) {
+__device__ __forceinline__ void product_from_tmem(uint32_t one, uint32_t d, uint32_t a, uint64_t b, uint32_t shape, bool add) {
     asm volatile(
-        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d), "r"(a), "l"(b),
-        "r"(shape), "r"(static_cast<uint32_t>(add))
+        "{\n.reg .pred p, q;\nsetp.ne.b32 p, %4, 0;\nsetp.ne.b32 q, %5, 0;\n@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, "
+        "p;\n}" ::"r"(d),
+        "r"(a), "l"(b), "r"(shape), "r"(static_cast<uint32_t>(add)), "r"(one)
         : "memory");
 }
 // The barrier gets one arrival when all products that this thread has issued are complete.
-__device__ __forceinline__ void products_arrive(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+__device__ __forceinline__ void products_arrive(uint32_t one, uint32_t bar) {
+    asm volatile(
+        "{\n.reg .pred q;\nsetp.ne.b32 q, %1, 0;\n@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}" ::"r"(bar),
+        "r"(one)
+        : "memory");
 }
+// The value of lane 0, for the compiler to know that it is the same in all lanes.
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
 
 // Two numbers rounded to the 16-bit type, the first in the low half.
 template <typename T>
