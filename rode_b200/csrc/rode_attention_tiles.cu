@@ -60,6 +60,120 @@ __device__ __forceinline__ void hide(uint32_t (&x)[n], const Range &r, uint32_t 
     }
 }
 
+// Two numbers in one 64-bit register: one instruction for both.
+struct Pair {
+    unsigned long long x;
+};
+__device__ __forceinline__ Pair pair_of(float a, float b) {
+    Pair r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r.x) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void split(Pair p, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p.x)); }
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+    Pair r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.x) : "l"(a.x), "l"(b.x), "l"(c.x));
+    return r;
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+    Pair r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.x) : "l"(a.x), "l"(b.x));
+    return r;
+}
+
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+    Pair r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.x) : "l"(a.x), "l"(b.x));
+    return r;
+}
+__device__ __forceinline__ Pair load_pair(uint32_t shared) {
+    Pair r;
+    asm volatile("ld.shared.b64 %0, [%1];" : "=l"(r.x) : "r"(shared));
+    return r;
+}
+
+// 2^x by additions and products, for x <= 128 (below -125: as -125): x = n + f with f in [-1/2, 1/2], 2^f by the polynomial of degree 4
+// with the least relative error there (Remez' exchange, 2.7e-6 after rounding its coefficients, far below the rounding of the weights to 16 bits), n
+// added to its exponent.  Adding 1.5 * 2^23 rounds to an integer, whose bits shifted by 23 are n alone.  NaN gives something not finite in 16 bits.
+__device__ __forceinline__ void exp2_by_fma(Pair x, float &a, float &b) {
+    split(x, a, b);
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(-125.f));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(b) : "f"(-125.f));
+    x = pair_of(a, b);
+    const Pair t = add2(x, pair_of(12582912.f, 12582912.f));
+    const Pair f = fma2(add2(t, pair_of(-12582912.f, -12582912.f)), pair_of(-1.f, -1.f), x);
+    Pair p = fma2(f, pair_of(0x1.3997d6p-7f, 0x1.3997d6p-7f), pair_of(0x1.ca1440p-5f, 0x1.ca1440p-5f));
+    p = fma2(f, p, pair_of(0x1.ec06dap-3f, 0x1.ec06dap-3f));
+    p = fma2(f, p, pair_of(0x1.62e0dcp-1f, 0x1.62e0dcp-1f));
+    p = fma2(f, p, pair_of(0x1.ffffe8p-1f, 0x1.ffffe8p-1f));
+    float na, nb;
+    split(t, na, nb);
+    split(p, a, b);
+    a = __uint_as_float(__float_as_uint(a) + (__float_as_uint(na) << 23));
+    b = __uint_as_float(__float_as_uint(b) + (__float_as_uint(nb) << 23));
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(x));
+    return x;
+}
+
+// Scores o .. o + 63 to weights 2^(s2 x + off), packed in pairs into registers o / 2 ..; their sum is added.  The exponential unit makes 16 of
+// them per clock and SM, which would take as long as the products: kByFma of every 8 pairs go to the FMA units instead (not in blocks with
+// hidden columns, whose weights are exactly 0).
+template <typename T, int o, int kByFma>
+__device__ __forceinline__ void weights_of(uint32_t (&s)[128], float s2, float off, Pair &sum) {
+    const Pair factor = pair_of(s2, s2), shift = pair_of(off, off);
+#pragma unroll
+    for (int j = o; j < o + 64; j += 2) {
+        const Pair x = fma2(pair_of(__uint_as_float(s[j]), __uint_as_float(s[j + 1])), factor, shift);
+        float a, b;
+        if (j / 2 % 8 < kByFma) {
+            exp2_by_fma(x, a, b);
+        } else {
+            split(x, a, b);
+            a = exp2_fast(a);
+            b = exp2_fast(b);
+        }
+        sum = add2(sum, pair_of(a, b));
+        s[j / 2] = pack2<T>(a, b);
+    }
+}
+constexpr int kByFma = 2;
+
+// Gradients: weights 2^(s2 x + off), left in 32 bits, of columns o .. o + 31 of a thread's 64.  The two warpgroups of a tile are at it side by side,
+// so more go to the FMA units.
+constexpr int kByFmaInPairs = 3;
+template <int o, int kByFma, typename Off>
+__device__ __forceinline__ void weights_in_place(uint32_t (&s)[64], float s2, Off &&off) {
+    const Pair factor = pair_of(s2, s2);
+#pragma unroll
+    for (int j = o; j < o + 32; j += 2) {
+        const Pair x = fma2(pair_of(__uint_as_float(s[j]), __uint_as_float(s[j + 1])), factor, off(j));
+        float a, b;
+        if (j / 2 % 8 < kByFma) {
+            exp2_by_fma(x, a, b);
+        } else {
+            split(x, a, b);
+            a = exp2_fast(a);
+            b = exp2_fast(b);
+        }
+        s[j] = __float_as_uint(a);
+        s[j + 1] = __float_as_uint(b);
+    }
+}
+// P (dP - delta) of columns o .. o + 31, rounded, in registers o / 2 .. of s (whose P it takes).
+template <typename T, int o, typename Minus>
+__device__ __forceinline__ void gradients_in_place(uint32_t (&s)[64], const uint32_t (&d)[64], Minus &&minus) {
+#pragma unroll
+    for (int j = o; j < o + 32; j += 2) {
+        const Pair x = mul2(pair_of(__uint_as_float(s[j]), __uint_as_float(s[j + 1])),
+                            add2(pair_of(__uint_as_float(d[j]), __uint_as_float(d[j + 1])), minus(j)));
+        float a, b;
+        split(x, a, b);
+        s[j / 2] = pack2<T>(a, b);
+    }
+}
+
 // What a CTA works on: two tiles of rows, the blocks of keys that any of them sees.
 struct Work {
     long long row0;     // first query (of the packed operand, or first request)
@@ -136,7 +250,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 
     const uint32_t base = uniform((shared_address(shared_raw) + 1023) & ~1023u);
     const uint32_t qs = base, ks = qs + 2 * kTile, vs = ks + kStages * kTile, bars = vs + kStages * kTile;
-    const uint32_t q_full = bars, v_raw = bars + 8, s_full = bars + 16, o_done = bars + 32, p_full = bars + 48, k_full = bars + 80,
+    const uint32_t q_full = bars, v_raw = bars + 8, s_full = bars + 16, o_done = bars + 32, p_full = bars + 48, turn = bars + 80, k_full = bars + 96,
                    k_empty = k_full + 8 * kStages, v_full = k_empty + 8 * kStages, v_empty = v_full + 8 * kStages,
                    tmem_at = v_empty + 8 * kStages;
     const int warp = uniform(threadIdx.x / 32), lane = threadIdx.x % 32;
@@ -145,6 +259,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         if (lane == 0) {
             barrier_init(q_full, 1);
             barrier_init(v_raw, 1);
+            barrier_init(turn, 128);
+            barrier_init(turn + 8, 128);
             for (int t = 0; t < 2; ++t) {
                 barrier_init(s_full + 8 * t, 1);
                 barrier_init(p_full + 16 * t, 128);
@@ -275,9 +391,19 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         const float s2 = w.scale * kLog2e;
         float m = -INFINITY, l = 0.f;
         int done = 0;
+        // The tiles' exponentials take turns: side by side they would take twice as long and then wait for the products side by side
+        // (blocks of both tiles in 3250 clocks instead of 3800).
+        const bool turns = queries_of(1) > 0;
         for (int i = 0; i < wk.blocks; ++i) {
             const int k0 = wk.key_of(i);
-            if (!sees_block(t, k0)) continue;
+            if (!sees_block(t, k0)) {
+                if (turns) {
+                    ok = barrier_wait(turn + 8 * t, (i + t + 1) & 1);
+                    if (!ok) break;
+                    barrier_arrive(turn + 8 * (t ^ 1));
+                }
+                continue;
+            }
             ok = barrier_wait(s_full + 8 * t, done & 1);
             if (!ok) break;
             tmem_fence_after();
@@ -303,7 +429,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             }
             float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int j = 0; j < 128; ++j) top[j % 4] = fmaxf(top[j % 4], __uint_as_float(s[j]));
+            for (int j = 0; j < 128; j += 2)
+                top[j / 2 % 4] = fmaxf(top[j / 2 % 4], fmaxf(__uint_as_float(s[j]), __uint_as_float(s[j + 1])));
             const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
             const bool grows = (high - m) * s2 > kLazy;
             if (__any_sync(0xffffffffu, grows)) {
@@ -324,27 +451,32 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 }
             }
             const float off = m == -INFINITY ? 0.f : -m * s2;
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {  // the first half's products run during the second half's exponentials
-#pragma unroll
-                for (int j = 64 * half; j < 64 * half + 64; j += 2) {
-                    float x = fmaf(__uint_as_float(s[j]), s2, off), y = fmaf(__uint_as_float(s[j + 1]), s2, off);
-                    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(x));
-                    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(y));
-                    sum[j / 2 % 2 * 2] += x;
-                    sum[j / 2 % 2 * 2 + 1] += y;
-                    s[j / 2] = pack2<T>(x, y);
-                }
-                if (half == 0)
-                    tmem_store32<0>(s_at, s);
-                else
-                    tmem_store32<32>(s_at + 32, s);
-                tmem_wait_store();
-                tmem_fence_before();
-                barrier_arrive(p_full + 16 * t + 8 * half);
+            if (turns) {
+                ok = barrier_wait(turn + 8 * t, (i + t + 1) & 1);
+                if (!ok) break;
             }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            // the first half's products run during the second half's exponentials
+            Pair sum = pair_of(0.f, 0.f);
+            if (whole)
+                weights_of<T, 0, kByFma>(s, s2, off, sum);
+            else
+                weights_of<T, 0, 0>(s, s2, off, sum);
+            tmem_store32<0>(s_at, s);
+            tmem_wait_store();
+            tmem_fence_before();
+            barrier_arrive(p_full + 16 * t);
+            if (whole)
+                weights_of<T, 64, kByFma>(s, s2, off, sum);
+            else
+                weights_of<T, 64, 0>(s, s2, off, sum);
+            tmem_store32<32>(s_at + 32, s);
+            tmem_wait_store();
+            tmem_fence_before();
+            barrier_arrive(p_full + 16 * t + 8);
+            if (turns) barrier_arrive(turn + 8 * (t ^ 1));
+            float even, odd;
+            split(sum, even, odd);
+            l += even + odd;
             ++done;
         }
         if (ok && done > 0) {
@@ -471,7 +603,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) query_gradient_tiles(const __
 
     const uint32_t base = uniform((shared_address(shared_raw) + 1023) & ~1023u);
     const uint32_t qs = base, gs = qs + kTile, ks = gs + kTile, vs = ks + kStages * kTile, bars = vs + kStages * kTile;
-    const uint32_t q_full = bars, k_raw = bars + 8, s_full = bars + 16, dp_full = bars + 32, ds_full = bars + 40, dq_done = bars + 48,
+    const uint32_t q_full = bars, k_raw = bars + 8, s_full = bars + 16, dp_full = bars + 32, ds_full = bars + 40, dq_done = bars + 56,
                    k_full = bars + 64, k_empty = k_full + 8 * kStages, v_full = k_empty + 8 * kStages, v_empty = v_full + 8 * kStages,
                    tmem_at = v_empty + 8 * kStages;
     const int warp = uniform(threadIdx.x / 32), lane = threadIdx.x % 32;
@@ -484,6 +616,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) query_gradient_tiles(const __
             barrier_init(s_full + 8, 1);
             barrier_init(dp_full, 1);
             barrier_init(ds_full, 256);
+            barrier_init(ds_full + 8, 256);
             barrier_init(dq_done, 1);
             for (int i = 0; i < kStages; ++i) {
                 barrier_init(k_full + 8 * i, 1);
@@ -573,13 +706,20 @@ __global__ void __launch_bounds__(kTileThreads, 1) query_gradient_tiles(const __
                 tmem_fence_after();
                 issue(tmem + (buf ^ 1) * kRows, qs, ks + next * kTile, s_full + 8 * (buf ^ 1));
             }
-            ok = barrier_wait(ds_full, i & 1);
-            if (!ok) break;
-            tmem_fence_after();
             const uint64_t keys_of_block = tile_descriptor(ks + st * kTile, kPanel);
 #pragma unroll
-            for (int s = 0; s < kRows / 16; ++s)
-                product_from_tmem(one, dq_at, tmem + buf * kRows + s / 4 * 64 + s % 4 * 8, keys_of_block + s * 128, sums, i > 0 || s > 0);
+            for (int piece = 0; piece < 2; ++piece) {  // 32 of each warpgroup's 64 columns
+                ok = ok && barrier_wait(ds_full + 8 * piece, i & 1);
+                tmem_fence_after();
+                if (ok)
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        const int s = u / 2 * 4 + piece * 2 + u % 2;
+                        product_from_tmem(one, dq_at, tmem + buf * kRows + s / 4 * 64 + s % 4 * 8, keys_of_block + s * 128, sums,
+                                          i > 0 || piece > 0 || u > 0);
+                    }
+            }
+            if (!ok) break;
             products_arrive(one, dq_done);
             products_arrive(one, k_empty + 8 * st);
             if (more) {
@@ -619,11 +759,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) query_gradient_tiles(const __
             tmem_wait_load32<0>(s);
             tmem_wait_load32<32>(s);
             if (!whole) hide(s, range, 0xff800000u);
-#pragma unroll
-            for (int j = 0; j < 64; ++j) {
-                float x = fmaf(__uint_as_float(s[j]), s2, off);
-                asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(x));
-                s[j] = __float_as_uint(x);
+            const auto weight_off = [&](int) { return pair_of(off, off); };
+            if (whole) {
+                weights_in_place<0, kByFmaInPairs>(s, s2, weight_off);
+                weights_in_place<32, kByFmaInPairs>(s, s2, weight_off);
+            } else {
+                weights_in_place<0, 0>(s, s2, weight_off);
+                weights_in_place<32, 0>(s, s2, weight_off);
             }
             ok = barrier_wait(dp_full, i & 1);
             if (!ok) break;
@@ -633,14 +775,17 @@ __global__ void __launch_bounds__(kTileThreads, 1) query_gradient_tiles(const __
             tmem_wait_load32<0>(d);
             tmem_wait_load32<32>(d);
             if (!whole) hide(d, range, 0u);
-#pragma unroll
-            for (int j = 0; j < 64; j += 2)
-                s[j / 2] = pack2<T>(__uint_as_float(s[j]) * (__uint_as_float(d[j]) - delta),
-                                    __uint_as_float(s[j + 1]) * (__uint_as_float(d[j + 1]) - delta));
-            tmem_store32<0>(s_at, s);
+            const auto minus = [&](int) { return pair_of(-delta, -delta); };
+            gradients_in_place<T, 0>(s, d, minus);
+            tmem_store16<0>(s_at, s);
             tmem_wait_store();
             tmem_fence_before();
             barrier_arrive(ds_full);
+            gradients_in_place<T, 32>(s, d, minus);
+            tmem_store16<16>(s_at + 16, s);
+            tmem_wait_store();
+            tmem_fence_before();
+            barrier_arrive(ds_full + 8);
         }
         if (ok && blocks.n > 0) {
             ok = barrier_wait(dq_done, (blocks.n - 1) & 1);
@@ -679,8 +824,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) key_gradient_tiles(const __gr
     const uint32_t base = uniform((shared_address(shared_raw) + 1023) & ~1023u);
     const uint32_t ks = base, vs = ks + kTile, qs = vs + kTile, gs = qs + kStages * kTile, rows_at = gs + kStages * kTile,
                    bars = rows_at + kStages * 2 * kRows * 4;
-    const uint32_t k_full = bars, raw = bars + 8, s_full = bars + 16, p_full = bars + 24, dp_full = bars + 32, ds_full = bars + 40,
-                   dv_done = bars + 48, dk_done = bars + 56, q_full = bars + 64, q_empty = q_full + 8 * kStages, g_full = q_empty + 8 * kStages,
+    const uint32_t k_full = bars, raw = bars + 8, s_full = bars + 16, dp_full = bars + 24, p_full = bars + 32, ds_full = bars + 48,
+                   dv_done = bars + 64, dk_done = bars + 72, q_full = bars + 80, q_empty = q_full + 8 * kStages, g_full = q_empty + 8 * kStages,
                    g_empty = g_full + 8 * kStages, rows_full = g_empty + 8 * kStages, tmem_at = rows_full + 8 * kStages;
     const int warp = uniform(threadIdx.x / 32), lane = threadIdx.x % 32;
     if (warp == 8) {
@@ -689,9 +834,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) key_gradient_tiles(const __gr
             barrier_init(k_full, 1);
             barrier_init(raw, 1);
             barrier_init(s_full, 1);
-            barrier_init(p_full, 256);
             barrier_init(dp_full, 1);
-            barrier_init(ds_full, 256);
+            for (int piece = 0; piece < 2; ++piece) {
+                barrier_init(p_full + 8 * piece, 256);
+                barrier_init(ds_full + 8 * piece, 256);
+            }
             barrier_init(dv_done, 1);
             barrier_init(dk_done, 1);
             for (int i = 0; i < kStages; ++i) {
@@ -766,7 +913,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) key_gradient_tiles(const __gr
                     delta = __ldg(p.delta + at);
                 }
                 asm volatile("st.shared.b32 [%0], %1;" ::"r"(rows_at + (st * 2 * kRows + r) * 4), "f"(lse) : "memory");
-                asm volatile("st.shared.b32 [%0], %1;" ::"r"(rows_at + (st * 2 * kRows + kRows + r) * 4), "f"(delta) : "memory");
+                asm volatile("st.shared.b32 [%0], %1;" ::"r"(rows_at + (st * 2 * kRows + kRows + r) * 4), "f"(-delta) : "memory");
             }
             barrier_arrive(rows_full + 8 * st);
         }
@@ -784,11 +931,20 @@ __global__ void __launch_bounds__(kTileThreads, 1) key_gradient_tiles(const __gr
                 }
             products_arrive(one, bar);
         };
-        const auto add_up = [&](uint32_t d, uint32_t a, uint32_t b, bool add, uint32_t bar, uint32_t free) {
+        // d += a b as soon as the pieces of a are there (32 of each warpgroup's 64 columns)
+        const auto add_up = [&](uint32_t d, uint32_t a, uint32_t b, int i, uint32_t pieces, uint32_t bar, uint32_t free) {
             const uint64_t y = tile_descriptor(b, kPanel);
 #pragma unroll
-            for (int s = 0; s < kRows / 16; ++s)
-                product_from_tmem(one, d, a + s / 4 * 64 + s % 4 * 8, y + s * 128, sums, add || s > 0);
+            for (int piece = 0; piece < 2; ++piece) {
+                ok = ok && barrier_wait(pieces + 8 * piece, i & 1);
+                tmem_fence_after();
+                if (ok)
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        const int s = u / 2 * 4 + piece * 2 + u % 2;
+                        product_from_tmem(one, d, a + s / 4 * 64 + s % 4 * 8, y + s * 128, sums, i > 0 || piece > 0 || u > 0);
+                    }
+            }
             products_arrive(one, bar);
             products_arrive(one, free);
         };
@@ -804,19 +960,15 @@ __global__ void __launch_bounds__(kTileThreads, 1) key_gradient_tiles(const __gr
             const int st = i % kStages, next = (i + 1) % kStages;
             const uint32_t next_full = (i + 1) / kStages & 1;
             const bool more = i + 1 < tiles;
-            ok = barrier_wait(p_full, i & 1);
+            add_up(dv_at, tmem, gs + st * kTile, i, p_full, dv_done, g_empty + 8 * st);
             if (!ok) break;
-            tmem_fence_after();
-            add_up(dv_at, tmem, gs + st * kTile, i > 0, dv_done, g_empty + 8 * st);
             if (more) {
                 ok = barrier_wait(q_full + 8 * next, next_full) && barrier_wait(dv_done, i & 1);
                 if (!ok) break;
                 issue(tmem, ks, qs + next * kTile, s_full);
             }
-            ok = barrier_wait(ds_full, i & 1);
+            add_up(dk_at, dp_at, qs + st * kTile, i, ds_full, dk_done, q_empty + 8 * st);
             if (!ok) break;
-            tmem_fence_after();
-            add_up(dk_at, dp_at, qs + st * kTile, i > 0, dk_done, q_empty + 8 * st);
             if (more) {
                 ok = barrier_wait(g_full + 8 * next, next_full) && barrier_wait(dk_done, i & 1);
                 if (!ok) break;
@@ -846,26 +998,21 @@ __global__ void __launch_bounds__(kTileThreads, 1) key_gradient_tiles(const __gr
             tmem_wait_load32<0>(s);
             tmem_wait_load32<32>(s);
             if (!whole) hide(s, range, 0xff800000u);
-#pragma unroll
-            for (int j = 0; j < 64; j += 4) {
-                float o[4];
-                asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(o[0]), "=f"(o[1]), "=f"(o[2]), "=f"(o[3]) : "r"(off_at + j * 4));
-#pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    float x = fmaf(__uint_as_float(s[j + u]), s2, o[u]);
-                    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(x));
-                    s[j + u] = __float_as_uint(x);
-                }
-            }
-            {
-                uint32_t packed[32];
-#pragma unroll
-                for (int j = 0; j < 64; j += 2) packed[j / 2] = pack2<T>(__uint_as_float(s[j]), __uint_as_float(s[j + 1]));
-                tmem_store32<0>(s_at, packed);
-                tmem_wait_store();
-                tmem_fence_before();
-                barrier_arrive(p_full);
-            }
+            const auto weight_off = [&](int j) { return load_pair(off_at + j * 4); };
+            uint32_t packed[32];
+#define RODE_WEIGHTS(o)                                                                                                 \
+    if (whole)                                                                                                          \
+        weights_in_place<o, kByFmaInPairs>(s, s2, weight_off);                                                          \
+    else                                                                                                                \
+        weights_in_place<o, 0>(s, s2, weight_off);                                                                      \
+    _Pragma("unroll") for (int j = o; j < o + 32; j += 2) packed[j / 2] = pack2<T>(__uint_as_float(s[j]), __uint_as_float(s[j + 1])); \
+    tmem_store16<o / 2>(s_at + o / 2, packed);                                                                          \
+    tmem_wait_store();                                                                                                  \
+    tmem_fence_before();                                                                                                \
+    barrier_arrive(p_full + o / 4)
+            RODE_WEIGHTS(0);
+            RODE_WEIGHTS(32);
+#undef RODE_WEIGHTS
             ok = barrier_wait(dp_full, i & 1);
             if (!ok) break;
             tmem_fence_after();
@@ -874,20 +1021,17 @@ __global__ void __launch_bounds__(kTileThreads, 1) key_gradient_tiles(const __gr
             tmem_wait_load32<0>(d);
             tmem_wait_load32<32>(d);
             if (!whole) hide(d, range, 0u);
-#pragma unroll
-            for (int j = 0; j < 64; j += 4) {
-                float o[4];
-                asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(o[0]), "=f"(o[1]), "=f"(o[2]), "=f"(o[3]) : "r"(delta_at + j * 4));
-                float x[4];
-#pragma unroll
-                for (int u = 0; u < 4; ++u) x[u] = __uint_as_float(s[j + u]) * (__uint_as_float(d[j + u]) - o[u]);
-                s[j / 2] = pack2<T>(x[0], x[1]);
-                s[j / 2 + 1] = pack2<T>(x[2], x[3]);
-            }
-            tmem_store32<0>(d_at, s);
+            const auto minus = [&](int j) { return load_pair(delta_at + j * 4); };
+            gradients_in_place<T, 0>(s, d, minus);
+            tmem_store16<0>(d_at, s);
             tmem_wait_store();
             tmem_fence_before();
             barrier_arrive(ds_full);
+            gradients_in_place<T, 32>(s, d, minus);
+            tmem_store16<16>(d_at + 16, s);
+            tmem_wait_store();
+            tmem_fence_before();
+            barrier_arrive(ds_full + 8);
         }
         if (ok && tiles > 0) {
             ok = barrier_wait(dk_done, (tiles - 1) & 1) && barrier_wait(dv_done, (tiles - 1) & 1);

@@ -124,6 +124,20 @@ __device__ __forceinline__ void tmem_store32(uint32_t address, const uint32_t (&
         : "memory");
 }
 
+// The same with 16 columns.
+#define RODE_W16(r, o)                                                                                                            \
+    "r"(r[o + 0]), "r"(r[o + 1]), "r"(r[o + 2]), "r"(r[o + 3]), "r"(r[o + 4]), "r"(r[o + 5]), "r"(r[o + 6]), "r"(r[o + 7]),       \
+        "r"(r[o + 8]), "r"(r[o + 9]), "r"(r[o + 10]), "r"(r[o + 11]), "r"(r[o + 12]), "r"(r[o + 13]), "r"(r[o + 14]), "r"(r[o + 15])
+template <int o, int n>
+__device__ __forceinline__ void tmem_store16(uint32_t address, const uint32_t (&r)[n]) {
+    static_assert(o + 16 <= n, "16 registers");
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::RODE_W16(
+            r, o),
+        "r"(address)
+        : "memory");
+}
+
 // --- matrix products ------------------------------------------------------------------------------------------------------------
 
 // Descriptor of an operand tile in shared memory: address, distance of the panels (MN-major only) and of the 8-row groups in units of
