@@ -83,6 +83,8 @@ int parts_of(long long ctas, long long keys) {
     return static_cast<int>(n < 1 ? 1 : n > 128 ? 128 : n);
 }
 
+size_t delta_bytes(int q_rows, int heads) { return (static_cast<size_t>(q_rows) * heads * sizeof(float) + 255) / 256 * 256; }
+
 struct Parts {
     int prefix, own;
     size_t bytes;
@@ -155,10 +157,16 @@ int rode_window_attention(int dtype, int n_seq, const int *q_offsets, const int 
     return tiles_take_prompt(dtype, p) ? tiles_prompt(dtype, p, stream) : simple_prompt(dtype, p, stream);
 }
 
-int rode_window_attention_backward_workspace_bytes(int q_rows, int heads, size_t *bytes) {
-    if (q_rows < 0 || q_rows > kMaxRows || heads <= 0 || heads > kMaxHeads || bytes == nullptr)
-        return fail(RODE_ERR_INVALID_ARGUMENT, "rode_window_attention_backward_workspace_bytes: bad argument");
-    *bytes = static_cast<size_t>(q_rows) * heads * sizeof(float);
+int rode_window_attention_backward_workspace_bytes(int n_seq, int q_rows, int heads, int kv_heads, int dim, int window, int sinks,
+                                                   size_t *bytes) {
+    const char *what = "rode_window_attention_backward_workspace_bytes";
+    if (bytes == nullptr) return fail(RODE_ERR_INVALID_ARGUMENT, "%s: null pointer bytes", what);
+    RODE_TRY(check_shape(what, RODE_F32, heads, kv_heads, dim, 1.f));
+    RODE_TRY(check_window(what, window, sinks));
+    if (q_rows < 0 || q_rows > kMaxRows || n_seq < 0 || n_seq > kMaxRows)
+        return fail(RODE_ERR_INVALID_ARGUMENT, "%s: q_rows = %d and n_seq = %d must be 0 to 2^30", what, q_rows, n_seq);
+    const FarPlan far = plan_far(n_seq, true, q_rows, kv_heads, dim, window, sinks);
+    *bytes = delta_bytes(q_rows, heads) + far.near_bytes + far.far_bytes;
     return RODE_OK;
 }
 
@@ -182,7 +190,7 @@ int rode_window_attention_backward(int dtype, int n_seq, const int *q_offsets, c
     RODE_TRY(check_result(what, "dv", dv, keys && k_rows > 0));
     if (q_rows > 0 && lse == nullptr) return fail(RODE_ERR_INVALID_ARGUMENT, "%s: null pointer lse", what);
     size_t need = 0;
-    RODE_TRY(rode_window_attention_backward_workspace_bytes(q_rows, heads, &need));
+    RODE_TRY(rode_window_attention_backward_workspace_bytes(n_seq, q_rows, heads, kv_heads, dim, window, sinks, &need));
     RODE_TRY(check_workspace(what, workspace, workspace_bytes, need));
     if (q_rows == 0 && (k_rows == 0 || !keys)) return RODE_OK;
     Prompt p = {};
@@ -203,7 +211,15 @@ int rode_window_attention_backward(int dtype, int n_seq, const int *q_offsets, c
     p.dv = dv;
     p.delta = static_cast<float *>(workspace);
     p.clear = clear != 0;
-    return tiles_take_backward(dtype, p) ? tiles_backward(dtype, p, stream) : simple_prompt_backward(dtype, p, stream);
+    if (!tiles_take_backward(dtype, p)) return simple_prompt_backward(dtype, p, stream);
+    const FarPlan far = plan_far(n_seq, q_offsets != nullptr, q_rows, kv_heads, dim, window, sinks);
+    if (keys) {
+        p.far_chunk = far.chunk;
+        p.far_slots = far.slots;
+        p.near_part = p.delta + delta_bytes(q_rows, heads) / sizeof(float);
+        p.far_part = p.near_part + far.near_bytes / sizeof(float);
+    }
+    return tiles_backward(dtype, p, stream);
 }
 
 static int check_cached_sizes(const char *what, int batch, int prefix, int capacity) {

@@ -42,6 +42,9 @@ struct Prompt {
     float *lse;
     void *dq, *dk, *dv;
     float *delta;
+    // Chunks of the queries that see sinks only (key_gradient_tiles); far_slots == 0: none
+    int far_chunk, far_slots;
+    float *near_part, *far_part;
     bool clear;  // rows of no sequence become zero (else they are left as they were)
 };
 
@@ -67,6 +70,11 @@ bool tiles_take_prompt(int dtype, const Prompt &p);
 bool tiles_take_shared(int dtype, const Cached &c);
 int tiles_prompt(int dtype, const Prompt &p, cudaStream_t stream);
 bool tiles_take_backward(int dtype, const Prompt &p);
+struct FarPlan {
+    int chunk, slots;
+    size_t near_bytes, far_bytes;
+};
+FarPlan plan_far(int n_seq, bool packed, int q_rows, int kv_heads, int dim, int window, int sinks);
 int tiles_backward(int dtype, const Prompt &p, cudaStream_t stream);
 int tiles_shared(int dtype, const Cached &c, int first_split, int splits, cudaStream_t stream);
 bool step_takes(int dtype, const Cached &c);

@@ -12,6 +12,7 @@
 // O stays in tensor memory.  The running maximum is taken over only when it grows by more than 8 (in base 2): weights may then be as large
 // as 2^8, which costs no precision (the sum has the same factor), and the multiplication of O by 2^(old - new) is rare.
 // P is rounded to the operands' type (the products take 16-bit operands); the sum is that of the unrounded weights.
+#include <algorithm>
 #include <type_traits>
 
 #include "rode_attention.cuh"
@@ -547,24 +548,33 @@ constexpr int backward_stages() {
 }
 template <int kDim>
 constexpr int backward_bytes() {
-    return 1024 + kDim / 64 * kPanel * (2 + 2 * backward_stages<kDim>()) + backward_stages<kDim>() * 2 * kRows * 4 + 512;
+    return 1024 + kDim / 64 * kPanel * (2 + 2 * backward_stages<kDim>()) + backward_stages<kDim>() * 2 * kRows * 4 + 512 + kRows * 4;
 }
 
 struct GradientMaps {
     CUtensorMap q, dout, k, v;
 };
 
-// 16-byte pieces of a row: sum of products.
+// delta = do . o of the rows of a tile (kRows of them, row r = query r / group, head r % group) by eight warps: sixteen lanes per row, so that a
+// warp reads two rows at once.
 template <typename T>
-__device__ __forceinline__ float dot_row(const T *a, const T *b, int dim) {
-    float sum = 0.f;
-    for (int d = 0; d < dim; d += 8) {
-        const uint4 x = __ldg(reinterpret_cast<const uint4 *>(a + d)), y = __ldg(reinterpret_cast<const uint4 *>(b + d));
-        const T *s = reinterpret_cast<const T *>(&x), *t = reinterpret_cast<const T *>(&y);
+__device__ __forceinline__ void row_deltas(const Prompt &p, long long row0, int head0, int group, int n, uint32_t deltas) {
+    const int dim = p.win.dim, piece = threadIdx.x % 16, d = piece * 8;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sum = fmaf(to_float(s[i]), to_float(t[i]), sum);
+    for (int r = threadIdx.x / 16; r < kRows; r += 16) {
+        const int query = r / group, head = head0 + r % group;
+        float sum = 0.f;
+        if (query < n && d < dim) {
+            const uint4 x = __ldg(reinterpret_cast<const uint4 *>(row_of<T>(p.dout, 0, row0 + query, head) + d));
+            const uint4 y = __ldg(reinterpret_cast<const uint4 *>(static_cast<const T *>(p.out) + ((row0 + query) * p.win.heads + head) * dim + d));
+            const T *s = reinterpret_cast<const T *>(&x), *t = reinterpret_cast<const T *>(&y);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum = fmaf(to_float(s[i]), to_float(t[i]), sum);
+        }
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (piece == 0) asm volatile("st.shared.f32 [%0], %1;" ::"r"(deltas + 4 * r), "f"(sum) : "memory");
     }
-    return sum;
 }
 
 // Columns x .. x + 31 of an accumulator row, times factor, to 32 elements of a row of `dim`.
@@ -634,7 +644,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) query_gradient_tiles(const __
     uint32_t tmem;
     asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem) : "r"(tmem_at));
     tmem = uniform(tmem);
-    const uint32_t dp_at = tmem + 256, dq_at = tmem + 384;
+    const uint32_t dp_at = tmem + 256, dq_at = tmem + 384, deltas = bars + 512;
     bool ok = true;
 
     if (warp >= 8) give_registers();
@@ -737,13 +747,15 @@ __global__ void __launch_bounds__(kTileThreads, 1) query_gradient_tiles(const __
         const int query = r / group, head = kv * group + r % group, pos = pos0 + query;
         const bool mine = query < n;
         const long long row = row0 + query, at = static_cast<long long>(head) * p.seqs.q_rows + row;
-        float delta = 0.f, off = 0.f;
+        float delta, off = 0.f;
         if (mine) {
-            delta = dot_row(row_of<T>(p.dout, 0, row, head), static_cast<const T *>(p.out) + (row * w.heads + head) * w.dim, w.dim);
-            const float lse = p.lse[at];
-            if (half == 0) p.delta[at] = delta;
+            const float lse = __ldg(p.lse + at);
             off = lse == -INFINITY ? 0.f : -lse * kLog2e;
         }
+        row_deltas<T>(p, row0, kv * group, group, n, deltas);
+        asm volatile("bar.sync 1, 256;" ::: "memory");  // these two warpgroups
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(delta) : "r"(deltas + 4 * r) : "memory");
+        if (mine && half == 0) p.delta[at] = delta;
         const float s2 = w.scale * kLog2e;
         for (int i = 0; i < blocks.n; ++i) {
             const int k0 = blocks.at(i) * kRows, buf = i & 1, c0 = k0 + half * 64;
@@ -803,29 +815,66 @@ __global__ void __launch_bounds__(kTileThreads, 1) query_gradient_tiles(const __
     if (warp == 8) tmem_free(tmem, 512);
 }
 
-// dK and dV of one tile of 128 keys: all rows of queries that see any of them, 128 at a time.  Tensor memory: S^T (P^T over it), dP^T
-// (dS^T over it), dV, dK.  Per tile of queries the products run in the order dV, next S^T, dK, next dP^T: while the threads make dS of this tile
-// the tensor cores work on dV and the next S^T, while they make the next P on dK and the next dP^T.
+// Queries up to the end of the window of the last of `have` keys from key `first` on.
+__device__ __forceinline__ int near_queries(int first, int have, int keys, int queries, int window) {
+    const int last = window >= keys - (first + have - 1) ? keys : first + have - 1 + window;
+    return min(max(last - (keys - queries), max(first - (keys - queries), 0)), queries);
+}
+// Whether the far queries of a sequence's first tile are worked on in chunks.
+__device__ __forceinline__ bool far_chunks(const Prompt &p, int near, int queries) {
+    return p.far_chunk > 0 && queries - near > p.far_chunk / 2;
+}
+
+// dK and dV of one tile of 128 keys: all rows of queries that see any of them, 128 at a time.  Tensor memory: S^T, dP^T (P^T and dS^T over it; twice
+// where the head dimension leaves room), dV, dK.  S^T of the next tile of queries is made as soon as the threads have this one's in registers, so
+// that they never wait for it; what they wait for is dP^T, which must wait for dV and dK of the tile before.
+//
+// The first tile of a sequence has the sinks, which all later queries see: as one CTA it took 4 times as long as the others on 8192 positions with a
+// window of 2048, and the grid waited for it (1436 us instead of RODE_KEYS).  So queries behind the window of the first tile's keys ("far" ones) are cut into chunks of
+// p.far_chunk for CTAs of their own, which come first in the grid; these and the first tile leave their sums in 32 bits, and add_far_gradients adds
+// them up in order.
 template <typename T, int kDim>
 __global__ void __launch_bounds__(kTileThreads, 1) key_gradient_tiles(const __grid_constant__ GradientMaps maps, const Prompt p) {
     constexpr int kPanels = kDim / 64, kStages = backward_stages<kDim>(), kTile = kPanels * kPanel;
     extern __shared__ char shared_raw[];
     const Window &w = p.win;
     const int group = w.heads / w.kv_heads, per_tile = kRows / group, kv = blockIdx.y;
-    const Tile t = find_tile(p.seqs.k_offsets, p.seqs.n_seq, p.seqs.k_rows, blockIdx.x, kRows);
-    if (t.first < 0 || t.first >= t.rows || (t.seq < 0 && !p.clear)) return;
-    const int2 queries = t.seq < 0 ? make_int2(0, 0) : sequence_rows(p.seqs.q_offsets, p.seqs.q_rows, t.seq);
+    const int far = static_cast<int>(blockIdx.x) < p.far_slots ? blockIdx.x : -1;
+    Tile t;
+    int2 queries;
+    int chunk = 0;  // first query of a far chunk
+    if (far >= 0) {
+        const Tile u = find_tile(p.seqs.q_offsets, p.seqs.n_seq, p.seqs.q_rows, far, p.far_chunk);
+        if (u.first < 0 || u.first >= u.rows || u.seq < 0) return;
+        const int2 keys = sequence_rows(p.seqs.k_offsets, p.seqs.k_rows, u.seq);
+        t = {u.seq, keys.x, keys.y, 0};
+        queries = make_int2(u.row0, u.rows);
+        chunk = u.first;
+    } else {
+        t = find_tile(p.seqs.k_offsets, p.seqs.n_seq, p.seqs.k_rows, blockIdx.x - p.far_slots, kRows);
+        if (t.first < 0 || t.first >= t.rows || (t.seq < 0 && !p.clear)) return;
+        queries = t.seq < 0 ? make_int2(0, 0) : sequence_rows(p.seqs.q_offsets, p.seqs.q_rows, t.seq);
+    }
     const long long row0 = static_cast<long long>(t.row0) + t.first;
     const int have = min(kRows, t.rows - t.first), shift = t.rows - queries.y;
+    const int near = near_queries(t.first, have, t.rows, queries.y, w.window);
+    const bool split = far_chunks(p, near, queries.y) && t.first == 0;  // the far queries are others' work
     // queries from the tile's first key to the end of its last key's window (sinks: to the end)
-    const int last = t.first < w.sinks || w.window >= t.rows - (t.first + have - 1) ? t.rows : t.first + have - 1 + w.window;
-    const int i0 = max(t.first - shift, 0), i1 = max(min(last - shift, queries.y), i0), tiles = (i1 - i0 + per_tile - 1) / per_tile;
+    int i0 = max(t.first - shift, 0), i1 = t.first < w.sinks && !split ? queries.y : near;
+    if (far >= 0) {
+        i0 = max(near, chunk);
+        i1 = min(queries.y, chunk + p.far_chunk);
+        if (!split || i0 >= i1) return;
+    }
+    const int tiles = max(i1 - i0 + per_tile - 1, 0) / per_tile;
+    // queries of tile i that exist
+    const auto queries_of = [&](int i) { return min(per_tile, i1 - i0 - i * per_tile); };
 
     const uint32_t base = uniform((shared_address(shared_raw) + 1023) & ~1023u);
     const uint32_t ks = base, vs = ks + kTile, qs = vs + kTile, gs = qs + kStages * kTile, rows_at = gs + kStages * kTile,
                    bars = rows_at + kStages * 2 * kRows * 4;
-    const uint32_t k_full = bars, raw = bars + 8, s_full = bars + 16, dp_full = bars + 24, p_full = bars + 32, ds_full = bars + 48,
-                   dv_done = bars + 64, dk_done = bars + 72, q_full = bars + 80, q_empty = q_full + 8 * kStages, g_full = q_empty + 8 * kStages,
+    const uint32_t k_full = bars, raw = bars + 8, s_full = bars + 16, s_read = bars + 24, dp_full = bars + 32, ds_full = bars + 48,
+                   done = bars + 64, q_full = bars + 80, q_empty = q_full + 8 * kStages, g_full = q_empty + 8 * kStages,
                    g_empty = g_full + 8 * kStages, rows_full = g_empty + 8 * kStages, tmem_at = rows_full + 8 * kStages;
     const int warp = uniform(threadIdx.x / 32), lane = threadIdx.x % 32;
     if (warp == 8) {
@@ -834,13 +883,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) key_gradient_tiles(const __gr
             barrier_init(k_full, 1);
             barrier_init(raw, 1);
             barrier_init(s_full, 1);
-            barrier_init(dp_full, 1);
-            for (int piece = 0; piece < 2; ++piece) {
-                barrier_init(p_full + 8 * piece, 256);
-                barrier_init(ds_full + 8 * piece, 256);
+            barrier_init(s_read, 256);
+            for (int i = 0; i < 2; ++i) {
+                barrier_init(dp_full + 8 * i, 1);
+                barrier_init(ds_full + 8 * i, 256);
             }
-            barrier_init(dv_done, 1);
-            barrier_init(dk_done, 1);
+            barrier_init(done, 1);
             for (int i = 0; i < kStages; ++i) {
                 barrier_init(q_full + 8 * i, 1);
                 barrier_init(q_empty + 8 * i, 1);
@@ -858,7 +906,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) key_gradient_tiles(const __gr
     uint32_t tmem;
     asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem) : "r"(tmem_at));
     tmem = uniform(tmem);
-    const uint32_t dp_at = tmem + 128, dv_at = tmem + 256, dk_at = tmem + 384;
+    constexpr int kBuffers = kDim == 64 ? 2 : 1;  // of dP
+    const uint32_t dp_at = tmem + 128, dv_at = tmem + 512 - 2 * kDim, dk_at = tmem + 512 - kDim;
     bool ok = true;
 
     if (warp >= 8) give_registers();
@@ -879,7 +928,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) key_gradient_tiles(const __gr
             }
         int cleared = 0;
         for (int i = 0; i < tiles && ok; ++i) {
-            const int st = i % kStages, n = min(per_tile, queries.y - i0 - i * per_tile), y = queries.x + i0 + i * per_tile;
+            const int st = i % kStages, n = queries_of(i), y = queries.x + i0 + i * per_tile;
             const uint32_t free = (i / kStages & 1) ^ 1;
             for (int u = 0; u < 2 && ok; ++u) {  // queries, then gradients of the results
                 const uint32_t tile = (u ? gs : qs) + st * kTile, done = (u ? g_full : q_full) + 8 * st, bar = n < per_tile ? raw : done;
@@ -899,7 +948,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) key_gradient_tiles(const __gr
     } else if (warp == 10) {
         // lse and delta of the tiles' rows
         for (int i = 0; i < tiles && ok; ++i) {
-            const int st = i % kStages, n = min(per_tile, queries.y - i0 - i * per_tile);
+            const int st = i % kStages, n = queries_of(i);
             const long long first = static_cast<long long>(queries.x) + i0 + i * per_tile;
             // (free when the queries of the stage are: their last product comes behind ds_full)
             ok = barrier_wait(q_empty + 8 * st, (i / kStages & 1) ^ 1);
@@ -931,23 +980,6 @@ __global__ void __launch_bounds__(kTileThreads, 1) key_gradient_tiles(const __gr
                 }
             products_arrive(one, bar);
         };
-        // d += a b as soon as the pieces of a are there (32 of each warpgroup's 64 columns)
-        const auto add_up = [&](uint32_t d, uint32_t a, uint32_t b, int i, uint32_t pieces, uint32_t bar, uint32_t free) {
-            const uint64_t y = tile_descriptor(b, kPanel);
-#pragma unroll
-            for (int piece = 0; piece < 2; ++piece) {
-                ok = ok && barrier_wait(pieces + 8 * piece, i & 1);
-                tmem_fence_after();
-                if (ok)
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        const int s = u / 2 * 4 + piece * 2 + u % 2;
-                        product_from_tmem(one, d, a + s / 4 * 64 + s % 4 * 8, y + s * 128, sums, i > 0 || piece > 0 || u > 0);
-                    }
-            }
-            products_arrive(one, bar);
-            products_arrive(one, free);
-        };
         if (tiles > 0) {
             ok = barrier_wait(k_full, 0) && barrier_wait(q_full, 0) && barrier_wait(g_full, 0);
             tmem_fence_after();
@@ -958,21 +990,43 @@ __global__ void __launch_bounds__(kTileThreads, 1) key_gradient_tiles(const __gr
         }
         for (int i = 0; i < tiles && ok; ++i) {
             const int st = i % kStages, next = (i + 1) % kStages;
-            const uint32_t next_full = (i + 1) / kStages & 1;
+            const uint32_t next_full = (i + 1) / kStages & 1, buf = dp_at + i % kBuffers * kRows;
             const bool more = i + 1 < tiles;
-            add_up(dv_at, tmem, gs + st * kTile, i, p_full, dv_done, g_empty + 8 * st);
-            if (!ok) break;
             if (more) {
-                ok = barrier_wait(q_full + 8 * next, next_full) && barrier_wait(dv_done, i & 1);
+                ok = barrier_wait(q_full + 8 * next, next_full) && barrier_wait(s_read, i & 1);
                 if (!ok) break;
+                tmem_fence_after();
                 issue(tmem, ks, qs + next * kTile, s_full);
             }
-            add_up(dk_at, dp_at, qs + st * kTile, i, ds_full, dk_done, q_empty + 8 * st);
+            // (every phase of `done` is waited for here, so that the threads' wait for the last one cannot be a phase early)
+            ok = i == 0 || kBuffers == 1 || barrier_wait(done, (i - 1) & 1);
             if (!ok) break;
-            if (more) {
-                ok = barrier_wait(g_full + 8 * next, next_full) && barrier_wait(dk_done, i & 1);
+            if (kBuffers == 2 && more) {
+                ok = barrier_wait(g_full + 8 * next, next_full);
                 if (!ok) break;
-                issue(dp_at, vs, gs + next * kTile, dp_full);
+                issue(dp_at + (i + 1) % 2 * kRows, vs, gs + next * kTile, dp_full + (i + 1) % 2 * 8);
+            }
+            const uint64_t x = tile_descriptor(qs + st * kTile, kPanel), y = tile_descriptor(gs + st * kTile, kPanel);
+#pragma unroll
+            for (int piece = 0; piece < 2; ++piece) {  // 32 of each warpgroup's 64 columns
+                ok = ok && barrier_wait(ds_full + 8 * piece, i & 1);
+                tmem_fence_after();
+                if (ok)
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) {
+                        const int s = u / 2 % 2 * 4 + piece * 2 + u % 2;
+                        product_from_tmem(one, u < 4 ? dv_at : dk_at, buf + s / 4 * 64 + s % 4 * 8 + (u < 4 ? 32 : 0), (u < 4 ? y : x) + s * 128, sums,
+                                          i > 0 || piece > 0 || u % 4 > 0);
+                    }
+            }
+            if (!ok) break;
+            products_arrive(one, done);
+            products_arrive(one, q_empty + 8 * st);
+            products_arrive(one, g_empty + 8 * st);
+            if (kBuffers == 1) {
+                ok = barrier_wait(done, i & 1) && (!more || barrier_wait(g_full + 8 * next, next_full));
+                if (!ok) break;
+                if (more) issue(dp_at, vs, gs + next * kTile, dp_full);
             }
             __syncwarp();
         }
@@ -980,14 +1034,15 @@ __global__ void __launch_bounds__(kTileThreads, 1) key_gradient_tiles(const __gr
         take_registers();
         const int half = warp / 4, r = threadIdx.x % 128, key = t.first + r;
         const uint32_t lanes = static_cast<uint32_t>(warp % 4 * 32) << 16;
-        const uint32_t s_at = tmem + lanes + half * 64, d_at = dp_at + lanes + half * 64;
+        const uint32_t s_at = tmem + lanes + half * 64;
         const float s2 = w.scale * kLog2e;
         for (int i = 0; i < tiles; ++i) {
-            const int st = i % kStages, q0 = i0 + i * per_tile, n = min(per_tile, queries.y - q0), pos0 = q0 + shift;
+            const int st = i % kStages, q0 = i0 + i * per_tile, n = queries_of(i), pos0 = q0 + shift;
             // columns are (query, head): the queries that see this thread's key are a range of them
             const bool whole = n * group == kRows && pos0 >= t.first + have - 1 && (pos0 + n - 1 - t.first < w.window || t.first + have <= w.sinks);
             const int a = min(max(key - pos0, 0), n), b = key < w.sinks ? n : max(min(n, key - pos0 + w.window), 0);
             const Range range = {a * group - half * 64, b * group - half * 64, 0};
+            const uint32_t d_at = dp_at + lanes + i % kBuffers * kRows + half * 64;
             const uint32_t off_at = rows_at + (st * 2 * kRows + half * 64) * 4, delta_at = off_at + kRows * 4;
             ok = barrier_wait(rows_full + 8 * st, i / kStages & 1) && barrier_wait(s_full, i & 1);
             if (!ok) break;
@@ -997,23 +1052,21 @@ __global__ void __launch_bounds__(kTileThreads, 1) key_gradient_tiles(const __gr
             tmem_load32<32>(s_at + 32, s);
             tmem_wait_load32<0>(s);
             tmem_wait_load32<32>(s);
+            tmem_fence_before();
+            barrier_arrive(s_read);
             if (!whole) hide(s, range, 0xff800000u);
             const auto weight_off = [&](int j) { return load_pair(off_at + j * 4); };
             uint32_t packed[32];
-#define RODE_WEIGHTS(o)                                                                                                 \
-    if (whole)                                                                                                          \
-        weights_in_place<o, kByFmaInPairs>(s, s2, weight_off);                                                          \
-    else                                                                                                                \
-        weights_in_place<o, 0>(s, s2, weight_off);                                                                      \
-    _Pragma("unroll") for (int j = o; j < o + 32; j += 2) packed[j / 2] = pack2<T>(__uint_as_float(s[j]), __uint_as_float(s[j + 1])); \
-    tmem_store16<o / 2>(s_at + o / 2, packed);                                                                          \
-    tmem_wait_store();                                                                                                  \
-    tmem_fence_before();                                                                                                \
-    barrier_arrive(p_full + o / 4)
-            RODE_WEIGHTS(0);
-            RODE_WEIGHTS(32);
-#undef RODE_WEIGHTS
-            ok = barrier_wait(dp_full, i & 1);
+            if (whole) {
+                weights_in_place<0, kByFmaInPairs>(s, s2, weight_off);
+                weights_in_place<32, kByFmaInPairs>(s, s2, weight_off);
+            } else {
+                weights_in_place<0, 0>(s, s2, weight_off);
+                weights_in_place<32, 0>(s, s2, weight_off);
+            }
+#pragma unroll
+            for (int j = 0; j < 64; j += 2) packed[j / 2] = pack2<T>(__uint_as_float(s[j]), __uint_as_float(s[j + 1]));
+            ok = barrier_wait(dp_full + i % kBuffers * 8, i / kBuffers & 1);
             if (!ok) break;
             tmem_fence_after();
             tmem_load32<0>(d_at, d);
@@ -1021,7 +1074,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) key_gradient_tiles(const __gr
             tmem_wait_load32<0>(d);
             tmem_wait_load32<32>(d);
             if (!whole) hide(d, range, 0u);
+            // over this thread's part of dP: 32 columns of dS, 32 of P
             const auto minus = [&](int j) { return load_pair(delta_at + j * 4); };
+            tmem_store32<0>(d_at + 32, packed);
             gradients_in_place<T, 0>(s, d, minus);
             tmem_store16<0>(d_at, s);
             tmem_wait_store();
@@ -1034,20 +1089,61 @@ __global__ void __launch_bounds__(kTileThreads, 1) key_gradient_tiles(const __gr
             barrier_arrive(ds_full + 8);
         }
         if (ok && tiles > 0) {
-            ok = barrier_wait(dk_done, (tiles - 1) & 1) && barrier_wait(dv_done, (tiles - 1) & 1);
+            ok = barrier_wait(done, (tiles - 1) & 1);
             tmem_fence_after();
         }
-        const long long at = ((row0 + r) * w.kv_heads + kv) * w.dim;
-        T *out = static_cast<T *>(half == 0 ? p.dv : p.dk) + at;
+        const uint32_t sum_at = (half == 0 ? dv_at : dk_at) + lanes;
+        const float factor = half == 0 ? 1.f : w.scale;
+        if (split) {
+            float *part = far >= 0 ? p.far_part + (static_cast<long long>(far) * w.kv_heads + kv) * 2 * kRows * w.dim
+                                   : p.near_part + (static_cast<long long>(t.seq) * w.kv_heads + kv) * 2 * kRows * w.dim;
+            part += (half * kRows + r) * w.dim;
 #pragma unroll
-        for (int x = 0; x < kDim; x += 32)
-            store_columns(out, (half == 0 ? dv_at : dk_at) + lanes, x, w.dim, half == 0 ? 1.f : w.scale, r < have, tiles > 0);
+            for (int x = 0; x < kDim; x += 32) {
+                uint32_t o[32];
+                tmem_load32<0>(sum_at + x, o);
+                tmem_wait_load32<0>(o);
+#pragma unroll
+                for (int j = 0; j < 32; j += 4)
+                    if (r < have && x + j < w.dim)
+                        *reinterpret_cast<float4 *>(part + x + j) =
+                            tiles > 0 ? make_float4(__uint_as_float(o[j]) * factor, __uint_as_float(o[j + 1]) * factor,
+                                                    __uint_as_float(o[j + 2]) * factor, __uint_as_float(o[j + 3]) * factor)
+                                      : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+        } else {
+            T *out = static_cast<T *>(half == 0 ? p.dv : p.dk) + ((row0 + r) * w.kv_heads + kv) * w.dim;
+#pragma unroll
+            for (int x = 0; x < kDim; x += 32) store_columns(out, sum_at, x, w.dim, factor, r < have, tiles > 0);
+        }
     }
     if (!ok) waits_failed = 1;
     tmem_fence_before();
     __syncthreads();
     tmem_fence_after();
     if (warp == 8) tmem_free(tmem, 512);
+}
+
+// dK and dV of the first tiles whose far queries were worked on in chunks: the tile's own part, then the chunks' in order.
+template <typename T>
+__global__ void __launch_bounds__(256) add_far_gradients(const Prompt p) {
+    const Window &w = p.win;
+    const int seq = blockIdx.x, kv = blockIdx.y, chunk = p.far_chunk;
+    const int2 keys = sequence_rows(p.seqs.k_offsets, p.seqs.k_rows, seq), queries = sequence_rows(p.seqs.q_offsets, p.seqs.q_rows, seq);
+    const int have = min(kRows, keys.y), near = near_queries(0, have, keys.y, queries.y, w.window);
+    if (have == 0 || !far_chunks(p, near, queries.y)) return;
+    const int slot = p.seqs.q_offsets == nullptr ? 0 : queries.x / chunk + seq + 1;
+    const int first = near / chunk, n = (queries.y + chunk - 1) / chunk;
+    const long long size = 2ll * kRows * w.dim, step = size * w.kv_heads;
+    for (int i = (blockIdx.z * 256 + threadIdx.x) * 4; i < 2 * have * w.dim; i += gridDim.z * 256 * 4) {
+        const int half = i / (have * w.dim), at = i % (have * w.dim);  // row * dim + column
+        const long long from = static_cast<long long>(half) * kRows * w.dim + at;
+        float4 sum = *reinterpret_cast<const float4 *>(p.near_part + (static_cast<long long>(seq) * w.kv_heads + kv) * size + from);
+        for (int f = first; f < n; ++f)
+            vadd(sum, *reinterpret_cast<const float4 *>(p.far_part + (slot + f) * step + kv * size + from));
+        store4(static_cast<T *>(half == 0 ? p.dv : p.dk) + (static_cast<long long>(keys.x) + at / w.dim) * w.kv_heads * w.dim + kv * w.dim + at % w.dim,
+               sum);
+    }
 }
 
 // --- host -----------------------------------------------------------------------------------------------------------------------
@@ -1141,6 +1237,21 @@ int tiles_prompt(int dtype, const Prompt &p, cudaStream_t stream) {
     });
 }
 
+// Chunks of about a tile's own work, and only where the sequences are long on average: the first tile is then at least three times the work
+// of the others.
+FarPlan plan_far(int n_seq, bool packed, int q_rows, int kv_heads, int dim, int window, int sinks) {
+    FarPlan f = {0, 0, 0, 0};
+    if (sinks <= 0 || sinks > kRows || n_seq <= 0 || window > (1 << 29)) return f;
+    const int chunk = std::max(1024, window + kRows);
+    if (q_rows / n_seq <= 2ll * chunk) return f;
+    f.chunk = chunk;
+    f.slots = packed ? q_rows / chunk + n_seq + 2 : (q_rows + chunk - 1) / chunk;
+    const size_t tile = 2 * sizeof(float) * kRows * dim * kv_heads;
+    f.near_bytes = tile * n_seq;
+    f.far_bytes = tile * f.slots;
+    return f;
+}
+
 int tiles_backward(int dtype, const Prompt &p, cudaStream_t stream) {
     const Window &w = p.win;
     const int group = w.heads / w.kv_heads, per_tile = kRows / group;
@@ -1161,8 +1272,12 @@ int tiles_backward(int dtype, const Prompt &p, cudaStream_t stream) {
         RODE_CHECK_LAUNCH("query_gradient_tiles");
         if (p.dk == nullptr) return static_cast<int>(RODE_OK);
         const int k_slots = tile_slots(p.seqs.k_offsets, p.seqs.n_seq, p.seqs.k_rows, kRows);
-        keys<<<dim3(k_slots, w.kv_heads), kTileThreads, backward_bytes<kDim>(), stream>>>(maps, p);
+        keys<<<dim3(p.far_slots + k_slots, w.kv_heads), kTileThreads, backward_bytes<kDim>(), stream>>>(maps, p);
         RODE_CHECK_LAUNCH("key_gradient_tiles");
+        if (p.far_slots > 0) {
+            add_far_gradients<T><<<dim3(p.seqs.n_seq, w.kv_heads, 8), 256, 0, stream>>>(p);
+            RODE_CHECK_LAUNCH("add_far_gradients");
+        }
         return static_cast<int>(RODE_OK);
     });
 }

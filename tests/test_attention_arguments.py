@@ -40,9 +40,11 @@ def test_nothing_to_do_needs_no_device(built_library):
 
 def test_workspaces(built_library):
     lib, need = capi.load(), ctypes.c_size_t(0)
-    assert lib.rode_window_attention_backward_workspace_bytes(10, 4, ctypes.byref(need)) == 0 and need.value >= 4 * 10 * 4
-    assert lib.rode_window_attention_backward_workspace_bytes(-1, 4, ctypes.byref(need)) == BAD
-    assert lib.rode_window_attention_backward_workspace_bytes(1, 4, None) == BAD
+    backward = lambda n_seq, q_rows, out=ctypes.byref(need): lib.rode_window_attention_backward_workspace_bytes(
+        n_seq, q_rows, 4, 2, 64, 4, 1, out)
+    assert backward(1, 10) == 0 and need.value >= 4 * 10 * 4
+    assert backward(1, -1) == BAD and backward(-1, 10) == BAD and backward(1, 10, None) == BAD
+    assert backward(0, 10**6) == 0
     back = lambda ws, n, dk=256, dv=256: lib.rode_window_attention_backward(
         0, 1, None, None, 8, 8, 4, 2, 64, 4, 0, 1.0, 1, _heads(), _heads(), _heads(), 256, 256, _heads(), 256, dk, dv, ws, n, None)
     assert back(None, 0) == WS and back(256, 8) == WS and back(264, 1 << 20) == WS

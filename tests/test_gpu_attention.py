@@ -88,6 +88,24 @@ def test_lengths_and_masks(case, dim, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("case", [([5000], [5000], 100, 5), ([30, 6500], None, 700, 1), ([4200, 3], [4500, 3], 300, 128),
+                                  ([2100, 2700, 0], [2100, 2600, 5], 1, 2), ([4000], [4000], 50, 129)])
+@pytest.mark.parametrize("dim", [64, 120])
+def test_sinks_seen_from_far(case, dim, dtype):
+    """Long sequences, whose first keys get gradients from queries far behind their window."""
+    q_lens, k_lens, window, sinks = case
+    k_lens = k_lens or q_lens
+    q, k, v, dout = _make(q_lens, k_lens, 2, 1, dim, dtype, seed=12)
+    k[:3] *= 2
+    want = R.packed(q, k, v, q_lens, k_lens, window, sinks, dim ** -0.5, dout)
+    kw = {} if len(q_lens) == 1 else {"q_offsets": _offsets(q_lens), "k_offsets": _offsets(k_lens) if k_lens != q_lens else None}
+    got = _run(q, k, v, dout, window, sinks, **kw)
+    _check(got, want)
+    again = _run(q, k, v, dout, window, sinks, **kw)
+    assert all(torch.equal(got[n], again[n]) for n in got)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("heads,kv_heads,dim", [(1, 1, 4), (3, 1, 20), (6, 3, 40), (8, 1, 80), (5, 5, 96), (4, 2, 100), (2, 2, 16),
                                                 (16, 2, 120), (2, 1, 132), (4, 2, 256)])
 def test_head_layouts(heads, kv_heads, dim, dtype):
