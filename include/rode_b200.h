@@ -347,8 +347,8 @@ int rode_window_attention_backward(int dtype, int n_seq, const int *q_offsets, c
  * used) stands at position lengths[b] - 1 of its cache (k_cache, v_cache [batch, capacity, kv_heads, dim]), whose rows from
  * lengths[b] on are not read.  lengths int32[batch] on the device, taken as at least 0 and at most capacity.
  * out [batch, heads, dim] contiguous.  workspace as above, 0 bytes for some sizes; it depends on the current device. */
-int rode_window_attention_step_workspace_bytes(int batch, int capacity, int heads, int kv_heads, int dim, int window,
-                                               int sinks, size_t *bytes);
+int rode_window_attention_step_workspace_bytes(int dtype, int batch, int capacity, int heads, int kv_heads, int dim,
+                                               int window, int sinks, size_t *bytes);
 int rode_window_attention_step(int dtype, int batch, int capacity, int heads, int kv_heads, int dim, int window,
                                int sinks, float scale, const rode_heads_t *q, const rode_heads_t *k_cache,
                                const rode_heads_t *v_cache, const int *lengths, void *out, void *workspace,
@@ -357,8 +357,8 @@ int rode_window_attention_step(int dtype, int batch, int capacity, int heads, in
 /* One new token per request behind a prefix that all requests share: request b's query sees all rows of the prefix (prefix_k,
  * prefix_v [prefix, kv_heads, dim], .batch is not used) and the first lengths[b] rows of its own cache.  The queries of all
  * requests go through the prefix together, so that it is read once. */
-int rode_shared_prefix_attention_workspace_bytes(int batch, int prefix, int capacity, int heads, int kv_heads, int dim,
-                                                 size_t *bytes);
+int rode_shared_prefix_attention_workspace_bytes(int dtype, int batch, int prefix, int capacity, int heads, int kv_heads,
+                                                 int dim, size_t *bytes);
 int rode_shared_prefix_attention(int dtype, int batch, int prefix, int capacity, int heads, int kv_heads, int dim,
                                  float scale, const rode_heads_t *q, const rode_heads_t *prefix_k,
                                  const rode_heads_t *prefix_v, const rode_heads_t *k_cache, const rode_heads_t *v_cache,

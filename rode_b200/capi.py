@@ -113,9 +113,9 @@ def load() -> ctypes.CDLL:
     lib.rode_window_attention_backward_workspace_bytes.argtypes = [ci] * 7 + [ctypes.POINTER(sz)]
     lib.rode_window_attention_backward.argtypes = ([ci, ci, vp, vp] + [ci] * 7 + [cf, ci] + [heads] * 3 + [vp, vp, heads]
                                                    + [vp] * 4 + [sz, vp])
-    lib.rode_window_attention_step_workspace_bytes.argtypes = [ci] * 7 + [ctypes.POINTER(sz)]
+    lib.rode_window_attention_step_workspace_bytes.argtypes = [ci] * 8 + [ctypes.POINTER(sz)]
     lib.rode_window_attention_step.argtypes = [ci] * 8 + [cf] + [heads] * 3 + [vp] * 3 + [sz, vp]
-    lib.rode_shared_prefix_attention_workspace_bytes.argtypes = [ci] * 6 + [ctypes.POINTER(sz)]
+    lib.rode_shared_prefix_attention_workspace_bytes.argtypes = [ci] * 7 + [ctypes.POINTER(sz)]
     lib.rode_shared_prefix_attention.argtypes = [ci] * 7 + [cf] + [heads] * 5 + [vp] * 3 + [sz, vp]
     lib.rode_attention_waits_failed.argtypes = [ctypes.POINTER(ci)]
     for name in ("rode_preprocess_workspace_bytes", "rode_preprocess_capacity", "rode_preprocess",

@@ -75,51 +75,73 @@ int check_packed(const char *what, int n_seq, const int *q_offsets, const int *k
         if (const int rode_e_ = (expr)) return rode_e_; \
     } while (0)
 
-// Into how many parts the keys of a call with few rows are cut: enough for about four CTAs of the single-token kernel per SM, none
-// of fewer than 256 keys.
-int parts_of(long long ctas, long long keys) {
-    const long long want = (4ll * sm_count() + ctas - 1) / ctas, most = (keys + 255) / 256;
-    const long long n = want < most ? want : most;
-    return static_cast<int>(n < 1 ? 1 : n > 128 ? 128 : n);
-}
-
 size_t delta_bytes(int q_rows, int heads) { return (static_cast<size_t>(q_rows) * heads * sizeof(float) + 255) / 256 * 256; }
 
+// How a call on caches is cut up (Cached), and the floats of its workspace.
 struct Parts {
-    int prefix, own;
-    size_t bytes;
+    int chunk, ctas, prefix;
+    bool whole;
+    size_t prefix_rows, own_rows, piece_rows, bytes;
 };
 
-Parts plan_parts(int batch, int prefix, long long seen, int heads, int kv_heads, int dim) {
-    Parts p = {0, 0, 0};
+// Own keys: as many CTAs as are resident at a time, two per SM, with equal shares of all blocks (step_batch 207 us with whole segments, 188 so); segments of
+// at most 256 keys stay whole and save the joining, and so do they behind a prefix where there are enough of them, for there CTAs must be free to go
+// to the SMs that the prefix leaves.
+// Prefix, 16-bit operands: CTAs of 256 rows of queries, one per SM, which the tensor cores bound, while the own keys' are bound by memory and take
+// whatever SMs are left; so the prefix gets the SMs in proportion to its time (blocks of 128 keys at 1.75 us, own keys at 5.4 TB/s with caches half
+// full).  fp32: CTAs of 64 rows, parts down to 64 keys.
+Parts plan_parts(int dtype, int batch, int prefix, long long seen, int heads, int kv_heads, int dim) {
+    Parts p = {};
+    p.whole = true;
     if (batch == 0) return p;
-    const int group = heads / kv_heads;
-    p.own = parts_of(static_cast<long long>(batch) * kv_heads * ((group + 7) / 8), seen);
+    const int group = heads / kv_heads, sms = sm_count();
+    const bool half = dtype != RODE_F32;
+    p.chunk = half ? kTensorCoreChunk : kSimpleChunk;
+    const long long segments = static_cast<long long>(batch) * kv_heads * ((group + p.chunk - 1) / p.chunk);
+    const long long least = half ? 256 : 64;  // keys
+    p.whole = seen <= least || (prefix > 0 && segments >= 2 * sms);
+    p.ctas = static_cast<int>(p.whole ? segments : std::min((prefix > 0 ? 8ll : 2ll) * sms, segments * ((seen + least - 1) / least)));
     if (prefix > 0) {
-        // one CTA per SM: 256 rows of queries each, as the tensor-core kernel takes them
-        const int per_cta = group <= 128 ? 2 * (128 / group) : 1;
-        const long long ctas = (static_cast<long long>(batch) + per_cta - 1) / per_cta * kv_heads, blocks = (prefix + 127ll) / 128;
-        p.prefix = static_cast<int>(std::max(1ll, std::min(sm_count() / ctas, (blocks + 1) / 2)));
+        const int per_cta = half ? 2 * std::max(128 / group, 1) : std::max(64 / group, 1);
+        const long long ctas = (static_cast<long long>(batch) + per_cta - 1) / per_cta * kv_heads;
+        long long share = 2 * sms;
+        if (half) {
+            const double own_us = 0.5 * 4.0 * batch * kv_heads * static_cast<double>(seen) * dim / 5.4e6;
+            const double prefix_us = ctas * ((prefix + 127) / 128) * 1.75 / sms;
+            share = static_cast<long long>(sms * prefix_us / (prefix_us + own_us));
+        }
+        p.prefix = static_cast<int>(std::min(std::max((share + ctas / 2) / ctas, 1ll), (prefix + least - 1) / least));
     }
-    const int n = p.prefix + p.own;
-    if (n > 1) p.bytes = static_cast<size_t>(n) * batch * heads * (dim + 1) * sizeof(float);
+    const size_t rows = static_cast<size_t>(batch) * heads;
+    p.prefix_rows = p.prefix * rows;
+    p.own_rows = p.prefix > 0 ? rows : 0;
+    p.piece_rows = p.whole ? 0 : 2ull * p.ctas * p.chunk;
+    p.bytes = (p.prefix_rows + p.own_rows + p.piece_rows) * (dim + 1) * sizeof(float);
     return p;
 }
 
 int run_cached(const char *what, int dtype, Cached c, const Parts &parts, void *workspace, size_t workspace_bytes,
                cudaStream_t stream) {
     RODE_TRY(check_workspace(what, workspace, workspace_bytes, parts.bytes));
-    const int n = parts.prefix + parts.own;
-    if (n > 1) {
-        c.part_out = static_cast<float *>(workspace);
-        c.part_lse = c.part_out + static_cast<size_t>(n) * c.batch * c.win.heads * c.win.dim;
+    c.chunk = parts.chunk;
+    c.whole = parts.whole;
+    c.ctas = parts.ctas;
+    c.prefix_parts = parts.prefix;
+    const size_t dim = c.win.dim;
+    c.prefix_out = static_cast<float *>(workspace);
+    c.own_out = c.prefix_out + parts.prefix_rows * dim;
+    c.piece_out = c.own_out + parts.own_rows * dim;
+    c.prefix_lse = c.piece_out + parts.piece_rows * dim;
+    c.own_lse = c.prefix_lse + parts.prefix_rows;
+    c.piece_lse = c.own_lse + parts.own_rows;
+    const bool tensor_cores = step_takes(dtype, c);
+    if (!tensor_cores && c.chunk != kSimpleChunk) {  // 16-bit operands that are not whole 16-byte units
+        c.chunk = kSimpleChunk;
+        if (c.whole) c.ctas = c.batch * c.win.kv_heads * ((c.win.heads / c.win.kv_heads + kSimpleChunk - 1) / kSimpleChunk);
     }
-    if (parts.prefix > 0)
-        RODE_TRY(tiles_take_shared(dtype, c) ? tiles_shared(dtype, c, 0, parts.prefix, stream)
-                                             : simple_shared(dtype, c, 0, parts.prefix, stream));
-    RODE_TRY(step_takes(dtype, c) ? step_on_tensor_cores(dtype, c, parts.prefix, parts.own, stream)
-                                  : simple_step(dtype, c, parts.prefix, parts.own, stream));
-    if (n > 1) RODE_TRY(join_parts(dtype, c, n, stream));
+    if (parts.prefix > 0) RODE_TRY(tiles_take_shared(dtype, c) ? tiles_shared(dtype, c, stream) : simple_shared(dtype, c, stream));
+    RODE_TRY(tensor_cores ? step_on_tensor_cores(dtype, c, stream) : simple_step(dtype, c, stream));
+    if (parts.prefix > 0 || !parts.whole) RODE_TRY(join_parts(dtype, c, stream));
     return RODE_OK;
 }
 
@@ -234,14 +256,14 @@ static long long seen_at_most(int capacity, int window, int sinks) {
     return seen < capacity ? seen : capacity;
 }
 
-int rode_window_attention_step_workspace_bytes(int batch, int capacity, int heads, int kv_heads, int dim, int window,
+int rode_window_attention_step_workspace_bytes(int dtype, int batch, int capacity, int heads, int kv_heads, int dim, int window,
                                                int sinks, size_t *bytes) {
     const char *what = "rode_window_attention_step_workspace_bytes";
     if (bytes == nullptr) return fail(RODE_ERR_INVALID_ARGUMENT, "%s: null pointer bytes", what);
-    RODE_TRY(check_shape(what, RODE_F32, heads, kv_heads, dim, 1.f));
+    RODE_TRY(check_shape(what, dtype, heads, kv_heads, dim, 1.f));
     RODE_TRY(check_window(what, window, sinks));
     RODE_TRY(check_cached_sizes(what, batch, 0, capacity));
-    *bytes = plan_parts(batch, 0, seen_at_most(capacity, window, sinks), heads, kv_heads, dim).bytes;
+    *bytes = plan_parts(dtype, batch, 0, seen_at_most(capacity, window, sinks), heads, kv_heads, dim).bytes;
     return RODE_OK;
 }
 
@@ -270,17 +292,17 @@ int rode_window_attention_step(int dtype, int batch, int capacity, int heads, in
     }
     c.lengths = lengths;
     c.out = out;
-    return run_cached(what, dtype, c, plan_parts(batch, 0, seen_at_most(capacity, window, sinks), heads, kv_heads, dim), workspace,
+    return run_cached(what, dtype, c, plan_parts(dtype, batch, 0, seen_at_most(capacity, window, sinks), heads, kv_heads, dim), workspace,
                       workspace_bytes, stream);
 }
 
-int rode_shared_prefix_attention_workspace_bytes(int batch, int prefix, int capacity, int heads, int kv_heads, int dim,
+int rode_shared_prefix_attention_workspace_bytes(int dtype, int batch, int prefix, int capacity, int heads, int kv_heads, int dim,
                                                  size_t *bytes) {
     const char *what = "rode_shared_prefix_attention_workspace_bytes";
     if (bytes == nullptr) return fail(RODE_ERR_INVALID_ARGUMENT, "%s: null pointer bytes", what);
-    RODE_TRY(check_shape(what, RODE_F32, heads, kv_heads, dim, 1.f));
+    RODE_TRY(check_shape(what, dtype, heads, kv_heads, dim, 1.f));
     RODE_TRY(check_cached_sizes(what, batch, prefix, capacity));
-    *bytes = plan_parts(batch, prefix, capacity, heads, kv_heads, dim).bytes;
+    *bytes = plan_parts(dtype, batch, prefix, capacity, heads, kv_heads, dim).bytes;
     return RODE_OK;
 }
 
@@ -317,7 +339,7 @@ int rode_shared_prefix_attention(int dtype, int batch, int prefix, int capacity,
     }
     c.lengths = lengths;
     c.out = out;
-    return run_cached(what, dtype, c, plan_parts(batch, prefix, capacity, heads, kv_heads, dim), workspace, workspace_bytes, stream);
+    return run_cached(what, dtype, c, plan_parts(dtype, batch, prefix, capacity, heads, kv_heads, dim), workspace, workspace_bytes, stream);
 }
 
 int rode_attention_waits_failed(int *failed) {

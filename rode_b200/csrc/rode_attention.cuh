@@ -49,21 +49,31 @@ struct Prompt {
 };
 
 // One query per request against its cache and, if prefix > 0, against keys that all requests share.
+//
+// The work on the caches is a list of segments, (request, key head, chunk of the heads of its group), each with as many blocks of 16 keys as its request
+// sees.  `whole`: one CTA per segment.  Else all blocks, segment by segment, are dealt out to `ctas` CTAs in equal shares, whatever the
+// lengths are: a CTA works on the end of one segment, on whole ones, on the beginning of another.  What a CTA has of a segment that it shares with others is a
+// piece: 2 * cta for the first segment of its share, 2 * cta + 1 for the last one.
+constexpr int kTensorCoreChunk = 16, kSimpleChunk = 8;  // heads of a segment
 struct Cached {
     int batch, capacity, prefix;
     Window win;
     rode_heads_t q, k, v, pk, pv;
     const int *lengths;
     void *out;
-    // Partial results: [splits, batch, heads, dim] (normalised) and [splits, batch, heads] (base-2 logarithm of the sum)
-    float *part_out;
-    float *part_lse;
+    int chunk;  // heads of a segment
+    bool whole;
+    int ctas;
+    // Partial results, normalised, and the base-2 logarithms of their sums.  Prefix: [prefix_parts, batch, heads, dim] and without dim.  Own
+    // keys, if there is a prefix to join them with: [batch, heads, dim] of segments that one CTA had.  Pieces: [2 ctas, chunk, dim].
+    int prefix_parts;
+    float *prefix_out, *prefix_lse, *own_out, *own_lse, *piece_out, *piece_lse;
 };
 
 int simple_prompt(int dtype, const Prompt &p, cudaStream_t stream);
 int simple_prompt_backward(int dtype, const Prompt &p, cudaStream_t stream);
-int simple_shared(int dtype, const Cached &c, int first_split, int splits, cudaStream_t stream);
-int simple_step(int dtype, const Cached &c, int first_split, int splits, cudaStream_t stream);
+int simple_shared(int dtype, const Cached &c, cudaStream_t stream);
+int simple_step(int dtype, const Cached &c, cudaStream_t stream);
 
 // On the tensor cores, where *_take_* says so.
 bool tiles_take_prompt(int dtype, const Prompt &p);
@@ -76,12 +86,12 @@ struct FarPlan {
 };
 FarPlan plan_far(int n_seq, bool packed, int q_rows, int kv_heads, int dim, int window, int sinks);
 int tiles_backward(int dtype, const Prompt &p, cudaStream_t stream);
-int tiles_shared(int dtype, const Cached &c, int first_split, int splits, cudaStream_t stream);
+int tiles_shared(int dtype, const Cached &c, cudaStream_t stream);
 bool step_takes(int dtype, const Cached &c);
-int step_on_tensor_cores(int dtype, const Cached &c, int first_split, int splits, cudaStream_t stream);
+int step_on_tensor_cores(int dtype, const Cached &c, cudaStream_t stream);
 int tiles_waits_failed(int *failed);
 
-int join_parts(int dtype, const Cached &c, int splits, cudaStream_t stream);
+int join_parts(int dtype, const Cached &c, cudaStream_t stream);
 
 #ifdef __CUDACC__
 
@@ -191,10 +201,117 @@ __device__ __forceinline__ void store4(T *p, float4 v) {
     }
 }
 
+// Keys that the query of request b sees: those of the sinks, [0, sinks), and of the window, [lo, n); blocks of 16 of each.
+struct Seen {
+    int n, lo, sinks, sink_blocks, blocks;
+    __device__ __forceinline__ int first_of(int i) const { return i < sink_blocks ? i * 16 : lo + (i - sink_blocks) * 16; }
+    __device__ __forceinline__ int end_of(int i) const { return i < sink_blocks ? sinks : n; }
+};
+__device__ __forceinline__ Seen seen_by(const Cached &c, int b) {
+    Seen s;
+    s.n = min(max(__ldg(c.lengths + b), 0), c.capacity);
+    s.lo = max(s.n - c.win.window, 0);
+    s.sinks = min(c.win.sinks, s.lo);
+    s.sink_blocks = (s.sinks + 15) / 16;
+    s.blocks = s.sink_blocks + (s.n - s.lo + 15) / 16;
+    return s;
+}
+__device__ __forceinline__ int segments_per_request(const Cached &c) {
+    const int group = c.win.heads / c.win.kv_heads;
+    return c.win.kv_heads * ((group + c.chunk - 1) / c.chunk);
+}
+// Blocks of a CTA's share.
+__device__ __forceinline__ long long share_of(const Cached &c, long long total) { return (total + c.ctas - 1) / c.ctas; }
+
+// Where the share of CTA blockIdx.x begins and ends, in blocks of all segments, and the request that its first (or last) block is in, with that
+// request's own first block.  By all 128 threads of a CTA: each adds up a run of requests.
+struct Share {
+    long long begin, end, first;
+    int request;
+};
+__device__ __forceinline__ Share find_share(const Cached &c, bool last = false) {
+    __shared__ long long sums[4];
+    __shared__ Share found;
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, per = segments_per_request(c);
+    const int run = (c.batch + 127) / 128, b0 = min(static_cast<int>(threadIdx.x) * run, c.batch), b1 = min(b0 + run, c.batch);
+    long long mine = 0;
+    for (int b = b0; b < b1; ++b) mine += seen_by(c, b).blocks;
+    long long upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long x = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += x;
+    }
+    if (lane == 31) sums[warp] = upto;
+    __syncthreads();
+    long long before = upto - mine, total = 0;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+        if (u < warp) before += sums[u];
+        total += sums[u];
+    }
+    total *= per;
+    before *= per;
+    const long long share = share_of(c, total), begin = min(share * blockIdx.x, total), end = min(begin + share, total);
+    const long long at = last ? end - 1 : begin;
+    if (begin < end && at >= before && at < before + mine * per) {
+        int b = b0;
+        for (; b < b1; ++b) {
+            const long long blocks = static_cast<long long>(seen_by(c, b).blocks) * per;
+            if (at < before + blocks) break;
+            before += blocks;
+        }
+        found = {begin, end, before, b};
+    }
+    __syncthreads();
+    return begin < end ? found : Share{0, 0, 0, 0};
+}
+
+// Requests that see nothing are in no share: their rows become zero (with a prefix, join_rows does without them).
+template <typename T>
+__device__ __forceinline__ void clear_unseen(const Cached &c) {
+    if (c.whole || c.prefix_parts > 0) return;
+    for (int b = blockIdx.x; b < c.batch; b += gridDim.x) {
+        if (seen_by(c, b).blocks > 0) continue;
+        T *out = static_cast<T *>(c.out) + static_cast<long long>(b) * c.win.heads * c.win.dim;
+        for (int i = threadIdx.x * 4; i < c.win.heads * c.win.dim; i += 512) store4(out + i, make_float4(0.f, 0.f, 0.f, 0.f));
+    }
+}
+
 template <typename T>
 __device__ __forceinline__ const T *row_of(const rode_heads_t &x, long long batch, long long row, int head) {
     return static_cast<const T *>(x.data) + batch * x.batch + row * x.row + head * x.head;
 }
+
+// Where a CTA's result for a segment goes: to the output, to the rows that are joined with the prefix, or to a piece.
+struct StepResult {
+    float *lse;
+    float *part;
+    long long row;  // of the output
+    __device__ __forceinline__ StepResult(const Cached &c, int b, int head0, bool all, bool first_of_share) {
+        row = static_cast<long long>(b) * c.win.heads + head0;
+        lse = nullptr;
+        part = nullptr;
+        if (!all) {
+            const long long piece = (2ll * blockIdx.x + !first_of_share) * c.chunk;
+            lse = c.piece_lse + piece;
+            part = c.piece_out + piece * c.win.dim;
+        } else if (c.prefix_parts > 0) {
+            lse = c.own_lse + row;
+            part = c.own_out + row * c.win.dim;
+        }
+    }
+    template <typename T>
+    __device__ __forceinline__ void store(const Cached &c, int r, int d, float4 x) const {
+        if (part != nullptr)
+            store4(part + static_cast<long long>(r) * c.win.dim + d, x);
+        else
+            store4(static_cast<T *>(c.out) + (row + r) * c.win.dim + d, x);
+    }
+    __device__ __forceinline__ void store_lse(int r, float x) const {
+        if (lse != nullptr) lse[r] = x;
+    }
+};
 
 #endif  // __CUDACC__
 
@@ -203,6 +320,22 @@ template <typename K>
 int allow_shared(K *kernel, int bytes) {
     RODE_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
     return RODE_OK;
+}
+
+// How a kernel of a call on a cache is launched: `chained`, it may start beside the one before it.
+template <typename K, typename... A>
+cudaError_t launch_part(K *kernel, dim3 grid, int threads, int shared, cudaStream_t stream, bool chained, A... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = shared;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = chained ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
 }  // namespace rode

@@ -9,6 +9,9 @@
 // the shared memory); a thread holds 4 x 4 scores and 4 rows x dim / 16 columns of the result, so that eight 16-byte
 // loads from shared memory feed 64 FMAs.  Rows of shared memory are 4 floats longer than the tile: eight threads that read one
 // column of eight keys hit different banks.
+#include <algorithm>
+#include <type_traits>
+
 #include "rode_attention.cuh"
 
 namespace rode {
@@ -193,11 +196,12 @@ __global__ void __launch_bounds__(kThreads) prompt_rows(Prompt p) {
 
 // Queries of all requests that share a key head, row r = request r / group, head r % group of the group, against a part of the prefix.
 template <typename T, int kDim>
-__global__ void __launch_bounds__(kThreads) shared_rows(Cached c, int first_split, int splits) {
+__global__ void __launch_bounds__(kThreads) shared_rows(Cached c) {
     constexpr int kRows = tile_rows<kDim>(), R = kRows / 16;
     extern __shared__ float4 shared4[];
     float *qs = reinterpret_cast<float *>(shared4), *ks = qs + kRows * (kDim + 4), *vs = ks + kRows * (kDim + 4),
           *ws = vs + kRows * (kDim + 4);
+    chain_begin();  // the requests' own keys are worked on beside the prefix
     const Window &w = c.win;
     const int kv = blockIdx.y, group = w.heads / w.kv_heads, split = blockIdx.z;
     const int row0 = blockIdx.x * kRows, have = min(kRows, c.batch * group - row0);
@@ -218,8 +222,8 @@ __global__ void __launch_bounds__(kThreads) shared_rows(Cached c, int first_spli
     }
     const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
     const int blocks = (c.prefix + kRows - 1) / kRows;
-    const int b1 = static_cast<int>(static_cast<long long>(blocks) * (split + 1) / splits);
-    for (int b = static_cast<int>(static_cast<long long>(blocks) * split / splits); b < b1; ++b) {
+    const int b1 = static_cast<int>(static_cast<long long>(blocks) * (split + 1) / c.prefix_parts);
+    for (int b = static_cast<int>(static_cast<long long>(blocks) * split / c.prefix_parts); b < b1; ++b) {
         const int k0 = b * kRows, n = min(kRows, c.prefix - k0);
         __syncthreads();
         fetch_tile<T, kDim>(ks, row_of<T>(c.pk, 0, k0, kv), c.pk.row, n, w.dim);
@@ -240,15 +244,15 @@ __global__ void __launch_bounds__(kThreads) shared_rows(Cached c, int first_spli
         const int r = row0 + ty * R + i;
         if (ty * R + i >= have) continue;
         const float inv = l[i] > 0.f || l[i] != l[i] ? 1.f / l[i] : 0.f;
-        const long long at = (static_cast<long long>(first_split + split) * c.batch + r / group) * w.heads + kv * group + r % group;
+        const long long at = (static_cast<long long>(split) * c.batch + r / group) * w.heads + kv * group + r % group;
 #pragma unroll
         for (int d4 = 0; d4 < kDim / 64; ++d4) {
             const int d = (tx + 16 * d4) * 4;
             if (d < w.dim)
-                store4(c.part_out + at * w.dim + d,
+                store4(c.prefix_out + at * w.dim + d,
                        make_float4(acc[i][d4].x * inv, acc[i][d4].y * inv, acc[i][d4].z * inv, acc[i][d4].w * inv));
         }
-        if (tx == 0) c.part_lse[at] = m[i] == -INFINITY ? -INFINITY : m[i] + log2f(l[i]);
+        if (tx == 0) c.prefix_lse[at] = m[i] == -INFINITY ? -INFINITY : m[i] + log2f(l[i]);
     }
 }
 
@@ -423,155 +427,254 @@ __global__ void __launch_bounds__(kThreads) key_gradients(Prompt p) {
 
 // --- single tokens -------------------------------------------------------------------------------------------------------------
 
-// One request's queries of a key head (eight of them at a time) against a part of the keys that they see, which is the same for
-// all of them: key i of the list is key i of the cache for the sinks, then the window's.
-constexpr int kStepThreads = 128, kStepKeys = 32, kStepQueries = 8;
+// Segments of eight heads: the queries of a request and a key head against a part of the keys that they see, 32 at a time.
+constexpr int kStepThreads = 128, kStepKeys = 32, kStepQueries = kSimpleChunk;
 
 template <typename T, int kDim>
-__global__ void __launch_bounds__(kStepThreads) step_rows(Cached c, int first_split, int splits) {
+__global__ void __launch_bounds__(kStepThreads) step_rows(Cached c) {
     constexpr int kQuads = kDim / 4, kGroups = kStepThreads / kQuads, kPer = kStepQueries / kGroups;
     extern __shared__ float4 shared4[];
     float *ks = reinterpret_cast<float *>(shared4), *vs = ks + kStepKeys * (kDim + 4), *qs = vs + kStepKeys * (kDim + 4),
-          *ws = qs + kStepQueries * (kDim + 4), *keeps = ws + kStepQueries * kStepKeys, *sums = keeps + kStepQueries;
+          *ws = qs + kStepQueries * (kDim + 4), *keeps = ws + kStepQueries * kStepKeys, *sums = keeps + kStepQueries,
+          *tops = sums + kStepQueries;
+    chain_begin();
     const Window &w = c.win;
-    const int b = blockIdx.x, split = blockIdx.z, group = w.heads / w.kv_heads;
-    const int chunks = (group + kStepQueries - 1) / kStepQueries, kv = blockIdx.y / chunks;
-    const int g0 = blockIdx.y % chunks * kStepQueries, have = min(kStepQueries, group - g0), head0 = kv * group + g0;
-    const int n = min(max(__ldg(c.lengths + b), 0), c.capacity);
-    const int lo = max(n - w.window, 0), sinks = min(w.sinks, lo), seen = sinks + n - lo;
-    const int part = ((seen + splits - 1) / splits + kStepKeys - 1) / kStepKeys * kStepKeys;
-    const int begin = static_cast<int>(min(static_cast<long long>(part) * split, static_cast<long long>(seen)));
-    const int end = min(begin + part, seen);
+    const int group = w.heads / w.kv_heads, chunks = (group + kStepQueries - 1) / kStepQueries, per = w.kv_heads * chunks;
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
-    for (int i = tid; i < kStepQueries * kQuads; i += kStepThreads) {
-        const int r = i / kQuads, d = i % kQuads * 4;
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (r < have && d < w.dim) x = load4(row_of<T>(c.q, b, 0, head0 + r) + d);
-        *reinterpret_cast<float4 *>(qs + r * (kDim + 4) + d) = x;
-    }
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};  // of queries 2 * warp and 2 * warp + 1, in every lane
-    float4 acc[kPer];
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
     const int d0 = tid % kQuads * 4, r0 = tid / kQuads * kPer;
-    for (int k0 = begin; k0 < end; k0 += kStepKeys) {
-        const int keys = min(kStepKeys, end - k0);
+    Share share = {0, 0, 0, 0};
+    if (!c.whole) share = find_share(c);
+    clear_unseen<T>(c);
+    int b = c.whole ? blockIdx.x / per : share.request;
+    Seen seen = seen_by(c, b);
+    int y = c.whole ? blockIdx.x % per : 0;
+    long long first = share.first;  // of segment (b, y)
+    if (!c.whole && seen.blocks > 0) {
+        y = static_cast<int>((share.begin - first) / seen.blocks);
+        first += static_cast<long long>(y) * seen.blocks;
+    }
+    while (c.whole || first < share.end) {
+        const int from = c.whole ? 0 : static_cast<int>(max(share.begin - first, 0ll));
+        const int to = c.whole ? seen.blocks : static_cast<int>(min(share.end - first, static_cast<long long>(seen.blocks)));
+        const int kv = y / chunks, g0 = y % chunks * kStepQueries, have = min(kStepQueries, group - g0), head0 = kv * group + g0;
         __syncthreads();
-        for (int i = tid; i < kStepKeys * kQuads; i += kStepThreads) {
+        for (int i = tid; i < kStepQueries * kQuads; i += kStepThreads) {
             const int r = i / kQuads, d = i % kQuads * 4;
-            float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
-            if (r < keys && d < w.dim) {
-                const int j = k0 + r < sinks ? k0 + r : k0 + r - sinks + lo;
-                x = load4(row_of<T>(c.k, b, j, kv) + d);
-                y = load4(row_of<T>(c.v, b, j, kv) + d);
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (r < have && d < w.dim) x = load4(row_of<T>(c.q, b, 0, head0 + r) + d);
+            *reinterpret_cast<float4 *>(qs + r * (kDim + 4) + d) = x;
+        }
+        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};  // of queries 2 * warp and 2 * warp + 1, in every lane
+        float4 acc[kPer];
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int i = from; i < to; i += 2) {  // two blocks of 16 keys
+            __syncthreads();
+            for (int x = tid; x < kStepKeys * kQuads; x += kStepThreads) {
+                const int r = x / kQuads, d = x % kQuads * 4, block = i + r / 16;
+                const int j = seen.first_of(block) + r % 16;
+                float4 key = make_float4(0.f, 0.f, 0.f, 0.f), value = key;
+                if (block < to && j < seen.end_of(block) && d < w.dim) {
+                    key = load4(row_of<T>(c.k, b, j, kv) + d);
+                    value = load4(row_of<T>(c.v, b, j, kv) + d);
+                }
+                *reinterpret_cast<float4 *>(ks + r * (kDim + 4) + d) = key;
+                *reinterpret_cast<float4 *>(vs + r * (kDim + 4) + d) = value;
             }
-            *reinterpret_cast<float4 *>(ks + r * (kDim + 4) + d) = x;
-            *reinterpret_cast<float4 *>(vs + r * (kDim + 4) + d) = y;
-        }
-        __syncthreads();
-        {
-            const int key = tid / 4, r = tid % 4 * 2;
-            float s0 = 0.f, s1 = 0.f;
-            for (int d = 0; d < w.dim; d += 4) {
-                const float4 x = *reinterpret_cast<const float4 *>(ks + key * (kDim + 4) + d);
-                const float4 y = *reinterpret_cast<const float4 *>(qs + r * (kDim + 4) + d);
-                const float4 z = *reinterpret_cast<const float4 *>(qs + (r + 1) * (kDim + 4) + d);
-                s0 = fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, fmaf(x.w, y.w, s0))));
-                s1 = fmaf(x.x, z.x, fmaf(x.y, z.y, fmaf(x.z, z.z, fmaf(x.w, z.w, s1))));
+            __syncthreads();
+            {
+                const int key = tid / 4, r = tid % 4 * 2;
+                float s0 = 0.f, s1 = 0.f;
+                for (int d = 0; d < w.dim; d += 4) {
+                    const float4 x = *reinterpret_cast<const float4 *>(ks + key * (kDim + 4) + d);
+                    const float4 p = *reinterpret_cast<const float4 *>(qs + r * (kDim + 4) + d);
+                    const float4 z = *reinterpret_cast<const float4 *>(qs + (r + 1) * (kDim + 4) + d);
+                    s0 = fmaf(x.x, p.x, fmaf(x.y, p.y, fmaf(x.z, p.z, fmaf(x.w, p.w, s0))));
+                    s1 = fmaf(x.x, z.x, fmaf(x.y, z.y, fmaf(x.z, z.z, fmaf(x.w, z.w, s1))));
+                }
+                const int block = i + key / 16;
+                const bool in = block < to && seen.first_of(block) + key % 16 < seen.end_of(block);
+                ws[r * kStepKeys + key] = in ? s0 * (w.scale * kLog2e) : -INFINITY;
+                ws[(r + 1) * kStepKeys + key] = in ? s1 * (w.scale * kLog2e) : -INFINITY;
             }
-            const bool in = key < keys;
-            ws[r * kStepKeys + key] = in ? s0 * (w.scale * kLog2e) : -INFINITY;
-            ws[(r + 1) * kStepKeys + key] = in ? s1 * (w.scale * kLog2e) : -INFINITY;
+            __syncthreads();
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int r = 2 * warp + u;
+                const float s = ws[r * kStepKeys + lane];
+                float top = s;
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                const float next = fmaxf(m[u], top), base = next == -INFINITY ? 0.f : next;
+                const float keep = exp2f(m[u] - base), e = exp2f(s - base);
+                float sum = e;
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                l[u] = l[u] * keep + sum;
+                m[u] = next;
+                ws[r * kStepKeys + lane] = e;
+                if (lane == 0) keeps[r] = keep;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int x = 0; x < kPer; ++x) {
+                const float keep = keeps[r0 + x];
+                acc[x].x *= keep;
+                acc[x].y *= keep;
+                acc[x].z *= keep;
+                acc[x].w *= keep;
+            }
+            for (int key = 0; key < kStepKeys; ++key) {
+                const float4 value = *reinterpret_cast<const float4 *>(vs + key * (kDim + 4) + d0);
+#pragma unroll
+                for (int x = 0; x < kPer; ++x) vfma(acc[x], ws[(r0 + x) * kStepKeys + key], value);
+            }
+        }
+        if (lane == 0) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                sums[2 * warp + u] = l[u];
+                tops[2 * warp + u] = m[u];
+            }
         }
         __syncthreads();
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int r = 2 * warp + u;
-            const float s = ws[r * kStepKeys + lane];
-            float top = s;
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            const float next = fmaxf(m[u], top), base = next == -INFINITY ? 0.f : next;
-            const float keep = exp2f(m[u] - base), e = exp2f(s - base);
-            float sum = e;
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            l[u] = l[u] * keep + sum;
-            m[u] = next;
-            ws[r * kStepKeys + lane] = e;
-            if (lane == 0) keeps[r] = keep;
-        }
-        __syncthreads();
+        const StepResult result(c, b, head0, from == 0 && to == seen.blocks, first < share.begin || c.whole);
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
-            const float keep = keeps[r0 + i];
-            acc[i].x *= keep;
-            acc[i].y *= keep;
-            acc[i].z *= keep;
-            acc[i].w *= keep;
+            const int r = r0 + i;
+            if (r >= have || d0 >= w.dim) continue;
+            const float inv = sums[r] > 0.f || sums[r] != sums[r] ? 1.f / sums[r] : 0.f;
+            result.store<T>(c, r, d0, make_float4(acc[i].x * inv, acc[i].y * inv, acc[i].z * inv, acc[i].w * inv));
+            if (d0 == 0) result.store_lse(r, tops[r] == -INFINITY ? -INFINITY : tops[r] + log2f(sums[r]));
         }
-        for (int key = 0; key < kStepKeys; ++key) {
-            const float4 y = *reinterpret_cast<const float4 *>(vs + key * (kDim + 4) + d0);
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) vfma(acc[i], ws[(r0 + i) * kStepKeys + key], y);
-        }
-    }
-    if (lane == 0) {
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int r = 2 * warp + u;
-            sums[r] = l[u];
-            if (c.part_out != nullptr && r < have)
-                c.part_lse[(static_cast<long long>(first_split + split) * c.batch + b) * w.heads + head0 + r] =
-                    m[u] == -INFINITY ? -INFINITY : m[u] + log2f(l[u]);
+        if (c.whole) break;
+        first += seen.blocks;
+        if (++y == per) {
+            y = 0;
+            do {
+                if (first >= share.end || ++b >= c.batch) break;
+                seen = seen_by(c, b);
+            } while (seen.blocks == 0);
         }
     }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-        const int r = r0 + i;
-        if (r >= have || d0 >= w.dim) continue;
-        const float inv = sums[r] > 0.f || sums[r] != sums[r] ? 1.f / sums[r] : 0.f;
-        const float4 x = make_float4(acc[i].x * inv, acc[i].y * inv, acc[i].z * inv, acc[i].w * inv);
-        const long long at = static_cast<long long>(b) * w.heads + head0 + r;
-        if (c.part_out != nullptr)
-            store4(c.part_out + (static_cast<long long>(first_split + split) * c.batch * w.heads + at) * w.dim + d0, x);
-        else
-            store4(static_cast<T *>(c.out) + at * w.dim + d0, x);
-    }
+    if (blockIdx.x == 0) chain_wait();  // this grid is not complete before the prefix is
 }
 
 template <int kDim>
 constexpr int step_shared() {
-    return 4 * ((2 * kStepKeys + kStepQueries) * (kDim + 4) + kStepQueries * kStepKeys + 2 * kStepQueries);
+    return 4 * ((2 * kStepKeys + kStepQueries) * (kDim + 4) + kStepQueries * kStepKeys + 3 * kStepQueries);
 }
 
-// Joins the parts of every row: weights 2^(lse - max lse).  A warp per row.
-template <typename T>
-__global__ void __launch_bounds__(128) join_rows(Cached c, int splits) {
-    const long long rows = static_cast<long long>(c.batch) * c.win.heads, row = blockIdx.x * 4ll + threadIdx.x / 32;
-    if (row >= rows) return;
-    const int lane = threadIdx.x % 32, dim = c.win.dim;
-    const float *lse = c.part_lse + row;
-    const float *part = c.part_out + row * dim;
+// Result of one row from its parts, by all 128 threads: weights 2^(lse - max lse), the warps take the parts in turn.  lse_of(s) and part_of(s, d):
+// part s's base-2 logarithm and its columns d .. d + 3.
+template <typename T, typename Lse, typename Part>
+__device__ __forceinline__ void join_parts_of_row(T *out, int dim, int parts, Lse &&lse_of, Part &&part_of) {
+    __shared__ float4 joined[4][64];
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     float top = -INFINITY, sum = 0.f;
-    for (int s = lane; s < splits; s += 32) top = fmaxf(top, lse[s * rows]);
+    for (int s = lane; s < parts; s += 32) top = fmaxf(top, lse_of(s));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     if (top == -INFINITY) top = 0.f;
-    for (int s = lane; s < splits; s += 32) sum += exp2f(lse[s * rows] - top);
+    for (int s = lane; s < parts; s += 32) sum += exp2f(lse_of(s) - top);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
     for (int d = lane * 4; d < dim; d += 128) {
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int s = 0; s < splits; ++s) {
-            const float x = exp2f(lse[s * rows] - top);
+#pragma unroll 4
+        for (int s = warp; s < parts; s += 4) {
+            const float x = exp2f(lse_of(s) - top);
+            const float4 part = part_of(s, d);
             // (a part without keys has no weight, whatever its rows hold)
-            if (x != 0.f) vfma(acc, x * inv, *reinterpret_cast<const float4 *>(part + s * rows * dim + d));
+            if (x != 0.f) vfma(acc, x * inv, part);
         }
-        store4(static_cast<T *>(c.out) + row * dim + d, acc);
+        joined[warp][d / 4] = acc;
     }
+    __syncthreads();
+    for (int d = threadIdx.x; d < dim / 4; d += 128) {
+        float4 acc = joined[0][d];
+#pragma unroll
+        for (int u = 1; u < 4; ++u) vadd(acc, joined[u][d]);
+        store4(out + d * 4, acc);
+    }
+    __syncthreads();
+}
+
+// Segments in pieces, without a prefix: CTA (x, r) has head r of the segment that begins in share x and goes on behind it.  (A CTA per row of
+// the result, most of which have no pieces, took 13 us behind step_batch.)
+template <typename T>
+__global__ void __launch_bounds__(128) join_pieces(Cached c) {
+    const int group = c.win.heads / c.win.kv_heads, chunks = (group + c.chunk - 1) / c.chunk, per = c.win.kv_heads * chunks;
+    const Share share = find_share(c, true);
+    const float *piece_lse = after_chain(c.piece_lse), *piece_out = after_chain(c.piece_out);
+    if (share.begin >= share.end) return;
+    const int blocks = seen_by(c, share.request).blocks;
+    const int y = static_cast<int>((share.end - 1 - share.first) / blocks);
+    const long long begin = share.first + static_cast<long long>(y) * blocks, end = begin + blocks, size = share.end - share.begin;
+    if (begin < share.begin || end <= share.end) return;  // another share's, or whole (the last share ends with its segment)
+    const int r = blockIdx.y, g = y % chunks * c.chunk + r;
+    if (g >= group) return;
+    const int parts = 1 + static_cast<int>((end - share.end + size - 1) / size);
+    const auto place = [&](int s) { return (2ll * (blockIdx.x + s) + (s == 0)) * c.chunk + r; };
+    const int dim = c.win.dim;
+    join_parts_of_row(static_cast<T *>(c.out) + (static_cast<long long>(share.request) * c.win.heads + y / chunks * group + g) * dim, dim, parts,
+                      [&](int s) { return __ldcg(piece_lse + place(s)); },
+                      [&](int s, int d) { return __ldcg(reinterpret_cast<const float4 *>(piece_out + place(s) * dim + d)); });
+}
+
+// With a prefix: every row, from the prefix's parts and what its own keys gave, which is one row or some pieces.
+template <typename T>
+__global__ void __launch_bounds__(128) join_rows(Cached c) {
+    __shared__ long long below[4], all[4];
+    const long long rows = static_cast<long long>(c.batch) * c.win.heads, row = blockIdx.x;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, dim = c.win.dim;
+    const int b = static_cast<int>(row / c.win.heads), head = static_cast<int>(row % c.win.heads), group = c.win.heads / c.win.kv_heads;
+    const int in_group = head % group, per = segments_per_request(c), y = head / group * (per / c.win.kv_heads) + in_group / c.chunk;
+    // the CTAs that had a part of this row's segment
+    int c0 = 0, c1 = 0;
+    bool none = false;
+    if (!c.whole) {
+        long long mine = 0, sum = 0;
+        for (int i = threadIdx.x; i < c.batch; i += 128) {
+            const int blocks = seen_by(c, i).blocks;
+            sum += blocks;
+            if (i < b) mine += blocks;
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            mine += __shfl_xor_sync(0xffffffffu, mine, o);
+            sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        }
+        if (lane == 0) {
+            below[warp] = mine;
+            all[warp] = sum;
+        }
+        __syncthreads();
+        const int blocks = seen_by(c, b).blocks;
+        const long long begin = (below[0] + below[1] + below[2] + below[3]) * per + static_cast<long long>(y) * blocks;
+        const long long share = max(share_of(c, (all[0] + all[1] + all[2] + all[3]) * per), 1ll);
+        none = blocks == 0;
+        c0 = static_cast<int>(begin / share);
+        c1 = none ? c0 : static_cast<int>((begin + blocks - 1) / share);
+    }
+    const bool pieces = c1 > c0;
+    const int parts = c.prefix_parts + (none ? 0 : c1 - c0 + 1);
+    // (through the result of the wait: what the grids before this one have written)
+    const float *prefix_lse = after_chain(c.prefix_lse), *own_lse = after_chain(c.own_lse), *piece_lse = after_chain(c.piece_lse);
+    const float *prefix_out = after_chain(c.prefix_out), *own_out = after_chain(c.own_out), *piece_out = after_chain(c.piece_out);
+    const auto place = [&](int s) {  // of part s, in rows of its array
+        if (s < c.prefix_parts) return s * rows + row;
+        if (!pieces) return row;
+        const int i = s - c.prefix_parts;
+        return (2ll * (c0 + i) + (i == 0)) * c.chunk + in_group % c.chunk;
+    };
+    join_parts_of_row(static_cast<T *>(c.out) + row * dim, dim, parts,
+                      [&](int s) { return __ldcg((s < c.prefix_parts ? prefix_lse : pieces ? piece_lse : own_lse) + place(s)); },
+                      [&](int s, int d) {
+                          const float *from = s < c.prefix_parts ? prefix_out : pieces ? piece_out : own_out;
+                          return __ldcg(reinterpret_cast<const float4 *>(from + place(s) * dim + d));
+                      });
 }
 
 template <typename F>
@@ -624,7 +727,7 @@ int simple_prompt_backward(int dtype, const Prompt &p, cudaStream_t stream) {
     });
 }
 
-int simple_shared(int dtype, const Cached &c, int first_split, int splits, cudaStream_t stream) {
+int simple_shared(int dtype, const Cached &c, cudaStream_t stream) {
     return by_type(dtype, [&](auto *type) {
         return by_dim(c.win.dim, [&](auto dim) {
             using T = std::remove_pointer_t<decltype(type)>;
@@ -633,35 +736,34 @@ int simple_shared(int dtype, const Cached &c, int first_split, int splits, cudaS
             if (const int e = allow_shared(kernel, forward_shared<kDim>())) return e;
             const long long rows = static_cast<long long>(c.batch) * (c.win.heads / c.win.kv_heads);
             const int tiles = static_cast<int>((rows + tile_rows<kDim>() - 1) / tile_rows<kDim>());
-            kernel<<<dim3(tiles, c.win.kv_heads, splits), kThreads, forward_shared<kDim>(), stream>>>(c, first_split, splits);
+            kernel<<<dim3(tiles, c.win.kv_heads, c.prefix_parts), kThreads, forward_shared<kDim>(), stream>>>(c);
             RODE_CHECK_LAUNCH("shared_rows");
             return static_cast<int>(RODE_OK);
         });
     });
 }
 
-int simple_step(int dtype, const Cached &c, int first_split, int splits, cudaStream_t stream) {
+int simple_step(int dtype, const Cached &c, cudaStream_t stream) {
     return by_type(dtype, [&](auto *type) {
         return by_dim(c.win.dim, [&](auto dim) {
             using T = std::remove_pointer_t<decltype(type)>;
             constexpr int kDim = decltype(dim)::value;
             auto *kernel = &step_rows<T, kDim>;
             if (const int e = allow_shared(kernel, step_shared<kDim>())) return e;
-            const int chunks = (c.win.heads / c.win.kv_heads + kStepQueries - 1) / kStepQueries;
-            kernel<<<dim3(c.batch, c.win.kv_heads * chunks, splits), kStepThreads, step_shared<kDim>(), stream>>>(c, first_split,
-                                                                                                                  splits);
-            RODE_CHECK_LAUNCH("step_rows");
+            RODE_CUDA_TRY(launch_part(kernel, dim3(c.ctas), kStepThreads, step_shared<kDim>(), stream, c.prefix_parts > 0, c));
             return static_cast<int>(RODE_OK);
         });
     });
 }
 
-int join_parts(int dtype, const Cached &c, int splits, cudaStream_t stream) {
+int join_parts(int dtype, const Cached &c, cudaStream_t stream) {
     return by_type(dtype, [&](auto *type) {
         using T = std::remove_pointer_t<decltype(type)>;
         const long long rows = static_cast<long long>(c.batch) * c.win.heads;
-        join_rows<T><<<static_cast<unsigned>((rows + 3) / 4), 128, 0, stream>>>(c, splits);
-        RODE_CHECK_LAUNCH("join_rows");
+        if (c.prefix_parts > 0)
+            RODE_CUDA_TRY(launch_part(&join_rows<T>, dim3(static_cast<unsigned>(rows)), 128, 0, stream, true, c));
+        else
+            RODE_CUDA_TRY(launch_part(&join_pieces<T>, dim3(c.ctas, std::min(c.chunk, c.win.heads / c.win.kv_heads)), 128, 0, stream, true, c));
         return static_cast<int>(RODE_OK);
     });
 }

@@ -208,7 +208,7 @@ __device__ __forceinline__ void give_registers() { asm volatile("setmaxnreg.dec.
 // kShared: rows are requests, keys a part of the prefix, results go to the parts; else prompts.
 template <typename T, int kDim, bool kShared>
 __global__ void __launch_bounds__(kTileThreads, 1)
-    forward_tiles(const __grid_constant__ TileMaps maps, const Prompt p, const Cached c, int first_split, int splits) {
+    forward_tiles(const __grid_constant__ TileMaps maps, const Prompt p, const Cached c) {
     constexpr int kPanels = kDim / 64, kStages = forward_stages<kDim>(), kTile = kPanels * kPanel;
     extern __shared__ char shared_raw[];
     const Window &w = kShared ? c.win : p.win;
@@ -216,6 +216,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 
     Work wk;
     if constexpr (kShared) {
+        chain_begin();  // the requests' own keys are worked on beside the prefix
         wk.row0 = static_cast<long long>(blockIdx.x) * 2 * per_tile;
         wk.n_queries = static_cast<int>(min(static_cast<long long>(2 * per_tile), c.batch - wk.row0));
         wk.pos0 = 0;
@@ -223,8 +224,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         wk.keys = c.prefix;
         const long long all = (c.prefix + kRows - 1) / kRows;
         wk.n_sink = 0;
-        wk.first = static_cast<int>(all * blockIdx.z / splits);
-        wk.blocks = static_cast<int>(all * (blockIdx.z + 1) / splits) - wk.first;
+        wk.first = static_cast<int>(all * blockIdx.z / c.prefix_parts);
+        wk.blocks = static_cast<int>(all * (blockIdx.z + 1) / c.prefix_parts) - wk.first;
     } else {
         const Tile t = find_tile(p.seqs.q_offsets, p.seqs.n_seq, p.seqs.q_rows, blockIdx.x, 2 * per_tile);
         if (t.first < 0 || t.first >= t.rows || (t.seq < 0 && !p.clear)) return;
@@ -487,8 +488,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
         const float lse2 = m == -INFINITY ? -INFINITY : m * s2 + log2f(l);
         if (kShared) {
-            const long long at = ((first_split + blockIdx.z) * static_cast<long long>(c.batch) + wk.row0 + t * per_tile + query) * w.heads + head;
-            if (mine) c.part_lse[at] = lse2;
+            const long long at = (blockIdx.z * static_cast<long long>(c.batch) + wk.row0 + t * per_tile + query) * w.heads + head;
+            if (mine) c.prefix_lse[at] = lse2;
 #pragma unroll
             for (int x = 0; x < kDim; x += 32) {
                 uint32_t o[32];
@@ -497,7 +498,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll
                 for (int j = 0; j < 32; j += 4)
                     if (mine && x + j < w.dim)
-                        store4(c.part_out + at * w.dim + x + j,
+                        store4(c.prefix_out + at * w.dim + x + j,
                                done > 0 ? make_float4(__uint_as_float(o[j]) * inv, __uint_as_float(o[j + 1]) * inv,
                                                       __uint_as_float(o[j + 2]) * inv, __uint_as_float(o[j + 3]) * inv)
                                         : make_float4(0.f, 0.f, 0.f, 0.f));
@@ -555,13 +556,14 @@ struct GradientMaps {
     CUtensorMap q, dout, k, v;
 };
 
-// delta = do . o of the rows of a tile (kRows of them, row r = query r / group, head r % group) by eight warps: sixteen lanes per row, so that a
-// warp reads two rows at once.
-template <typename T>
+// delta = do . o of the rows of a tile (kRows of them, row r = query r / group, head r % group) by eight warps, a lane per 16 bytes, so that a warp
+// reads two or four rows at once.
+template <typename T, int kDim>
 __device__ __forceinline__ void row_deltas(const Prompt &p, long long row0, int head0, int group, int n, uint32_t deltas) {
-    const int dim = p.win.dim, piece = threadIdx.x % 16, d = piece * 8;
+    constexpr int kLanes = kDim / 8;
+    const int dim = p.win.dim, piece = threadIdx.x % kLanes, d = piece * 8;
 #pragma unroll
-    for (int r = threadIdx.x / 16; r < kRows; r += 16) {
+    for (int r = threadIdx.x / kLanes; r < kRows; r += 256 / kLanes) {
         const int query = r / group, head = head0 + r % group;
         float sum = 0.f;
         if (query < n && d < dim) {
@@ -572,7 +574,7 @@ __device__ __forceinline__ void row_deltas(const Prompt &p, long long row0, int 
             for (int i = 0; i < 8; ++i) sum = fmaf(to_float(s[i]), to_float(t[i]), sum);
         }
 #pragma unroll
-        for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        for (int o = kLanes / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if (piece == 0) asm volatile("st.shared.f32 [%0], %1;" ::"r"(deltas + 4 * r), "f"(sum) : "memory");
     }
 }
@@ -752,7 +754,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) query_gradient_tiles(const __
             const float lse = __ldg(p.lse + at);
             off = lse == -INFINITY ? 0.f : -lse * kLog2e;
         }
-        row_deltas<T>(p, row0, kv * group, group, n, deltas);
+        row_deltas<T, kDim>(p, row0, kv * group, group, n, deltas);
         asm volatile("bar.sync 1, 256;" ::: "memory");  // these two warpgroups
         asm volatile("ld.shared.f32 %0, [%1];" : "=f"(delta) : "r"(deltas + 4 * r) : "memory");
         if (mine && half == 0) p.delta[at] = delta;
@@ -1231,7 +1233,7 @@ int tiles_prompt(int dtype, const Prompt &p, cudaStream_t stream) {
         if (const int e = encode(&maps.k, dtype, p.k, p.k.row, p.seqs.k_rows, w.kv_heads, w.dim, 1, kRows)) return e;
         if (const int e = encode(&maps.v, dtype, p.v, p.v.row, p.seqs.k_rows, w.kv_heads, w.dim, 1, kRows)) return e;
         const int slots = tile_slots(p.seqs.q_offsets, p.seqs.n_seq, p.seqs.q_rows, 2 * per_tile);
-        kernel<<<dim3(slots, w.kv_heads), kTileThreads, forward_bytes<kDim>(), stream>>>(maps, p, Cached{}, 0, 1);
+        kernel<<<dim3(slots, w.kv_heads), kTileThreads, forward_bytes<kDim>(), stream>>>(maps, p, Cached{});
         RODE_CHECK_LAUNCH("forward_tiles");
         return static_cast<int>(RODE_OK);
     });
@@ -1282,7 +1284,7 @@ int tiles_backward(int dtype, const Prompt &p, cudaStream_t stream) {
     });
 }
 
-int tiles_shared(int dtype, const Cached &c, int first_split, int splits, cudaStream_t stream) {
+int tiles_shared(int dtype, const Cached &c, cudaStream_t stream) {
     const Window &w = c.win;
     const int group = w.heads / w.kv_heads, per_tile = kRows / group;
     TileMaps maps;
@@ -1295,7 +1297,7 @@ int tiles_shared(int dtype, const Cached &c, int first_split, int splits, cudaSt
         if (const int e = encode(&maps.k, dtype, c.pk, c.pk.row, c.prefix, w.kv_heads, w.dim, 1, kRows)) return e;
         if (const int e = encode(&maps.v, dtype, c.pv, c.pv.row, c.prefix, w.kv_heads, w.dim, 1, kRows)) return e;
         const int tiles = (c.batch + 2 * per_tile - 1) / (2 * per_tile);
-        kernel<<<dim3(tiles, w.kv_heads, splits), kTileThreads, forward_bytes<kDim>(), stream>>>(maps, Prompt{}, c, first_split, splits);
+        kernel<<<dim3(tiles, w.kv_heads, c.prefix_parts), kTileThreads, forward_bytes<kDim>(), stream>>>(maps, Prompt{}, c);
         RODE_CHECK_LAUNCH("forward_tiles");
         return static_cast<int>(RODE_OK);
     });

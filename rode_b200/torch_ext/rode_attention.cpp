@@ -226,7 +226,7 @@ Tensor py_window_step(const Tensor &q_in, const Tensor &k_cache, const Tensor &v
     const Tensor q = fitting(q_in);
     Tensor out = empty_on(q.sizes(), q.scalar_type(), q.device());
     size_t bytes = 0;
-    check_status(rode_window_attention_step_workspace_bytes(c.batch, c.capacity, c.heads, c.kv_heads, c.dim, window_of(window),
+    check_status(rode_window_attention_step_workspace_bytes(c.dtype, c.batch, c.capacity, c.heads, c.kv_heads, c.dim, window_of(window),
                                                             sinks_of(sinks), &bytes));
     Tensor ws;
     if (bytes > 0) ws = empty_on({static_cast<int64_t>(bytes)}, torch::kUInt8, q.device());
@@ -252,7 +252,7 @@ Tensor py_shared_prefix(const Tensor &q_in, const Tensor &prefix_k, const Tensor
     const int prefix = to_int(prefix_k.size(0), "prefix");
     Tensor out = empty_on(q.sizes(), q.scalar_type(), q.device());
     size_t bytes = 0;
-    check_status(rode_shared_prefix_attention_workspace_bytes(c.batch, prefix, c.capacity, c.heads, c.kv_heads, c.dim, &bytes));
+    check_status(rode_shared_prefix_attention_workspace_bytes(c.dtype, c.batch, prefix, c.capacity, c.heads, c.kv_heads, c.dim, &bytes));
     Tensor ws;
     if (bytes > 0) ws = empty_on({static_cast<int64_t>(bytes)}, torch::kUInt8, q.device());
     const rode_heads_t qh = batch_heads(q), pk = rows_heads(prefix_k), pv = rows_heads(prefix_v);

@@ -50,17 +50,17 @@ def test_workspaces(built_library):
     assert back(None, 0) == WS and back(256, 8) == WS and back(264, 1 << 20) == WS
     assert back(256, 1 << 20, dk=None) == BAD and back(256, 1 << 20, dv=None) == BAD
     for batch, capacity, window, sinks in ((1, 100000, 100000, 0), (2, 5000, 3000, 4)):
-        assert lib.rode_window_attention_step_workspace_bytes(batch, capacity, 8, 2, 64, window, sinks, ctypes.byref(need)) == 0
+        assert lib.rode_window_attention_step_workspace_bytes(0, batch, capacity, 8, 2, 64, window, sinks, ctypes.byref(need)) == 0
         assert need.value > 0
         step = lambda ws, n: lib.rode_window_attention_step(0, batch, capacity, 8, 2, 64, window, sinks, 1.0, _heads(batch=512), _heads(),
                                                             _heads(), 256, 256, ws, n, None)
         assert step(None, 0) == WS and step(256, need.value - 1) == WS and step(260, need.value) == WS
-    assert lib.rode_window_attention_step_workspace_bytes(1, 8, 8, 2, 64, 8, 0, ctypes.byref(need)) == 0 and need.value == 0
+    assert lib.rode_window_attention_step_workspace_bytes(0, 1, 8, 8, 2, 64, 8, 0, ctypes.byref(need)) == 0 and need.value == 0
     assert lib.rode_window_attention_step(0, 1, 8, 8, 2, 64, 8, 0, 1.0, _heads(), _heads(), _heads(), None, 256, None, 0, None) == BAD
-    assert lib.rode_shared_prefix_attention_workspace_bytes(2, 500, 8, 8, 2, 64, ctypes.byref(need)) == 0 and need.value > 0
+    assert lib.rode_shared_prefix_attention_workspace_bytes(0, 2, 500, 8, 8, 2, 64, ctypes.byref(need)) == 0 and need.value > 0
     assert lib.rode_shared_prefix_attention(0, 2, 500, 8, 8, 2, 64, 1.0, _heads(), _heads(), _heads(), _heads(), _heads(), 256, 256, 256,
                                             need.value - 1, None) == WS
-    assert lib.rode_shared_prefix_attention_workspace_bytes(2, -1, 8, 8, 2, 64, ctypes.byref(need)) == BAD
+    assert lib.rode_shared_prefix_attention_workspace_bytes(0, 2, -1, 8, 8, 2, 64, ctypes.byref(need)) == BAD
 
 
 def test_reference_gradients_are_the_differences():
