@@ -95,6 +95,32 @@ int join_parts(int dtype, const Cached &c, cudaStream_t stream);
 
 #ifdef __CUDACC__
 
+// Two numbers in one 64-bit register: one instruction for both.
+struct Pair {
+    unsigned long long x;
+};
+__device__ __forceinline__ Pair pair_of(float a, float b) {
+    Pair r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r.x) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void split(Pair p, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p.x)); }
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+    Pair r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.x) : "l"(a.x), "l"(b.x), "l"(c.x));
+    return r;
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+    Pair r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.x) : "l"(a.x), "l"(b.x));
+    return r;
+}
+
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+    Pair r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.x) : "l"(a.x), "l"(b.x));
+    return r;
+}
 // One tile of a sequence.  Boundaries of the sequences, extended by the rows in front of the first and behind the last one, are
 // cut into tiles; sequence e's tiles start at slot boundary(e) / tile + e, so that a slot finds its sequence by bisection
 // over the offsets and a grid of rows / tile + n_seq + 2 slots covers any lengths, which the host does not know.

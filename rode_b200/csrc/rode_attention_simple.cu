@@ -24,42 +24,59 @@ constexpr int tile_rows() {
     return kDim <= 128 ? 64 : 32;
 }
 
-// rows x kDim floats, columns beyond dim and rows beyond `have` zero.
+// rows x kDim floats, columns beyond dim and rows beyond `have` zero.  The loads first, then the stores.
 template <typename T, int kDim>
 __device__ __forceinline__ void fetch_tile(float *dst, const T *src, long long stride, int have, int dim) {
-    constexpr int kRows = tile_rows<kDim>();
-    for (int i = threadIdx.x; i < kRows * (kDim / 4); i += kThreads) {
-        const int r = i / (kDim / 4), c = i % (kDim / 4) * 4;
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (r < have && c < dim) x = load4(src + r * stride + c);
-        *reinterpret_cast<float4 *>(dst + r * (kDim + 4) + c) = x;
+    constexpr int kQuads = kDim / 4, kLoads = tile_rows<kDim>() * kQuads / kThreads;
+    float4 x[kLoads];
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u) {
+        const int i = threadIdx.x + u * kThreads, r = i / kQuads, c = i % kQuads * 4;
+        x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (r < have && c < dim) x[u] = load4(src + r * stride + c);
     }
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u) {
+        const int i = threadIdx.x + u * kThreads, r = i / kQuads, c = i % kQuads * 4;
+        *reinterpret_cast<float4 *>(dst + r * (kDim + 4) + c) = x[u];
+    }
+}
+
+__device__ __forceinline__ void load_pairs(const float *p, Pair (&x)[2]) {
+    const ulonglong2 v = *reinterpret_cast<const ulonglong2 *>(p);
+    x[0].x = v.x;
+    x[1].x = v.y;
 }
 
 // acc[i][j] = a[row i] . b[row j] for rows ty * R + i and tx + 16 * j
 template <int kDim, int R>
 __device__ __forceinline__ void dot_tile(const float *a, const float *b, int dim, float (&acc)[R][R]) {
     const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
+    Pair two[R][R];  // sums over even and odd head dimensions
 #pragma unroll
     for (int i = 0; i < R; ++i)
 #pragma unroll
-        for (int j = 0; j < R; ++j) acc[i][j] = 0.f;
+        for (int j = 0; j < R; ++j) two[i][j] = pair_of(0.f, 0.f);
+#pragma unroll 2
     for (int d = 0; d < dim; d += 4) {
-        float4 x[R], y[R];
+        Pair x[R][2], y[R][2];
 #pragma unroll
-        for (int i = 0; i < R; ++i) x[i] = *reinterpret_cast<const float4 *>(a + (ty * R + i) * (kDim + 4) + d);
+        for (int i = 0; i < R; ++i) load_pairs(a + (ty * R + i) * (kDim + 4) + d, x[i]);
 #pragma unroll
-        for (int j = 0; j < R; ++j) y[j] = *reinterpret_cast<const float4 *>(b + (tx + 16 * j) * (kDim + 4) + d);
+        for (int j = 0; j < R; ++j) load_pairs(b + (tx + 16 * j) * (kDim + 4) + d, y[j]);
 #pragma unroll
         for (int i = 0; i < R; ++i)
 #pragma unroll
-            for (int j = 0; j < R; ++j) {
-                acc[i][j] = fmaf(x[i].x, y[j].x, acc[i][j]);
-                acc[i][j] = fmaf(x[i].y, y[j].y, acc[i][j]);
-                acc[i][j] = fmaf(x[i].z, y[j].z, acc[i][j]);
-                acc[i][j] = fmaf(x[i].w, y[j].w, acc[i][j]);
-            }
+            for (int j = 0; j < R; ++j) two[i][j] = fma2(x[i][1], y[j][1], fma2(x[i][0], y[j][0], two[i][j]));
     }
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+            float even, odd;
+            split(two[i][j], even, odd);
+            acc[i][j] = even + odd;
+        }
 }
 
 // acc[i][c] += sum over n of w[ty * R + i][n] * x[n][(tx + 16 * c) * 4 ..]; w has rows of kRows + 4 floats
@@ -75,9 +92,15 @@ __device__ __forceinline__ void weigh_rows(const float *w, const float *x, float
         for (int u = 0; u < 4; ++u)
 #pragma unroll
             for (int c = 0; c < kDim / 64; ++c) {
-                const float4 y = *reinterpret_cast<const float4 *>(x + (n + u) * (kDim + 4) + (tx + 16 * c) * 4);
+                Pair y[2];
+                load_pairs(x + (n + u) * (kDim + 4) + (tx + 16 * c) * 4, y);
 #pragma unroll
-                for (int i = 0; i < R; ++i) vfma(acc[i][c], reinterpret_cast<const float *>(&p[i])[u], y);
+                for (int i = 0; i < R; ++i) {
+                    const float weight = reinterpret_cast<const float *>(&p[i])[u];
+                    Pair *to = reinterpret_cast<Pair *>(&acc[i][c]);
+                    to[0] = fma2(pair_of(weight, weight), y[0], to[0]);
+                    to[1] = fma2(pair_of(weight, weight), y[1], to[1]);
+                }
             }
     }
 }
@@ -129,16 +152,15 @@ __device__ __forceinline__ void softmax_tile(float (&s)[R][R], float (&m)[R], fl
 
 template <int kDim>
 constexpr int forward_shared() {
-    return 4 * (3 * tile_rows<kDim>() * (kDim + 4) + tile_rows<kDim>() * (tile_rows<kDim>() + 4));
+    return 4 * (2 * tile_rows<kDim>() * (kDim + 4) + tile_rows<kDim>() * (tile_rows<kDim>() + 4));
 }
 
 // One tile of a sequence's queries, one head.
 template <typename T, int kDim>
-__global__ void __launch_bounds__(kThreads) prompt_rows(Prompt p) {
+__global__ void __launch_bounds__(kThreads, 2) prompt_rows(Prompt p) {
     constexpr int kRows = tile_rows<kDim>(), R = kRows / 16;
     extern __shared__ float4 shared4[];
-    float *qs = reinterpret_cast<float *>(shared4), *ks = qs + kRows * (kDim + 4), *vs = ks + kRows * (kDim + 4),
-          *ws = vs + kRows * (kDim + 4);
+    float *qs = reinterpret_cast<float *>(shared4), *ks = qs + kRows * (kDim + 4), *vs = ks, *ws = ks + kRows * (kDim + 4);
     const Window &w = p.win;
     const int head = blockIdx.y, kv = head / (w.heads / w.kv_heads);
     const Tile t = find_tile(p.seqs.q_offsets, p.seqs.n_seq, p.seqs.q_rows, blockIdx.x, kRows);
@@ -164,10 +186,11 @@ __global__ void __launch_bounds__(kThreads) prompt_rows(Prompt p) {
         const int k0 = blocks.at(b) * kRows, n = min(kRows, keys.y - k0);
         __syncthreads();
         fetch_tile<T, kDim>(ks, row_of<T>(p.k, 0, keys.x + k0, kv), p.k.row, n, w.dim);
-        fetch_tile<T, kDim>(vs, row_of<T>(p.v, 0, keys.x + k0, kv), p.v.row, n, w.dim);
         __syncthreads();
         float s[R][R];
         dot_tile<kDim, R>(qs, ks, w.dim, s);
+        __syncthreads();
+        fetch_tile<T, kDim>(vs, row_of<T>(p.v, 0, keys.x + k0, kv), p.v.row, n, w.dim);
 #pragma unroll
         for (int i = 0; i < R; ++i)
 #pragma unroll
@@ -196,11 +219,10 @@ __global__ void __launch_bounds__(kThreads) prompt_rows(Prompt p) {
 
 // Queries of all requests that share a key head, row r = request r / group, head r % group of the group, against a part of the prefix.
 template <typename T, int kDim>
-__global__ void __launch_bounds__(kThreads) shared_rows(Cached c) {
+__global__ void __launch_bounds__(kThreads, 2) shared_rows(Cached c) {
     constexpr int kRows = tile_rows<kDim>(), R = kRows / 16;
     extern __shared__ float4 shared4[];
-    float *qs = reinterpret_cast<float *>(shared4), *ks = qs + kRows * (kDim + 4), *vs = ks + kRows * (kDim + 4),
-          *ws = vs + kRows * (kDim + 4);
+    float *qs = reinterpret_cast<float *>(shared4), *ks = qs + kRows * (kDim + 4), *vs = ks, *ws = ks + kRows * (kDim + 4);
     chain_begin();  // the requests' own keys are worked on beside the prefix
     const Window &w = c.win;
     const int kv = blockIdx.y, group = w.heads / w.kv_heads, split = blockIdx.z;
@@ -227,10 +249,11 @@ __global__ void __launch_bounds__(kThreads) shared_rows(Cached c) {
         const int k0 = b * kRows, n = min(kRows, c.prefix - k0);
         __syncthreads();
         fetch_tile<T, kDim>(ks, row_of<T>(c.pk, 0, k0, kv), c.pk.row, n, w.dim);
-        fetch_tile<T, kDim>(vs, row_of<T>(c.pv, 0, k0, kv), c.pv.row, n, w.dim);
         __syncthreads();
         float s[R][R];
         dot_tile<kDim, R>(qs, ks, w.dim, s);
+        __syncthreads();
+        fetch_tile<T, kDim>(vs, row_of<T>(c.pv, 0, k0, kv), c.pv.row, n, w.dim);
 #pragma unroll
         for (int i = 0; i < R; ++i)
 #pragma unroll

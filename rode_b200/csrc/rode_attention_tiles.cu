@@ -61,32 +61,6 @@ __device__ __forceinline__ void hide(uint32_t (&x)[n], const Range &r, uint32_t 
     }
 }
 
-// Two numbers in one 64-bit register: one instruction for both.
-struct Pair {
-    unsigned long long x;
-};
-__device__ __forceinline__ Pair pair_of(float a, float b) {
-    Pair r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r.x) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ void split(Pair p, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p.x)); }
-__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
-    Pair r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.x) : "l"(a.x), "l"(b.x), "l"(c.x));
-    return r;
-}
-__device__ __forceinline__ Pair add2(Pair a, Pair b) {
-    Pair r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.x) : "l"(a.x), "l"(b.x));
-    return r;
-}
-
-__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
-    Pair r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.x) : "l"(a.x), "l"(b.x));
-    return r;
-}
 __device__ __forceinline__ Pair load_pair(uint32_t shared) {
     Pair r;
     asm volatile("ld.shared.b64 %0, [%1];" : "=l"(r.x) : "r"(shared));
