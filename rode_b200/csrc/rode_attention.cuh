@@ -137,15 +137,18 @@ __device__ __forceinline__ int boundary(const int *offsets, int n_seq, int total
     return min(max(__ldg(offsets + e - 1), 0), total);
 }
 
+// By whole warps: 32 offsets are looked at at once.
 __device__ __forceinline__ Tile find_tile(const int *offsets, int n_seq, int total, int slot, int tile) {
     if (offsets == nullptr) return {0, 0, total, slot * tile};
     int lo = 0, hi = n_seq + 2;  // the answer is in [lo, hi)
     while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (boundary(offsets, n_seq, total, mid) / tile + mid <= slot)
-            lo = mid;
-        else
-            hi = mid;
+        const int step = (hi - lo + 31) / 32, e = lo + static_cast<int>(threadIdx.x % 32) * step;
+        const bool below = e < hi && boundary(offsets, n_seq, total, e) / tile + e <= slot;
+        // (offsets that are out of order may leave holes: the lanes up to the first one count)
+        const unsigned votes = __ballot_sync(0xffffffffu, below) | 1u;
+        const int n = votes == 0xffffffffu ? 32 : __ffs(~votes) - 1;
+        lo += (n - 1) * step;
+        hi = min(lo + step, hi);
     }
     const int begin = boundary(offsets, n_seq, total, lo);
     const int rows = max(boundary(offsets, n_seq, total, lo + 1) - begin, 0);

@@ -13,6 +13,7 @@
 // as 2^8, which costs no precision (the sum has the same factor), and the multiplication of O by 2^(old - new) is rare.
 // P is rounded to the operands' type (the products take 16-bit operands); the sum is that of the unrounded weights.
 #include <algorithm>
+#include <climits>
 #include <type_traits>
 
 #include "rode_attention.cuh"
@@ -149,8 +150,9 @@ __device__ __forceinline__ void gradients_in_place(uint32_t (&s)[64], const uint
     }
 }
 
-// What a CTA works on: two tiles of rows, the blocks of keys that any of them sees.
+// A piece of work: two tiles of rows of a key head, the blocks of keys that any of them sees.
 struct Work {
+    int kv, part;       // key head, part of the prefix
     long long row0;     // first query (of the packed operand, or first request)
     int n_queries;      // queries of this CTA that exist
     int pos0;           // position of the first one
@@ -182,38 +184,45 @@ __device__ __forceinline__ void give_registers() { asm volatile("setmaxnreg.dec.
 // kShared: rows are requests, keys a part of the prefix, results go to the parts; else prompts.
 template <typename T, int kDim, bool kShared>
 __global__ void __launch_bounds__(kTileThreads, 1)
-    forward_tiles(const __grid_constant__ TileMaps maps, const Prompt p, const Cached c) {
+    forward_tiles(const __grid_constant__ TileMaps maps, const Prompt p, const Cached c, int items) {
     constexpr int kPanels = kDim / 64, kStages = forward_stages<kDim>(), kTile = kPanels * kPanel;
     extern __shared__ char shared_raw[];
     const Window &w = kShared ? c.win : p.win;
-    const int group = w.heads / w.kv_heads, per_tile = kRows / group, kv = blockIdx.y;
+    const int group = w.heads / w.kv_heads, per_tile = kRows / group;
+    if constexpr (kShared) chain_begin();  // the requests' own keys are worked on beside the prefix
 
     Work wk;
-    if constexpr (kShared) {
-        chain_begin();  // the requests' own keys are worked on beside the prefix
-        wk.row0 = static_cast<long long>(blockIdx.x) * 2 * per_tile;
-        wk.n_queries = static_cast<int>(min(static_cast<long long>(2 * per_tile), c.batch - wk.row0));
-        wk.pos0 = 0;
-        wk.key0 = 0;
-        wk.keys = c.prefix;
-        const long long all = (c.prefix + kRows - 1) / kRows;
-        wk.n_sink = 0;
-        wk.first = static_cast<int>(all * blockIdx.z / c.prefix_parts);
-        wk.blocks = static_cast<int>(all * (blockIdx.z + 1) / c.prefix_parts) - wk.first;
-    } else {
-        const Tile t = find_tile(p.seqs.q_offsets, p.seqs.n_seq, p.seqs.q_rows, blockIdx.x, 2 * per_tile);
-        if (t.first < 0 || t.first >= t.rows || (t.seq < 0 && !p.clear)) return;
-        const int2 keys = t.seq < 0 ? make_int2(0, 0) : sequence_rows(p.seqs.k_offsets, p.seqs.k_rows, t.seq);
-        wk.row0 = static_cast<long long>(t.row0) + t.first;
-        wk.n_queries = min(2 * per_tile, t.rows - t.first);
-        wk.pos0 = t.first + keys.y - t.rows;
-        wk.key0 = keys.x;
-        wk.keys = keys.y;
-        const KeyBlocks b(wk.pos0, wk.pos0 + wk.n_queries, w.window, w.sinks, kRows);
-        wk.blocks = b.n;
-        wk.n_sink = b.n_sink;
-        wk.first = b.first;
-    }
+    // Item i: row tiles innermost by key heads, so that heads of the same positions run side by side.  False: nothing there.
+    const auto load_work = [&](int item) {
+        wk.kv = item % w.kv_heads;
+        const int slot = item / w.kv_heads;
+        if constexpr (kShared) {
+            wk.part = slot % c.prefix_parts;
+            wk.row0 = static_cast<long long>(slot / c.prefix_parts) * 2 * per_tile;
+            wk.n_queries = static_cast<int>(min(static_cast<long long>(2 * per_tile), c.batch - wk.row0));
+            wk.pos0 = 0;
+            wk.key0 = 0;
+            wk.keys = c.prefix;
+            const long long all = (c.prefix + kRows - 1) / kRows;
+            wk.n_sink = 0;
+            wk.first = static_cast<int>(all * wk.part / c.prefix_parts);
+            wk.blocks = static_cast<int>(all * (wk.part + 1) / c.prefix_parts) - wk.first;
+        } else {
+            const Tile t = find_tile(p.seqs.q_offsets, p.seqs.n_seq, p.seqs.q_rows, slot, 2 * per_tile);
+            if (t.first < 0 || t.first >= t.rows || (t.seq < 0 && !p.clear)) return false;
+            const int2 keys = t.seq < 0 ? make_int2(0, 0) : sequence_rows(p.seqs.k_offsets, p.seqs.k_rows, t.seq);
+            wk.row0 = static_cast<long long>(t.row0) + t.first;
+            wk.n_queries = min(2 * per_tile, t.rows - t.first);
+            wk.pos0 = t.first + keys.y - t.rows;
+            wk.key0 = keys.x;
+            wk.keys = keys.y;
+            const KeyBlocks b(wk.pos0, wk.pos0 + wk.n_queries, w.window, w.sinks, kRows);
+            wk.blocks = b.n;
+            wk.n_sink = b.n_sink;
+            wk.first = b.first;
+        }
+        return true;
+    };
     // Queries of tile t, and whether it sees any key of the block from k0 on.
     const auto queries_of = [&](int t) { return min(per_tile, wk.n_queries - t * per_tile); };
     const auto sees_block = [&](int t, int k0) {
@@ -226,15 +235,17 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 
     const uint32_t base = uniform((shared_address(shared_raw) + 1023) & ~1023u);
     const uint32_t qs = base, ks = qs + 2 * kTile, vs = ks + kStages * kTile, bars = vs + kStages * kTile;
-    const uint32_t q_full = bars, v_raw = bars + 8, s_full = bars + 16, o_done = bars + 32, p_full = bars + 48, turn = bars + 80, k_full = bars + 96,
+    const uint32_t q_full = bars, v_raw = bars + 8, q_empty = bars + 96, s_full = bars + 16, o_done = bars + 32, p_full = bars + 48, turn = bars + 80, k_full = bars + 104,
                    k_empty = k_full + 8 * kStages, v_full = k_empty + 8 * kStages, v_empty = v_full + 8 * kStages,
                    tmem_at = v_empty + 8 * kStages;
     const int warp = uniform(threadIdx.x / 32), lane = threadIdx.x % 32;
+    if (warp == 9 && lane < 3) prefetch_map(lane == 0 ? &maps.q : lane == 1 ? &maps.k : &maps.v);
     if (warp == 8) {
         tmem_alloc(tmem_at, 512);
         if (lane == 0) {
             barrier_init(q_full, 1);
             barrier_init(v_raw, 1);
+            barrier_init(q_empty, 2);
             barrier_init(turn, 128);
             barrier_init(turn + 8, 128);
             for (int t = 0; t < 2; ++t) {
@@ -264,36 +275,41 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     if (warp >= 8) give_registers();
     if (warp == 9) {
         // copies
-        if (lane == 0 && wk.blocks > 0) {
-            const int tiles = queries_of(1) > 0 ? 2 : 1;
-            barrier_expect(q_full, tiles * kPanels * per_tile * group * 128);
-            for (int t = 0; t < tiles; ++t)
-                for (int x = 0; x < kPanels; ++x)
-                    copy_box(qs + t * kTile + x * kPanel, &maps.q, x * 64, kv * group, static_cast<int>(wk.row0) + t * per_tile, q_full);
-        }
-        int raw = 0;
-        for (int i = 0; i < wk.blocks && ok; ++i) {
-            const int st = i % kStages, k0 = wk.key_of(i), have = wk.keys - k0;
-            const uint32_t free = (i / kStages & 1) ^ 1;
-            const int y = static_cast<int>(wk.key0) + k0;
-            ok = barrier_wait(k_empty + 8 * st, free);
+        int raw = 0, loaded = 0, filled = 0;  // raw blocks, items, blocks so far
+        for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
+            if (!load_work(item) || wk.blocks == 0) continue;
+            ok = barrier_wait(q_empty, (loaded++ & 1) ^ 1);
             if (ok && lane == 0) {
-                barrier_expect(k_full + 8 * st, kTile);
-                for (int x = 0; x < kPanels; ++x) copy_box(ks + st * kTile + x * kPanel, &maps.k, x * 64, kv, y, k_full + 8 * st);
-            }
-            ok = ok && barrier_wait(v_empty + 8 * st, free);
-            if (!ok) break;
-            const uint32_t bar = have < kRows ? v_raw : v_full + 8 * st;
-            if (lane == 0) {
-                barrier_expect(bar, kTile);
-                for (int x = 0; x < kPanels; ++x) copy_box(vs + st * kTile + x * kPanel, &maps.v, x * 64, kv, y, bar);
+                const int tiles = queries_of(1) > 0 ? 2 : 1;
+                barrier_expect(q_full, tiles * kPanels * per_tile * group * 128);
+                for (int t = 0; t < tiles; ++t)
+                    for (int x = 0; x < kPanels; ++x)
+                        copy_box(qs + t * kTile + x * kPanel, &maps.q, x * 64, wk.kv * group, static_cast<int>(wk.row0) + t * per_tile, q_full);
             }
             __syncwarp();
-            if (have < kRows) {
-                ok = barrier_wait(v_raw, raw & 1);
-                ++raw;
-                clear_rows(vs + st * kTile, kPanels, have);
-                if (lane == 0) barrier_arrive(v_full + 8 * st);
+            for (int i = 0; i < wk.blocks && ok; ++i, ++filled) {
+                const int st = filled % kStages, k0 = wk.key_of(i), have = wk.keys - k0;
+                const uint32_t free = (filled / kStages & 1) ^ 1;
+                const int y = static_cast<int>(wk.key0) + k0;
+                ok = barrier_wait(k_empty + 8 * st, free);
+                if (ok && lane == 0) {
+                    barrier_expect(k_full + 8 * st, kTile);
+                    for (int x = 0; x < kPanels; ++x) copy_box(ks + st * kTile + x * kPanel, &maps.k, x * 64, wk.kv, y, k_full + 8 * st);
+                }
+                ok = ok && barrier_wait(v_empty + 8 * st, free);
+                if (!ok) break;
+                const uint32_t bar = have < kRows ? v_raw : v_full + 8 * st;
+                if (lane == 0) {
+                    barrier_expect(bar, kTile);
+                    for (int x = 0; x < kPanels; ++x) copy_box(vs + st * kTile + x * kPanel, &maps.v, x * 64, wk.kv, y, bar);
+                }
+                __syncwarp();
+                if (have < kRows) {
+                    ok = barrier_wait(v_raw, raw & 1);
+                    ++raw;
+                    clear_rows(vs + st * kTile, kPanels, have);
+                    if (lane == 0) barrier_arrive(v_full + 8 * st);
+                }
             }
         }
     } else if (warp == 8 || warp == 10) {
@@ -303,9 +319,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         const uint32_t one = elect_one();
         const int steps = (w.dim + 15) / 16;
         const uint32_t s_at = tmem + t * kRows, o_at = tmem + 256 + t * kDim;
-        const auto issue_scores = [&](int i) {  // of block i, and its keys' stage is done with
-            const int st = i % kStages;
-            ok = barrier_wait(k_full + 8 * st, i / kStages & 1);
+        int loaded = 0, filled = 0, issued = 0;  // items, blocks, blocks of this tile so far
+        const auto issue_scores = [&](int i) {   // of block i of the item, and its keys' stage is done with
+            const int st = (filled + i) % kStages;
+            ok = barrier_wait(k_full + 8 * st, (filled + i) / kStages & 1);
             if (!ok) return;
             if (sees_block(t, wk.key_of(i))) {
                 tmem_fence_after();
@@ -321,39 +338,43 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             } else if (one) {
                 barrier_arrive(k_empty + 8 * st);
             }
+            if (i + 1 == wk.blocks) products_arrive(one, q_empty);  // the next item's queries may come
             __syncwarp();
         };
-        int issued = 0;
-        if (wk.blocks > 0) {
-            ok = barrier_wait(q_full, 0);
+        for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
+            if (!load_work(item) || wk.blocks == 0) continue;
+            ok = barrier_wait(q_full, loaded++ & 1);
             if (ok) issue_scores(0);
-        }
-        for (int i = 0; i < wk.blocks && ok; ++i) {
-            const int st = i % kStages;
-            ok = barrier_wait(v_full + 8 * st, i / kStages & 1);
-            if (!ok) break;
-            if (sees_block(t, wk.key_of(i))) {
-                const uint64_t b = tile_descriptor(vs + st * kTile, kPanel);
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    ok = ok && barrier_wait(p_full + 16 * t + 8 * half, issued & 1);
-                    tmem_fence_after();
-                    if (ok)
-#pragma unroll
-                        for (int s = 4 * half; s < 4 * half + 4; ++s)
-                            product_from_tmem(one, o_at, s_at + s * 8, b + s * 128, values, issued > 0 || s > 0);
-                }
+            bool add = false;
+            for (int i = 0; i < wk.blocks && ok; ++i) {
+                const int st = (filled + i) % kStages;
+                ok = barrier_wait(v_full + 8 * st, (filled + i) / kStages & 1);
                 if (!ok) break;
-                products_arrive(one, o_done + 8 * t);
-                products_arrive(one, v_empty + 8 * st);
-                // the next scores go where the weights were
-                ok = barrier_wait(o_done + 8 * t, issued & 1);
-                ++issued;
-            } else if (one) {
-                barrier_arrive(v_empty + 8 * st);
+                if (sees_block(t, wk.key_of(i))) {
+                    const uint64_t b = tile_descriptor(vs + st * kTile, kPanel);
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        ok = ok && barrier_wait(p_full + 16 * t + 8 * half, issued & 1);
+                        tmem_fence_after();
+                        if (ok)
+#pragma unroll
+                            for (int s = 4 * half; s < 4 * half + 4; ++s)
+                                product_from_tmem(one, o_at, s_at + s * 8, b + s * 128, values, add || s > 0);
+                    }
+                    if (!ok) break;
+                    add = true;
+                    products_arrive(one, o_done + 8 * t);
+                    products_arrive(one, v_empty + 8 * st);
+                    // the next scores go where the weights were
+                    ok = barrier_wait(o_done + 8 * t, issued & 1);
+                    ++issued;
+                } else if (one) {
+                    barrier_arrive(v_empty + 8 * st);
+                }
+                __syncwarp();
+                if (ok && i + 1 < wk.blocks) issue_scores(i + 1);
             }
-            __syncwarp();
-            if (ok && i + 1 < wk.blocks) issue_scores(i + 1);
+            filled += wk.blocks;
         }
     } else if (warp < 8) {
         // softmax: one row per thread
@@ -361,142 +382,148 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         const int t = warp / 4, r = threadIdx.x % 128;
         const uint32_t lanes = static_cast<uint32_t>(warp % 4 * 32) << 16;
         const uint32_t s_at = tmem + lanes + t * kRows, o_at = tmem + lanes + 256 + t * kDim;
-        const int n = queries_of(t), query = r / group, head = kv * group + r % group;
-        const bool mine = query < n;
-        const int a = wk.pos0 + t * per_tile, pos = a + query;
+        const int query = r / group;
         const float s2 = w.scale * kLog2e;
-        float m = -INFINITY, l = 0.f;
-        int done = 0;
-        // The tiles' exponentials take turns: side by side they would take twice as long and then wait for the products side by side
-        // (blocks of both tiles in 3250 clocks instead of 3800).
-        const bool turns = queries_of(1) > 0;
-        for (int i = 0; i < wk.blocks; ++i) {
-            const int k0 = wk.key_of(i);
-            if (!sees_block(t, k0)) {
-                if (turns) {
-                    ok = barrier_wait(turn + 8 * t, (i + t + 1) & 1);
-                    if (!ok) break;
-                    barrier_arrive(turn + 8 * (t ^ 1));
-                }
-                continue;
-            }
-            ok = barrier_wait(s_full + 8 * t, done & 1);
-            if (!ok) break;
-            tmem_fence_after();
-            uint32_t s[128];
-            tmem_load32<0>(s_at, s);
-            tmem_load32<32>(s_at + 32, s);
-            tmem_load32<64>(s_at + 64, s);
-            tmem_load32<96>(s_at + 96, s);
-            tmem_wait_load32<0>(s);
-            tmem_wait_load32<32>(s);
-            tmem_wait_load32<64>(s);
-            tmem_wait_load32<96>(s);
-            bool whole;
-            if constexpr (kShared)
-                whole = k0 + kRows <= wk.keys;
-            else
-                whole = k0 + kRows - 1 <= a && (a + n - 1 - k0 < w.window || k0 + kRows <= w.sinks);
-            if (!whole) {
-                if constexpr (kShared)
-                    hide(s, {0, wk.keys - k0, 0}, 0xff800000u);  // -infinity
-                else
-                    hide(s, {pos - w.window + 1 - k0, pos + 1 - k0, w.sinks - k0}, 0xff800000u);
-            }
-            float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-            for (int j = 0; j < 128; j += 2)
-                top[j / 2 % 4] = fmaxf(top[j / 2 % 4], fmaxf(__uint_as_float(s[j]), __uint_as_float(s[j + 1])));
-            const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-            const bool grows = (high - m) * s2 > kLazy;
-            if (__any_sync(0xffffffffu, grows)) {
-                const float next = grows ? high : m;
-                const float keep = grows ? exp2f((m - next) * s2) : 1.f;
-                m = next;
-                l *= keep;
-                if (done > 0) {
-#pragma unroll
-                    for (int x = 0; x < kDim; x += 32) {
-                        uint32_t o[32];
-                        tmem_load32<0>(o_at + x, o);
-                        tmem_wait_load32<0>(o);
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * keep);
-                        tmem_store32<0>(o_at + x, o);
+        int seen = 0, turn_of = 0;  // blocks of this tile, turns so far
+        for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
+            if (!load_work(item)) continue;
+            const int n = queries_of(t), head = wk.kv * group + r % group;
+            const bool mine = query < n;
+            const int a = wk.pos0 + t * per_tile, pos = a + query;
+            float m = -INFINITY, l = 0.f;
+            int done = 0;
+            // The tiles' exponentials take turns: side by side they would take twice as long and then wait for the products side by side
+            // (blocks of both tiles in 3250 clocks instead of 3800).
+            const bool turns = queries_of(1) > 0;
+            for (int i = 0; i < wk.blocks; ++i) {
+                const int k0 = wk.key_of(i);
+                if (!sees_block(t, k0)) {
+                    if (turns) {
+                        ok = barrier_wait(turn + 8 * t, (turn_of++ + t + 1) & 1);
+                        if (!ok) break;
+                        barrier_arrive(turn + 8 * (t ^ 1));
                     }
+                    continue;
                 }
-            }
-            const float off = m == -INFINITY ? 0.f : -m * s2;
-            if (turns) {
-                ok = barrier_wait(turn + 8 * t, (i + t + 1) & 1);
+                ok = barrier_wait(s_full + 8 * t, seen & 1);
                 if (!ok) break;
-            }
-            // the first half's products run during the second half's exponentials
-            Pair sum = pair_of(0.f, 0.f);
-            if (whole)
-                weights_of<T, 0, kByFma>(s, s2, off, sum);
-            else
-                weights_of<T, 0, 0>(s, s2, off, sum);
-            tmem_store32<0>(s_at, s);
-            tmem_wait_store();
-            tmem_fence_before();
-            barrier_arrive(p_full + 16 * t);
-            if (whole)
-                weights_of<T, 64, kByFma>(s, s2, off, sum);
-            else
-                weights_of<T, 64, 0>(s, s2, off, sum);
-            tmem_store32<32>(s_at + 32, s);
-            tmem_wait_store();
-            tmem_fence_before();
-            barrier_arrive(p_full + 16 * t + 8);
-            if (turns) barrier_arrive(turn + 8 * (t ^ 1));
-            float even, odd;
-            split(sum, even, odd);
-            l += even + odd;
-            ++done;
-        }
-        if (ok && done > 0) {
-            ok = barrier_wait(o_done + 8 * t, (done - 1) & 1);
-            tmem_fence_after();
-        }
-        const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-        const float lse2 = m == -INFINITY ? -INFINITY : m * s2 + log2f(l);
-        if (kShared) {
-            const long long at = (blockIdx.z * static_cast<long long>(c.batch) + wk.row0 + t * per_tile + query) * w.heads + head;
-            if (mine) c.prefix_lse[at] = lse2;
+                tmem_fence_after();
+                uint32_t s[128];
+                tmem_load32<0>(s_at, s);
+                tmem_load32<32>(s_at + 32, s);
+                tmem_load32<64>(s_at + 64, s);
+                tmem_load32<96>(s_at + 96, s);
+                tmem_wait_load32<0>(s);
+                tmem_wait_load32<32>(s);
+                tmem_wait_load32<64>(s);
+                tmem_wait_load32<96>(s);
+                bool whole;
+                if constexpr (kShared)
+                    whole = k0 + kRows <= wk.keys;
+                else
+                    whole = k0 + kRows - 1 <= a && (a + n - 1 - k0 < w.window || k0 + kRows <= w.sinks);
+                if (!whole) {
+                    if constexpr (kShared)
+                        hide(s, {0, wk.keys - k0, 0}, 0xff800000u);  // -infinity
+                    else
+                        hide(s, {pos - w.window + 1 - k0, pos + 1 - k0, w.sinks - k0}, 0xff800000u);
+                }
+                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int x = 0; x < kDim; x += 32) {
-                uint32_t o[32];
-                tmem_load32<0>(o_at + x, o);
-                tmem_wait_load32<0>(o);
-#pragma unroll
-                for (int j = 0; j < 32; j += 4)
-                    if (mine && x + j < w.dim)
-                        store4(c.prefix_out + at * w.dim + x + j,
-                               done > 0 ? make_float4(__uint_as_float(o[j]) * inv, __uint_as_float(o[j + 1]) * inv,
-                                                      __uint_as_float(o[j + 2]) * inv, __uint_as_float(o[j + 3]) * inv)
-                                        : make_float4(0.f, 0.f, 0.f, 0.f));
-            }
-        } else {
-            const long long row = wk.row0 + t * per_tile + query;
-            if (mine && p.lse != nullptr)
-                p.lse[static_cast<long long>(head) * p.seqs.q_rows + row] = lse2 == -INFINITY ? -INFINITY : lse2 * kLn2;
-            T *out = static_cast<T *>(p.out) + (row * w.heads + head) * w.dim;
-#pragma unroll
-            for (int x = 0; x < kDim; x += 32) {
-                uint32_t o[32];
-                tmem_load32<0>(o_at + x, o);
-                tmem_wait_load32<0>(o);
-#pragma unroll
-                for (int j = 0; j < 32; j += 8) {
-                    uint4 y = make_uint4(0, 0, 0, 0);
+                for (int j = 0; j < 128; j += 2)
+                    top[j / 2 % 4] = fmaxf(top[j / 2 % 4], fmaxf(__uint_as_float(s[j]), __uint_as_float(s[j + 1])));
+                const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+                const bool grows = (high - m) * s2 > kLazy;
+                if (__any_sync(0xffffffffu, grows)) {
+                    const float next = grows ? high : m;
+                    const float keep = grows ? exp2f((m - next) * s2) : 1.f;
+                    m = next;
+                    l *= keep;
                     if (done > 0) {
-                        y.x = pack2<T>(__uint_as_float(o[j]) * inv, __uint_as_float(o[j + 1]) * inv);
-                        y.y = pack2<T>(__uint_as_float(o[j + 2]) * inv, __uint_as_float(o[j + 3]) * inv);
-                        y.z = pack2<T>(__uint_as_float(o[j + 4]) * inv, __uint_as_float(o[j + 5]) * inv);
-                        y.w = pack2<T>(__uint_as_float(o[j + 6]) * inv, __uint_as_float(o[j + 7]) * inv);
+#pragma unroll
+                        for (int x = 0; x < kDim; x += 32) {
+                            uint32_t o[32];
+                            tmem_load32<0>(o_at + x, o);
+                            tmem_wait_load32<0>(o);
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * keep);
+                            tmem_store32<0>(o_at + x, o);
+                        }
                     }
-                    if (mine && x + j < w.dim) *reinterpret_cast<uint4 *>(out + x + j) = y;
+                }
+                const float off = m == -INFINITY ? 0.f : -m * s2;
+                if (turns) {
+                    ok = barrier_wait(turn + 8 * t, (turn_of++ + t + 1) & 1);
+                    if (!ok) break;
+                }
+                // the first half's products run during the second half's exponentials
+                Pair sum = pair_of(0.f, 0.f);
+                if (whole)
+                    weights_of<T, 0, kByFma>(s, s2, off, sum);
+                else
+                    weights_of<T, 0, 0>(s, s2, off, sum);
+                tmem_store32<0>(s_at, s);
+                tmem_wait_store();
+                tmem_fence_before();
+                barrier_arrive(p_full + 16 * t);
+                if (whole)
+                    weights_of<T, 64, kByFma>(s, s2, off, sum);
+                else
+                    weights_of<T, 64, 0>(s, s2, off, sum);
+                tmem_store32<32>(s_at + 32, s);
+                tmem_wait_store();
+                tmem_fence_before();
+                barrier_arrive(p_full + 16 * t + 8);
+                if (turns) barrier_arrive(turn + 8 * (t ^ 1));
+                float even, odd;
+                split(sum, even, odd);
+                l += even + odd;
+                ++done;
+                ++seen;
+            }
+            if (ok && done > 0) {
+                ok = barrier_wait(o_done + 8 * t, (seen - 1) & 1);
+                tmem_fence_after();
+            }
+            const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+            const float lse2 = m == -INFINITY ? -INFINITY : m * s2 + log2f(l);
+            if (kShared) {
+                const long long at = (wk.part * static_cast<long long>(c.batch) + wk.row0 + t * per_tile + query) * w.heads + head;
+                if (mine) c.prefix_lse[at] = lse2;
+#pragma unroll
+                for (int x = 0; x < kDim; x += 32) {
+                    uint32_t o[32];
+                    tmem_load32<0>(o_at + x, o);
+                    tmem_wait_load32<0>(o);
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4)
+                        if (mine && x + j < w.dim)
+                            store4(c.prefix_out + at * w.dim + x + j,
+                                   done > 0 ? make_float4(__uint_as_float(o[j]) * inv, __uint_as_float(o[j + 1]) * inv,
+                                                          __uint_as_float(o[j + 2]) * inv, __uint_as_float(o[j + 3]) * inv)
+                                            : make_float4(0.f, 0.f, 0.f, 0.f));
+                }
+            } else {
+                const long long row = wk.row0 + t * per_tile + query;
+                if (mine && p.lse != nullptr)
+                    p.lse[static_cast<long long>(head) * p.seqs.q_rows + row] = lse2 == -INFINITY ? -INFINITY : lse2 * kLn2;
+                T *out = static_cast<T *>(p.out) + (row * w.heads + head) * w.dim;
+#pragma unroll
+                for (int x = 0; x < kDim; x += 32) {
+                    uint32_t o[32];
+                    tmem_load32<0>(o_at + x, o);
+                    tmem_wait_load32<0>(o);
+#pragma unroll
+                    for (int j = 0; j < 32; j += 8) {
+                        uint4 y = make_uint4(0, 0, 0, 0);
+                        if (done > 0) {
+                            y.x = pack2<T>(__uint_as_float(o[j]) * inv, __uint_as_float(o[j + 1]) * inv);
+                            y.y = pack2<T>(__uint_as_float(o[j + 2]) * inv, __uint_as_float(o[j + 3]) * inv);
+                            y.z = pack2<T>(__uint_as_float(o[j + 4]) * inv, __uint_as_float(o[j + 5]) * inv);
+                            y.w = pack2<T>(__uint_as_float(o[j + 6]) * inv, __uint_as_float(o[j + 7]) * inv);
+                        }
+                        if (mine && x + j < w.dim) *reinterpret_cast<uint4 *>(out + x + j) = y;
+                    }
                 }
             }
         }
@@ -523,33 +550,49 @@ constexpr int backward_stages() {
 }
 template <int kDim>
 constexpr int backward_bytes() {
-    return 1024 + kDim / 64 * kPanel * (2 + 2 * backward_stages<kDim>()) + backward_stages<kDim>() * 2 * kRows * 4 + 512 + kRows * 4;
+    return 1024 + kDim / 64 * kPanel * (2 + 2 * backward_stages<kDim>()) + backward_stages<kDim>() * 2 * kRows * 4 + 512;
 }
 
 struct GradientMaps {
     CUtensorMap q, dout, k, v;
 };
 
-// delta = do . o of the rows of a tile (kRows of them, row r = query r / group, head r % group) by eight warps, a lane per 16 bytes, so that a warp
-// reads two or four rows at once.
+// delta = do . o of all rows, a lane per 16 bytes.  (By two spare warps of the kernel below it took as long as three blocks of keys, more than short windows
+// have; here 41 us of train_long's 2400.)
 template <typename T, int kDim>
-__device__ __forceinline__ void row_deltas(const Prompt &p, long long row0, int head0, int group, int n, uint32_t deltas) {
+__global__ void __launch_bounds__(256) row_deltas(const Prompt p) {
     constexpr int kLanes = kDim / 8;
-    const int dim = p.win.dim, piece = threadIdx.x % kLanes, d = piece * 8;
+    chain_begin();
+    const int dim = p.win.dim, heads = p.win.heads, d = threadIdx.x % kLanes * 8;
+    const long long rows = static_cast<long long>(p.seqs.q_rows) * heads, i = blockIdx.x * (256ll / kLanes) + threadIdx.x / kLanes;
+    const long long row = i / heads;
+    const int head = static_cast<int>(i % heads);
+    float sum = 0.f;
+    if (i < rows && d < dim) {
+        const uint4 x = __ldg(reinterpret_cast<const uint4 *>(row_of<T>(p.dout, 0, row, head) + d));
+        const uint4 y = __ldg(reinterpret_cast<const uint4 *>(static_cast<const T *>(p.out) + i * dim + d));
+        const T *s = reinterpret_cast<const T *>(&x), *t = reinterpret_cast<const T *>(&y);
 #pragma unroll
-    for (int r = threadIdx.x / kLanes; r < kRows; r += 256 / kLanes) {
-        const int query = r / group, head = head0 + r % group;
-        float sum = 0.f;
-        if (query < n && d < dim) {
-            const uint4 x = __ldg(reinterpret_cast<const uint4 *>(row_of<T>(p.dout, 0, row0 + query, head) + d));
-            const uint4 y = __ldg(reinterpret_cast<const uint4 *>(static_cast<const T *>(p.out) + ((row0 + query) * p.win.heads + head) * dim + d));
-            const T *s = reinterpret_cast<const T *>(&x), *t = reinterpret_cast<const T *>(&y);
+        for (int u = 0; u < 8; ++u) sum = fmaf(to_float(s[u]), to_float(t[u]), sum);
+    }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sum = fmaf(to_float(s[i]), to_float(t[i]), sum);
+    for (int o = kLanes / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (i < rows && threadIdx.x % kLanes == 0) p.delta[head * static_cast<long long>(p.seqs.q_rows) + row] = sum;
+}
+
+// -lse in base 2 and -delta of the rows of a tile (row r = query r / group, head r % group) to shared memory, by one warp.
+__device__ __forceinline__ void fetch_rows(const Prompt &p, const float *deltas, long long row0, int head0, int group, int n, uint32_t to) {
+#pragma unroll
+    for (int r = threadIdx.x % 32; r < kRows; r += 32) {
+        float lse = 0.f, delta = 0.f;
+        if (r / group < n) {
+            const long long at = static_cast<long long>(head0 + r % group) * p.seqs.q_rows + row0 + r / group;
+            lse = __ldg(p.lse + at);
+            lse = lse == -INFINITY ? 0.f : -lse * kLog2e;
+            delta = __ldcg(deltas + at);
         }
-#pragma unroll
-        for (int o = kLanes / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (piece == 0) asm volatile("st.shared.f32 [%0], %1;" ::"r"(deltas + 4 * r), "f"(sum) : "memory");
+        asm volatile("st.shared.f32 [%0], %1;" ::"r"(to + r * 4), "f"(lse) : "memory");
+        asm volatile("st.shared.f32 [%0], %1;" ::"r"(to + (kRows + r) * 4), "f"(-delta) : "memory");
     }
 }
 
@@ -572,38 +615,60 @@ __device__ __forceinline__ void store_columns(T *row, uint32_t at, int x, int di
     }
 }
 
-// dQ of one tile of rows, and delta.  Tensor memory: S twice (dS over it), dP, dQ.  The products of block i + 1 that need no dS (S, then
-// dP) run while the threads work on block i.
+// dQ, a tile of rows at a time.  Tensor memory: S twice (dS over it), dP, dQ.  The products of block i + 1 that need no dS (S, then
+// dP) run while the threads work on block i.  Persistent: the next tile's rows, sums and first products come while this tile's dQ is written (tiles of 18
+// blocks of 2000 clocks took another 20000 each as CTAs of their own).
 template <typename T, int kDim>
-__global__ void __launch_bounds__(kTileThreads, 1) query_gradient_tiles(const __grid_constant__ GradientMaps maps, const Prompt p) {
+__global__ void __launch_bounds__(kTileThreads, 1)
+    query_gradient_tiles(const __grid_constant__ GradientMaps maps, const Prompt p, int items) {
     constexpr int kPanels = kDim / 64, kStages = backward_stages<kDim>(), kTile = kPanels * kPanel;
     extern __shared__ char shared_raw[];
     const Window &w = p.win;
-    const int group = w.heads / w.kv_heads, per_tile = kRows / group, kv = blockIdx.y;
-    const Tile t = find_tile(p.seqs.q_offsets, p.seqs.n_seq, p.seqs.q_rows, blockIdx.x, per_tile);
-    if (t.first < 0 || t.first >= t.rows || (t.seq < 0 && !p.clear)) return;
-    const int2 keys = t.seq < 0 ? make_int2(0, 0) : sequence_rows(p.seqs.k_offsets, p.seqs.k_rows, t.seq);
-    const long long row0 = static_cast<long long>(t.row0) + t.first;
-    const int n = min(per_tile, t.rows - t.first), pos0 = t.first + keys.y - t.rows;
-    const KeyBlocks blocks(pos0, pos0 + n, w.window, w.sinks, kRows);
+    const int group = w.heads / w.kv_heads, per_tile = kRows / group;
+    struct {
+        int kv, n, pos0, keys, key0;
+        long long row0;
+    } wk;
+    KeyBlocks blocks(0, 0, 1, 0, kRows);
+    // Item i: tiles by key heads, so that heads of the same positions run side by side.  False: nothing there.
+    const auto load_work = [&](int item) {
+        wk.kv = item % w.kv_heads;
+        const Tile t = find_tile(p.seqs.q_offsets, p.seqs.n_seq, p.seqs.q_rows, item / w.kv_heads, per_tile);
+        if (t.first < 0 || t.first >= t.rows || (t.seq < 0 && !p.clear)) return false;
+        const int2 keys = t.seq < 0 ? make_int2(0, 0) : sequence_rows(p.seqs.k_offsets, p.seqs.k_rows, t.seq);
+        wk.row0 = static_cast<long long>(t.row0) + t.first;
+        wk.n = min(per_tile, t.rows - t.first);
+        wk.pos0 = t.first + keys.y - t.rows;
+        wk.key0 = keys.x;
+        wk.keys = keys.y;
+        blocks = KeyBlocks(wk.pos0, wk.pos0 + wk.n, w.window, w.sinks, kRows);
+        return true;
+    };
 
     const uint32_t base = uniform((shared_address(shared_raw) + 1023) & ~1023u);
-    const uint32_t qs = base, gs = qs + kTile, ks = gs + kTile, vs = ks + kStages * kTile, bars = vs + kStages * kTile;
-    const uint32_t q_full = bars, k_raw = bars + 8, s_full = bars + 16, dp_full = bars + 32, ds_full = bars + 40, dq_done = bars + 56,
-                   k_full = bars + 64, k_empty = k_full + 8 * kStages, v_full = k_empty + 8 * kStages, v_empty = v_full + 8 * kStages,
+    const uint32_t qs = base, gs = qs + kTile, ks = gs + kTile, vs = ks + kStages * kTile, rows_at = vs + kStages * kTile,
+                   bars = rows_at + kStages * 2 * kRows * 4;
+    const uint32_t q_full = bars, q_empty = bars + 8, k_raw = bars + 16, dp_full = bars + 24, dq_done = bars + 32, dq_free = bars + 40,
+                   s_full = bars + 48, ds_full = bars + 64, rows_full = bars + 80, rows_empty = bars + 96, k_full = bars + 112,
+                   k_empty = k_full + 8 * kStages, v_full = k_empty + 8 * kStages, v_empty = v_full + 8 * kStages,
                    tmem_at = v_empty + 8 * kStages;
     const int warp = uniform(threadIdx.x / 32), lane = threadIdx.x % 32;
+    if (warp == 9 && lane < 4) prefetch_map(lane == 0 ? &maps.q : lane == 1 ? &maps.dout : lane == 2 ? &maps.k : &maps.v);
     if (warp == 8) {
         tmem_alloc(tmem_at, 512);
         if (lane == 0) {
             barrier_init(q_full, 1);
+            barrier_init(q_empty, 1);
             barrier_init(k_raw, 1);
-            barrier_init(s_full, 1);
-            barrier_init(s_full + 8, 1);
             barrier_init(dp_full, 1);
-            barrier_init(ds_full, 256);
-            barrier_init(ds_full + 8, 256);
             barrier_init(dq_done, 1);
+            barrier_init(dq_free, 256);
+            for (int i = 0; i < 2; ++i) {
+                barrier_init(s_full + 8 * i, 1);
+                barrier_init(ds_full + 8 * i, 256);
+                barrier_init(rows_full + 8 * i, 32);
+                barrier_init(rows_empty + 8 * i, 256);
+            }
             for (int i = 0; i < kStages; ++i) {
                 barrier_init(k_full + 8 * i, 1);
                 barrier_init(k_empty + 8 * i, 1);
@@ -620,40 +685,45 @@ __global__ void __launch_bounds__(kTileThreads, 1) query_gradient_tiles(const __
     uint32_t tmem;
     asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem) : "r"(tmem_at));
     tmem = uniform(tmem);
-    const uint32_t dp_at = tmem + 256, dq_at = tmem + 384, deltas = bars + 512;
+    const uint32_t dp_at = tmem + 256, dq_at = tmem + 384;
     bool ok = true;
 
     if (warp >= 8) give_registers();
     if (warp == 9) {
-        if (lane == 0 && blocks.n > 0) {
-            barrier_expect(q_full, 2 * kPanels * per_tile * group * 128);
-            for (int x = 0; x < kPanels; ++x) {
-                copy_box(qs + x * kPanel, &maps.q, x * 64, kv * group, static_cast<int>(row0), q_full);
-                copy_box(gs + x * kPanel, &maps.dout, x * 64, kv * group, static_cast<int>(row0), q_full);
-            }
-        }
-        int raw = 0;
-        for (int i = 0; i < blocks.n && ok; ++i) {
-            const int st = i % kStages, k0 = blocks.at(i) * kRows, have = keys.y - k0, y = keys.x + k0;
-            const uint32_t free = (i / kStages & 1) ^ 1;
-            ok = barrier_wait(k_empty + 8 * st, free);
-            const uint32_t bar = have < kRows ? k_raw : k_full + 8 * st;
+        int raw = 0, loaded = 0, filled = 0;  // raw blocks, items, blocks so far
+        for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
+            if (!load_work(item) || blocks.n == 0) continue;
+            ok = barrier_wait(q_empty, (loaded++ & 1) ^ 1);
             if (ok && lane == 0) {
-                barrier_expect(bar, kTile);
-                for (int x = 0; x < kPanels; ++x) copy_box(ks + st * kTile + x * kPanel, &maps.k, x * 64, kv, y, bar);
+                barrier_expect(q_full, 2 * kPanels * per_tile * group * 128);
+                for (int x = 0; x < kPanels; ++x) {
+                    copy_box(qs + x * kPanel, &maps.q, x * 64, wk.kv * group, static_cast<int>(wk.row0), q_full);
+                    copy_box(gs + x * kPanel, &maps.dout, x * 64, wk.kv * group, static_cast<int>(wk.row0), q_full);
+                }
             }
             __syncwarp();
-            if (ok && have < kRows) {
-                ok = barrier_wait(k_raw, raw++ & 1);
-                clear_rows(ks + st * kTile, kPanels, have);
-                if (lane == 0) barrier_arrive(k_full + 8 * st);
+            for (int i = 0; i < blocks.n && ok; ++i, ++filled) {
+                const int st = filled % kStages, k0 = blocks.at(i) * kRows, have = wk.keys - k0, y = wk.key0 + k0;
+                const uint32_t free = (filled / kStages & 1) ^ 1;
+                ok = barrier_wait(k_empty + 8 * st, free);
+                const uint32_t bar = have < kRows ? k_raw : k_full + 8 * st;
+                if (ok && lane == 0) {
+                    barrier_expect(bar, kTile);
+                    for (int x = 0; x < kPanels; ++x) copy_box(ks + st * kTile + x * kPanel, &maps.k, x * 64, wk.kv, y, bar);
+                }
+                __syncwarp();
+                if (ok && have < kRows) {
+                    ok = barrier_wait(k_raw, raw++ & 1);
+                    clear_rows(ks + st * kTile, kPanels, have);
+                    if (lane == 0) barrier_arrive(k_full + 8 * st);
+                }
+                ok = ok && barrier_wait(v_empty + 8 * st, free);
+                if (ok && lane == 0) {
+                    barrier_expect(v_full + 8 * st, kTile);
+                    for (int x = 0; x < kPanels; ++x) copy_box(vs + st * kTile + x * kPanel, &maps.v, x * 64, wk.kv, y, v_full + 8 * st);
+                }
+                __syncwarp();
             }
-            ok = ok && barrier_wait(v_empty + 8 * st, free);
-            if (ok && lane == 0) {
-                barrier_expect(v_full + 8 * st, kTile);
-                for (int x = 0; x < kPanels; ++x) copy_box(vs + st * kTile + x * kPanel, &maps.v, x * 64, kv, y, v_full + 8 * st);
-            }
-            __syncwarp();
         }
     } else if (warp == 8) {
         const uint32_t scores = product_descriptor<T>(kRows, false), sums = product_descriptor<T>((w.dim + 15) / 16 * 16, true);
@@ -669,120 +739,150 @@ __global__ void __launch_bounds__(kTileThreads, 1) query_gradient_tiles(const __
                 }
             products_arrive(one, bar);
         };
-        if (blocks.n > 0) {
-            ok = barrier_wait(q_full, 0) && barrier_wait(k_full, 0) && barrier_wait(v_full, 0);
+        int loaded = 0, g = 0;  // items and blocks so far
+        for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
+            if (!load_work(item) || blocks.n == 0) continue;
+            // the first block's S and dP: S goes where dS of the block before the last one was
+            ok = barrier_wait(q_full, loaded & 1) && barrier_wait(k_full + 8 * (g % kStages), g / kStages & 1) &&
+                 barrier_wait(v_full + 8 * (g % kStages), g / kStages & 1);
+            if (!ok) break;
             tmem_fence_after();
-            if (ok) {
-                issue(tmem, qs, ks, s_full);
-                issue(dp_at, gs, vs, dp_full);
-                products_arrive(one, v_empty);
+            issue(tmem + (g & 1) * kRows, qs, ks + g % kStages * kTile, s_full + 8 * (g & 1));
+            issue(dp_at, gs, vs + g % kStages * kTile, dp_full);
+            products_arrive(one, v_empty + 8 * (g % kStages));
+            if (blocks.n == 1) products_arrive(one, q_empty);
+            for (int i = 0; i < blocks.n && ok; ++i, ++g) {
+                const int st = g % kStages, next = (g + 1) % kStages, buf = g & 1;
+                const uint32_t next_full = (g + 1) / kStages & 1;
+                const bool more = i + 1 < blocks.n;
+                ok = g == 0 || barrier_wait(dq_done, (g - 1) & 1);
+                if (!ok) break;
+                if (more) {
+                    // S of the next block where dS of the last one was
+                    ok = barrier_wait(k_full + 8 * next, next_full);
+                    if (!ok) break;
+                    tmem_fence_after();
+                    issue(tmem + (buf ^ 1) * kRows, qs, ks + next * kTile, s_full + 8 * (buf ^ 1));
+                }
+                if (i == 0) {  // dQ of the item before is written
+                    ok = barrier_wait(dq_free, (loaded & 1) ^ 1);
+                    if (!ok) break;
+                }
+                const uint64_t keys_of_block = tile_descriptor(ks + st * kTile, kPanel);
+#pragma unroll
+                for (int piece = 0; piece < 2; ++piece) {  // 32 of each warpgroup's 64 columns
+                    ok = ok && barrier_wait(ds_full + 8 * piece, g & 1);
+                    tmem_fence_after();
+                    if (ok)
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) {
+                            const int s = u / 2 * 4 + piece * 2 + u % 2;
+                            product_from_tmem(one, dq_at, tmem + buf * kRows + s / 4 * 64 + s % 4 * 8, keys_of_block + s * 128, sums,
+                                              i > 0 || piece > 0 || u > 0);
+                        }
+                }
+                if (!ok) break;
+                products_arrive(one, dq_done);
+                products_arrive(one, k_empty + 8 * st);
+                if (more) {
+                    ok = barrier_wait(v_full + 8 * next, next_full);
+                    if (!ok) break;
+                    issue(dp_at, gs, vs + next * kTile, dp_full);
+                    products_arrive(one, v_empty + 8 * next);
+                    if (i + 2 == blocks.n) products_arrive(one, q_empty);
+                }
+                __syncwarp();
             }
+            ++loaded;
         }
-        for (int i = 0; i < blocks.n && ok; ++i) {
-            const int st = i % kStages, next = (i + 1) % kStages, buf = i & 1;
-            const uint32_t next_full = (i + 1) / kStages & 1;
-            const bool more = i + 1 < blocks.n;
-            // (every phase of dq_done is waited for here, so that the threads' wait for the last one cannot be a phase early)
-            ok = i == 0 || barrier_wait(dq_done, (i - 1) & 1);
+    } else if (warp == 10) {
+        const float *deltas = after_chain(p.delta);
+        int i = 0;
+        for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
+            if (!load_work(item) || blocks.n == 0) continue;
+            ok = barrier_wait(rows_empty + 8 * (i & 1), (i / 2 & 1) ^ 1);
             if (!ok) break;
-            if (more) {
-                // S of the next block where dS of the last one was
-                ok = barrier_wait(k_full + 8 * next, next_full);
-                if (!ok) break;
-                tmem_fence_after();
-                issue(tmem + (buf ^ 1) * kRows, qs, ks + next * kTile, s_full + 8 * (buf ^ 1));
-            }
-            const uint64_t keys_of_block = tile_descriptor(ks + st * kTile, kPanel);
-#pragma unroll
-            for (int piece = 0; piece < 2; ++piece) {  // 32 of each warpgroup's 64 columns
-                ok = ok && barrier_wait(ds_full + 8 * piece, i & 1);
-                tmem_fence_after();
-                if (ok)
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        const int s = u / 2 * 4 + piece * 2 + u % 2;
-                        product_from_tmem(one, dq_at, tmem + buf * kRows + s / 4 * 64 + s % 4 * 8, keys_of_block + s * 128, sums,
-                                          i > 0 || piece > 0 || u > 0);
-                    }
-            }
-            if (!ok) break;
-            products_arrive(one, dq_done);
-            products_arrive(one, k_empty + 8 * st);
-            if (more) {
-                ok = barrier_wait(v_full + 8 * next, next_full);
-                if (!ok) break;
-                issue(dp_at, gs, vs + next * kTile, dp_full);
-                products_arrive(one, v_empty + 8 * next);
-            }
-            __syncwarp();
+            fetch_rows(p, deltas, wk.row0, wk.kv * group, group, wk.n, rows_at + (i & 1) * 2 * kRows * 4);
+            barrier_arrive(rows_full + 8 * (i & 1));
+            ++i;
         }
     } else if (warp < 8) {
         take_registers();
-        const int half = warp / 4, r = threadIdx.x % 128;
+        const int half = warp / 4, r = threadIdx.x % 128, query = r / group;
         const uint32_t lanes = static_cast<uint32_t>(warp % 4 * 32) << 16;
-        const int query = r / group, head = kv * group + r % group, pos = pos0 + query;
-        const bool mine = query < n;
-        const long long row = row0 + query, at = static_cast<long long>(head) * p.seqs.q_rows + row;
-        float delta, off = 0.f;
-        if (mine) {
-            const float lse = __ldg(p.lse + at);
-            off = lse == -INFINITY ? 0.f : -lse * kLog2e;
-        }
-        row_deltas<T, kDim>(p, row0, kv * group, group, n, deltas);
-        asm volatile("bar.sync 1, 256;" ::: "memory");  // these two warpgroups
-        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(delta) : "r"(deltas + 4 * r) : "memory");
-        if (mine && half == 0) p.delta[at] = delta;
         const float s2 = w.scale * kLog2e;
-        for (int i = 0; i < blocks.n; ++i) {
-            const int k0 = blocks.at(i) * kRows, buf = i & 1, c0 = k0 + half * 64;
-            const uint32_t s_at = tmem + lanes + buf * kRows + half * 64;
-            const bool whole = k0 + kRows - 1 <= pos0 && (pos0 + n - 1 - k0 < w.window || k0 + kRows <= w.sinks);
-            const Range range = {pos - w.window + 1 - c0, pos + 1 - c0, w.sinks - c0};
-            ok = barrier_wait(s_full + 8 * buf, i / 2 & 1);
-            if (!ok) break;
-            tmem_fence_after();
-            uint32_t s[64], d[64];
-            tmem_load32<0>(s_at, s);
-            tmem_load32<32>(s_at + 32, s);
-            tmem_wait_load32<0>(s);
-            tmem_wait_load32<32>(s);
-            if (!whole) hide(s, range, 0xff800000u);
-            const auto weight_off = [&](int) { return pair_of(off, off); };
-            if (whole) {
-                weights_in_place<0, kByFmaInPairs>(s, s2, weight_off);
-                weights_in_place<32, kByFmaInPairs>(s, s2, weight_off);
-            } else {
-                weights_in_place<0, 0>(s, s2, weight_off);
-                weights_in_place<32, 0>(s, s2, weight_off);
+        int started = 0, g = 0;  // items and blocks so far
+        for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
+            if (!load_work(item)) continue;
+            const int head = wk.kv * group + r % group, pos = wk.pos0 + query, n = wk.n;
+            const bool mine = query < n;
+            const uint32_t rows = rows_at + (started & 1) * 2 * kRows * 4;
+            float off = 0.f, minus_delta = 0.f;
+            if (blocks.n > 0) {
+                ok = barrier_wait(rows_full + 8 * (started & 1), started / 2 & 1);
+                if (!ok) break;
+                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(off) : "r"(rows + 4 * r) : "memory");
+                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(minus_delta) : "r"(rows + 4 * (kRows + r)) : "memory");
+                barrier_arrive(rows_empty + 8 * (started & 1));
+                ++started;
             }
-            ok = barrier_wait(dp_full, i & 1);
-            if (!ok) break;
-            tmem_fence_after();
-            tmem_load32<0>(dp_at + lanes + half * 64, d);
-            tmem_load32<32>(dp_at + lanes + half * 64 + 32, d);
-            tmem_wait_load32<0>(d);
-            tmem_wait_load32<32>(d);
-            if (!whole) hide(d, range, 0u);
-            const auto minus = [&](int) { return pair_of(-delta, -delta); };
-            gradients_in_place<T, 0>(s, d, minus);
-            tmem_store16<0>(s_at, s);
-            tmem_wait_store();
-            tmem_fence_before();
-            barrier_arrive(ds_full);
-            gradients_in_place<T, 32>(s, d, minus);
-            tmem_store16<16>(s_at + 16, s);
-            tmem_wait_store();
-            tmem_fence_before();
-            barrier_arrive(ds_full + 8);
-        }
-        if (ok && blocks.n > 0) {
-            ok = barrier_wait(dq_done, (blocks.n - 1) & 1);
-            tmem_fence_after();
-        }
-        T *out = static_cast<T *>(p.dq) + (row * w.heads + head) * w.dim;
+            for (int i = 0; i < blocks.n; ++i, ++g) {
+                const int k0 = blocks.at(i) * kRows, buf = g & 1, c0 = k0 + half * 64;
+                const uint32_t s_at = tmem + lanes + buf * kRows + half * 64;
+                const bool whole = k0 + kRows - 1 <= wk.pos0 && (wk.pos0 + n - 1 - k0 < w.window || k0 + kRows <= w.sinks);
+                const Range range = {pos - w.window + 1 - c0, pos + 1 - c0, w.sinks - c0};
+                ok = barrier_wait(s_full + 8 * buf, g / 2 & 1);
+                if (!ok) break;
+                tmem_fence_after();
+                uint32_t s[64], d[64];
+                tmem_load32<0>(s_at, s);
+                tmem_load32<32>(s_at + 32, s);
+                tmem_wait_load32<0>(s);
+                tmem_wait_load32<32>(s);
+                if (!whole) hide(s, range, 0xff800000u);
+                const auto weight_off = [&](int) { return pair_of(off, off); };
+                if (whole) {
+                    weights_in_place<0, kByFmaInPairs>(s, s2, weight_off);
+                    weights_in_place<32, kByFmaInPairs>(s, s2, weight_off);
+                } else {
+                    weights_in_place<0, 0>(s, s2, weight_off);
+                    weights_in_place<32, 0>(s, s2, weight_off);
+                }
+                // (dQ of the block before is complete by now; every phase of its barrier is waited for, so that the last one of the item
+                // cannot be taken for an earlier one)
+                ok = barrier_wait(dp_full, g & 1) && (i == 0 || barrier_wait(dq_done, (g - 1) & 1));
+                if (!ok) break;
+                tmem_fence_after();
+                tmem_load32<0>(dp_at + lanes + half * 64, d);
+                tmem_load32<32>(dp_at + lanes + half * 64 + 32, d);
+                tmem_wait_load32<0>(d);
+                tmem_wait_load32<32>(d);
+                if (!whole) hide(d, range, 0u);
+                const auto minus = [&](int) { return pair_of(minus_delta, minus_delta); };
+                gradients_in_place<T, 0>(s, d, minus);
+                tmem_store16<0>(s_at, s);
+                tmem_wait_store();
+                tmem_fence_before();
+                barrier_arrive(ds_full);
+                gradients_in_place<T, 32>(s, d, minus);
+                tmem_store16<16>(s_at + 16, s);
+                tmem_wait_store();
+                tmem_fence_before();
+                barrier_arrive(ds_full + 8);
+            }
+            if (ok && blocks.n > 0) {
+                ok = barrier_wait(dq_done, (g - 1) & 1);
+                tmem_fence_after();
+            }
+            T *out = static_cast<T *>(p.dq) + ((wk.row0 + query) * w.heads + head) * w.dim;
 #pragma unroll
-        for (int x = 0; x < kDim / 2; x += 32)
-            store_columns(out, dq_at + lanes, half * (kDim / 2) + x, w.dim, w.scale, mine, blocks.n > 0);
+            for (int x = 0; x < kDim / 2; x += 32)
+                store_columns(out, dq_at + lanes, half * (kDim / 2) + x, w.dim, w.scale, mine, blocks.n > 0);
+            if (blocks.n > 0) {
+                tmem_fence_before();
+                barrier_arrive(dq_free);
+            }
+        }
     }
     if (!ok) waits_failed = 1;
     tmem_fence_before();
@@ -815,7 +915,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) key_gradient_tiles(const __gr
     extern __shared__ char shared_raw[];
     const Window &w = p.win;
     const int group = w.heads / w.kv_heads, per_tile = kRows / group, kv = blockIdx.y;
-    const int far = static_cast<int>(blockIdx.x) < p.far_slots ? blockIdx.x : -1;
+    const int far = static_cast<int>(blockIdx.x) < p.far_slots ? static_cast<int>(blockIdx.x) : -1;
     Tile t;
     int2 queries;
     int chunk = 0;  // first query of a far chunk
@@ -850,7 +950,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) key_gradient_tiles(const __gr
     const uint32_t ks = base, vs = ks + kTile, qs = vs + kTile, gs = qs + kStages * kTile, rows_at = gs + kStages * kTile,
                    bars = rows_at + kStages * 2 * kRows * 4;
     const uint32_t k_full = bars, raw = bars + 8, s_full = bars + 16, s_read = bars + 24, dp_full = bars + 32, ds_full = bars + 48,
-                   done = bars + 64, q_full = bars + 80, q_empty = q_full + 8 * kStages, g_full = q_empty + 8 * kStages,
+                   done = bars + 64, all_done = bars + 72, q_full = bars + 80, q_empty = q_full + 8 * kStages, g_full = q_empty + 8 * kStages,
                    g_empty = g_full + 8 * kStages, rows_full = g_empty + 8 * kStages, tmem_at = rows_full + 8 * kStages;
     const int warp = uniform(threadIdx.x / 32), lane = threadIdx.x % 32;
     if (warp == 8) {
@@ -865,6 +965,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) key_gradient_tiles(const __gr
                 barrier_init(ds_full + 8 * i, 256);
             }
             barrier_init(done, 1);
+            barrier_init(all_done, 1);
             for (int i = 0; i < kStages; ++i) {
                 barrier_init(q_full + 8 * i, 1);
                 barrier_init(q_empty + 8 * i, 1);
@@ -924,22 +1025,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) key_gradient_tiles(const __gr
     } else if (warp == 10) {
         // lse and delta of the tiles' rows
         for (int i = 0; i < tiles && ok; ++i) {
-            const int st = i % kStages, n = queries_of(i);
-            const long long first = static_cast<long long>(queries.x) + i0 + i * per_tile;
+            const int st = i % kStages;
             // (free when the queries of the stage are: their last product comes behind ds_full)
             ok = barrier_wait(q_empty + 8 * st, (i / kStages & 1) ^ 1);
             if (!ok) break;
-            for (int r = lane; r < kRows; r += 32) {
-                float lse = 0.f, delta = 0.f;
-                if (r / group < n) {
-                    const long long at = static_cast<long long>(kv * group + r % group) * p.seqs.q_rows + first + r / group;
-                    lse = __ldg(p.lse + at);
-                    lse = lse == -INFINITY ? 0.f : -lse * kLog2e;
-                    delta = __ldg(p.delta + at);
-                }
-                asm volatile("st.shared.b32 [%0], %1;" ::"r"(rows_at + (st * 2 * kRows + r) * 4), "f"(lse) : "memory");
-                asm volatile("st.shared.b32 [%0], %1;" ::"r"(rows_at + (st * 2 * kRows + kRows + r) * 4), "f"(-delta) : "memory");
-            }
+            fetch_rows(p, p.delta, static_cast<long long>(queries.x) + i0 + i * per_tile, kv * group, group, queries_of(i),
+                       rows_at + st * 2 * kRows * 4);
             barrier_arrive(rows_full + 8 * st);
         }
     } else if (warp == 8) {
@@ -974,7 +1065,6 @@ __global__ void __launch_bounds__(kTileThreads, 1) key_gradient_tiles(const __gr
                 tmem_fence_after();
                 issue(tmem, ks, qs + next * kTile, s_full);
             }
-            // (every phase of `done` is waited for here, so that the threads' wait for the last one cannot be a phase early)
             ok = i == 0 || kBuffers == 1 || barrier_wait(done, (i - 1) & 1);
             if (!ok) break;
             if (kBuffers == 2 && more) {
@@ -997,6 +1087,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) key_gradient_tiles(const __gr
             }
             if (!ok) break;
             products_arrive(one, done);
+            if (!more) products_arrive(one, all_done);
             products_arrive(one, q_empty + 8 * st);
             products_arrive(one, g_empty + 8 * st);
             if (kBuffers == 1) {
@@ -1065,7 +1156,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) key_gradient_tiles(const __gr
             barrier_arrive(ds_full + 8);
         }
         if (ok && tiles > 0) {
-            ok = barrier_wait(done, (tiles - 1) & 1);
+            // (not `done`, which may still be two tiles behind the threads: a wait for its last phase would take an earlier one for it)
+            ok = barrier_wait(all_done, 0);
             tmem_fence_after();
         }
         const uint32_t sum_at = (half == 0 ? dv_at : dk_at) + lanes;
@@ -1206,8 +1298,10 @@ int tiles_prompt(int dtype, const Prompt &p, cudaStream_t stream) {
         if (const int e = encode(&maps.q, dtype, p.q, p.q.row, p.seqs.q_rows, w.heads, w.dim, group, per_tile)) return e;
         if (const int e = encode(&maps.k, dtype, p.k, p.k.row, p.seqs.k_rows, w.kv_heads, w.dim, 1, kRows)) return e;
         if (const int e = encode(&maps.v, dtype, p.v, p.v.row, p.seqs.k_rows, w.kv_heads, w.dim, 1, kRows)) return e;
-        const int slots = tile_slots(p.seqs.q_offsets, p.seqs.n_seq, p.seqs.q_rows, 2 * per_tile);
-        kernel<<<dim3(slots, w.kv_heads), kTileThreads, forward_bytes<kDim>(), stream>>>(maps, p, Cached{});
+        const long long items = static_cast<long long>(tile_slots(p.seqs.q_offsets, p.seqs.n_seq, p.seqs.q_rows, 2 * per_tile)) * w.kv_heads;
+        if (items > INT_MAX / 2) return fail(RODE_ERR_INVALID_ARGUMENT, "rode_window_attention: too many rows and heads");
+        const int ctas = static_cast<int>(std::min<long long>(items, sm_count()));
+        kernel<<<ctas, kTileThreads, forward_bytes<kDim>(), stream>>>(maps, p, Cached{}, static_cast<int>(items));
         RODE_CHECK_LAUNCH("forward_tiles");
         return static_cast<int>(RODE_OK);
     });
@@ -1243,11 +1337,16 @@ int tiles_backward(int dtype, const Prompt &p, cudaStream_t stream) {
         if (const int e = encode(&maps.dout, dtype, p.dout, p.dout.row, p.seqs.q_rows, w.heads, w.dim, group, per_tile)) return e;
         if (const int e = encode(&maps.k, dtype, p.k, p.k.row, p.seqs.k_rows, w.kv_heads, w.dim, 1, kRows)) return e;
         if (const int e = encode(&maps.v, dtype, p.v, p.v.row, p.seqs.k_rows, w.kv_heads, w.dim, 1, kRows)) return e;
-        const int slots = tile_slots(p.seqs.q_offsets, p.seqs.n_seq, p.seqs.q_rows, per_tile);
-        rows<<<dim3(slots, w.kv_heads), kTileThreads, backward_bytes<kDim>(), stream>>>(maps, p);
-        RODE_CHECK_LAUNCH("query_gradient_tiles");
+        const long long items = static_cast<long long>(tile_slots(p.seqs.q_offsets, p.seqs.n_seq, p.seqs.q_rows, per_tile)) * w.kv_heads;
+        if (items > INT_MAX / 2) return fail(RODE_ERR_INVALID_ARGUMENT, "rode_window_attention_backward: too many rows and heads");
+        const long long all = static_cast<long long>(p.seqs.q_rows) * w.heads, per_cta = 256 / (kDim / 8);
+        row_deltas<T, kDim><<<static_cast<unsigned>((all + per_cta - 1) / per_cta), 256, 0, stream>>>(p);
+        RODE_CHECK_LAUNCH("row_deltas");
+        RODE_CUDA_TRY(launch_part(rows, dim3(static_cast<unsigned>(std::min<long long>(items, sm_count()))), kTileThreads, backward_bytes<kDim>(),
+                                  stream, true, maps, p, static_cast<int>(items)));
         if (p.dk == nullptr) return static_cast<int>(RODE_OK);
         const int k_slots = tile_slots(p.seqs.k_offsets, p.seqs.n_seq, p.seqs.k_rows, kRows);
+        // (Not beside dQ's grid: a grid that starts early sees what the grids before its predecessor wrote only by waiting for that one.)
         keys<<<dim3(p.far_slots + k_slots, w.kv_heads), kTileThreads, backward_bytes<kDim>(), stream>>>(maps, p);
         RODE_CHECK_LAUNCH("key_gradient_tiles");
         if (p.far_slots > 0) {
@@ -1270,8 +1369,10 @@ int tiles_shared(int dtype, const Cached &c, cudaStream_t stream) {
         if (const int e = encode(&maps.q, dtype, c.q, c.q.batch, c.batch, w.heads, w.dim, group, per_tile)) return e;
         if (const int e = encode(&maps.k, dtype, c.pk, c.pk.row, c.prefix, w.kv_heads, w.dim, 1, kRows)) return e;
         if (const int e = encode(&maps.v, dtype, c.pv, c.pv.row, c.prefix, w.kv_heads, w.dim, 1, kRows)) return e;
-        const int tiles = (c.batch + 2 * per_tile - 1) / (2 * per_tile);
-        kernel<<<dim3(tiles, w.kv_heads, c.prefix_parts), kTileThreads, forward_bytes<kDim>(), stream>>>(maps, Prompt{}, c);
+        const long long items = (static_cast<long long>(c.batch) + 2 * per_tile - 1) / (2 * per_tile) * w.kv_heads * c.prefix_parts;
+        if (items > INT_MAX / 2) return fail(RODE_ERR_INVALID_ARGUMENT, "rode_shared_prefix_attention: too many requests and heads");
+        const int ctas = static_cast<int>(std::min<long long>(items, sm_count()));
+        kernel<<<ctas, kTileThreads, forward_bytes<kDim>(), stream>>>(maps, Prompt{}, c, static_cast<int>(items));
         RODE_CHECK_LAUNCH("forward_tiles");
         return static_cast<int>(RODE_OK);
     });

@@ -66,6 +66,8 @@ __device__ __forceinline__ void copy_box(uint32_t dst, const CUtensorMap *map, i
         : "memory");
 }
 
+__device__ __forceinline__ void prefetch_map(const CUtensorMap *map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
+
 // --- tensor memory --------------------------------------------------------------------------------------------------------------
 
 // One warp; the address is written to shared memory.
