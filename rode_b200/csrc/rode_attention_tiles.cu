@@ -950,7 +950,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) key_gradient_tiles(const __gr
     const uint32_t ks = base, vs = ks + kTile, qs = vs + kTile, gs = qs + kStages * kTile, rows_at = gs + kStages * kTile,
                    bars = rows_at + kStages * 2 * kRows * 4;
     const uint32_t k_full = bars, raw = bars + 8, s_full = bars + 16, s_read = bars + 24, dp_full = bars + 32, ds_full = bars + 48,
-                   done = bars + 64, all_done = bars + 72, q_full = bars + 80, q_empty = q_full + 8 * kStages, g_full = q_empty + 8 * kStages,
+                   done = bars + 80, all_done = bars + 88, q_full = bars + 96, q_empty = q_full + 8 * kStages, g_full = q_empty + 8 * kStages,
                    g_empty = g_full + 8 * kStages, rows_full = g_empty + 8 * kStages, tmem_at = rows_full + 8 * kStages;
     const int warp = uniform(threadIdx.x / 32), lane = threadIdx.x % 32;
     if (warp == 8) {
@@ -962,7 +962,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) key_gradient_tiles(const __gr
             barrier_init(s_read, 256);
             for (int i = 0; i < 2; ++i) {
                 barrier_init(dp_full + 8 * i, 1);
-                barrier_init(ds_full + 8 * i, 256);
+                barrier_init(ds_full + 16 * i, 256);
+                barrier_init(ds_full + 16 * i + 8, 256);
             }
             barrier_init(done, 1);
             barrier_init(all_done, 1);
@@ -983,7 +984,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) key_gradient_tiles(const __gr
     uint32_t tmem;
     asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem) : "r"(tmem_at));
     tmem = uniform(tmem);
-    constexpr int kBuffers = kDim == 64 ? 2 : 1;  // of dP
+    constexpr int kBuffers = kDim == 64 ? 2 : 1;  // of dP (each with barriers of its own: the threads may be a tile ahead of the products)
     const uint32_t dp_at = tmem + 128, dv_at = tmem + 512 - 2 * kDim, dk_at = tmem + 512 - kDim;
     bool ok = true;
 
@@ -1075,7 +1076,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) key_gradient_tiles(const __gr
             const uint64_t x = tile_descriptor(qs + st * kTile, kPanel), y = tile_descriptor(gs + st * kTile, kPanel);
 #pragma unroll
             for (int piece = 0; piece < 2; ++piece) {  // 32 of each warpgroup's 64 columns
-                ok = ok && barrier_wait(ds_full + 8 * piece, i & 1);
+                ok = ok && barrier_wait(ds_full + i % kBuffers * 16 + 8 * piece, i / kBuffers & 1);
                 tmem_fence_after();
                 if (ok)
 #pragma unroll
@@ -1148,12 +1149,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) key_gradient_tiles(const __gr
             tmem_store16<0>(d_at, s);
             tmem_wait_store();
             tmem_fence_before();
-            barrier_arrive(ds_full);
+            barrier_arrive(ds_full + i % kBuffers * 16);
             gradients_in_place<T, 32>(s, d, minus);
             tmem_store16<16>(d_at + 16, s);
             tmem_wait_store();
             tmem_fence_before();
-            barrier_arrive(ds_full + 8);
+            barrier_arrive(ds_full + i % kBuffers * 16 + 8);
         }
         if (ok && tiles > 0) {
             // (not `done`, which may still be two tiles behind the threads: a wait for its last phase would take an earlier one for it)
