@@ -14,28 +14,8 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import rode_sddmm_cuda
-
-
-class _WindowAttention(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, window, sinks, q_offsets, k_offsets, scale):
-        out, lse = rode_sddmm_cuda.window_attention_forward(q, k, v, window, sinks, q_offsets, k_offsets, scale, True)
-        ctx.save_for_backward(q, k, v, out, lse, q_offsets, k_offsets)
-        ctx.pattern = (window, sinks, scale)
-        return out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dout):
-        q, k, v, out, lse, q_offsets, k_offsets = ctx.saved_tensors
-        window, sinks, scale = ctx.pattern
-        keys = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
-        dq, dk, dv = rode_sddmm_cuda.window_attention_backward(q, k, v, out, lse, dout, window, sinks, q_offsets, k_offsets, scale,
-                                                               keys)
-        return dq, dk, dv, None, None, None, None, None
 
 
 def _scale(scale: Optional[float], q: torch.Tensor) -> float:
@@ -46,7 +26,7 @@ def rode_window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, win
                           q_offsets: Optional[torch.Tensor] = None, k_offsets: Optional[torch.Tensor] = None,
                           scale: Optional[float] = None) -> torch.Tensor:
     """Attention in which a query sees the ``window`` keys up to its own position and the first ``sinks`` keys of its sequence;
-    differentiable with respect to q, k and v.
+    differentiable with respect to q, k and v, once.
 
     q [q_rows, heads, dim], k and v [k_rows, kv_heads, dim] hold sequences one behind the other: sequence s is rows
     ``q_offsets[s]`` to ``q_offsets[s + 1]`` of q and ``k_offsets[s]`` to ``k_offsets[s + 1]`` of k and v (int32 on the device, not
@@ -55,10 +35,7 @@ def rode_window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, win
     sequence: causal attention.  Rows that belong to no sequence get zeros, in the result and in the gradients.
 
     ``scale`` multiplies the scores, ``dim ** -0.5`` by default.  Operands whose strides the kernels cannot take are copied."""
-    scale = _scale(scale, q)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        return _WindowAttention.apply(q, k, v, window, sinks, q_offsets, k_offsets, scale)
-    return rode_sddmm_cuda.window_attention_forward(q, k, v, window, sinks, q_offsets, k_offsets, scale, False)[0]
+    return rode_sddmm_cuda.window_attention(q, k, v, window, sinks, q_offsets, k_offsets, _scale(scale, q))
 
 
 def rode_window_attention_step(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, lengths: torch.Tensor, window: int,

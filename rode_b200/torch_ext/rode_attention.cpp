@@ -4,6 +4,7 @@
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
 #include <tuple>
@@ -123,7 +124,7 @@ void check_prompt(const Tensor &q, const Tensor &k, const Tensor &v) {
     TORCH_CHECK_VALUE(k.size(2) == q.size(2), "k must have the head dimension of q, got ", k.size(2), " and ", q.size(2));
 }
 
-std::tuple<Tensor, OptionalTensor> py_window_forward(const Tensor &q_in, const Tensor &k_in, const Tensor &v_in, int64_t window,
+std::tuple<Tensor, Tensor> window_forward(const Tensor &q_in, const Tensor &k_in, const Tensor &v_in, int64_t window,
                                                       int64_t sinks, const OptionalTensor &q_offsets,
                                                       const OptionalTensor &k_offsets, double scale, bool want_lse) {
     check_prompt(q_in, k_in, v_in);
@@ -133,38 +134,30 @@ std::tuple<Tensor, OptionalTensor> py_window_forward(const Tensor &q_in, const T
     const Tensor q = fitting(q_in), k = fitting(k_in), v = fitting(v_in);
     const int rows = to_int(q.size(0), "rows of q"), heads = to_int(q.size(1), "heads"), dim = to_int(q.size(2), "dim");
     Tensor out = empty_on(q.sizes(), q.scalar_type(), q.device());
-    OptionalTensor lse;
+    Tensor lse;
     if (want_lse) lse = empty_on({heads, rows}, torch::kFloat32, q.device());
     const rode_heads_t qh = rows_heads(q), kh = rows_heads(k), vh = rows_heads(v);
     check_status(rode_window_attention(dtype, s.n, s.q, s.k, rows, to_int(k.size(0), "rows of k"), heads,
                                        to_int(k.size(1), "key heads"), dim, window_of(window), sinks_of(sinks),
                                        static_cast<float>(scale), 1, &qh, &kh, &vh, out.data_ptr(),
-                                       want_lse ? lse->data_ptr<float>() : nullptr,
+                                       want_lse ? lse.data_ptr<float>() : nullptr,
                                        at::cuda::getCurrentCUDAStream(q.device().index()).stream()));
     return {out, lse};
 }
 
-std::tuple<Tensor, OptionalTensor, OptionalTensor> py_window_backward(const Tensor &q_in, const Tensor &k_in, const Tensor &v_in,
-                                                                        const Tensor &out, const Tensor &lse,
-                                                                        const Tensor &dout_in, int64_t window, int64_t sinks,
-                                                                        const OptionalTensor &q_offsets,
-                                                                        const OptionalTensor &k_offsets, double scale,
-                                                                        bool want_keys) {
-    check_prompt(q_in, k_in, v_in);
+// out and lse are window_forward's.
+std::tuple<Tensor, Tensor, Tensor> window_backward(const Tensor &q_in, const Tensor &k_in, const Tensor &v_in, const Tensor &out,
+                                                    const Tensor &lse, const Tensor &dout_in, int64_t window, int64_t sinks,
+                                                    const OptionalTensor &q_offsets, const OptionalTensor &k_offsets, double scale,
+                                                    bool want_keys) {
     const int dtype = dtype_of(q_in);
-    check_like(out, "out", q_in, 3);
-    check_like(dout_in, "dout", q_in, 3);
-    TORCH_CHECK_VALUE(out.sizes() == q_in.sizes() && out.is_contiguous(), "out must be contiguous and of q's shape");
-    TORCH_CHECK_VALUE(dout_in.sizes() == q_in.sizes(), "dout must have q's shape, got ", dout_in.sizes());
-    TORCH_CHECK_VALUE(lse.scalar_type() == torch::kFloat32 && lse.is_contiguous() && lse.device() == q_in.device() &&
-                          lse.dim() == 2 && lse.size(0) == q_in.size(1) && lse.size(1) == q_in.size(0),
-                      "lse must be contiguous float32 [heads, rows]");
+    check_like(dout_in, "the gradient of the result", q_in, 3);
     const c10::cuda::CUDAGuard guard(q_in.device());
     const Sequences s = sequences(q_in, k_in, q_offsets, k_offsets);
     const Tensor q = fitting(q_in), k = fitting(k_in), v = fitting(v_in), dout = fitting(dout_in);
     const int rows = to_int(q.size(0), "rows of q"), heads = to_int(q.size(1), "heads"), dim = to_int(q.size(2), "dim");
     Tensor dq = empty_on(q.sizes(), q.scalar_type(), q.device());
-    OptionalTensor dk, dv;
+    Tensor dk, dv;
     if (want_keys) {
         dk = empty_on(k.sizes(), q.scalar_type(), q.device());
         dv = empty_on(k.sizes(), q.scalar_type(), q.device());
@@ -177,9 +170,54 @@ std::tuple<Tensor, OptionalTensor, OptionalTensor> py_window_backward(const Tens
     check_status(rode_window_attention_backward(
         dtype, s.n, s.q, s.k, rows, to_int(k.size(0), "rows of k"), heads, to_int(k.size(1), "key heads"), dim, window_of(window),
         sinks_of(sinks), static_cast<float>(scale), 1, &qh, &kh, &vh, out.data_ptr(), lse.data_ptr<float>(), &gh, dq.data_ptr(),
-        want_keys ? dk->data_ptr() : nullptr, want_keys ? dv->data_ptr() : nullptr, ws.data_ptr(), bytes,
+        want_keys ? dk.data_ptr() : nullptr, want_keys ? dv.data_ptr() : nullptr, ws.data_ptr(), bytes,
         at::cuda::getCurrentCUDAStream(q.device().index()).stream()));
     return {dq, dk, dv};
+}
+
+OptionalTensor given(const Tensor &x) { return x.defined() ? OptionalTensor(x) : OptionalTensor(); }
+
+// (In C++: a training step of a few thousand tokens is bound by the host, and the same in Python took 100 us of it.)
+struct WindowAttention : torch::autograd::Function<WindowAttention> {
+    static Tensor forward(torch::autograd::AutogradContext *ctx, const Tensor &q, const Tensor &k, const Tensor &v, int64_t window,
+                          int64_t sinks, const OptionalTensor &q_offsets, const OptionalTensor &k_offsets, double scale) {
+        auto [out, lse] = window_forward(q, k, v, window, sinks, q_offsets, k_offsets, scale, true);
+        ctx->save_for_backward({q, k, v, out, lse, q_offsets.value_or(Tensor()), k_offsets.value_or(Tensor())});
+        ctx->saved_data["window"] = window;
+        ctx->saved_data["sinks"] = sinks;
+        ctx->saved_data["scale"] = scale;
+        return out;
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list dout) {
+        const auto saved = ctx->get_saved_variables();
+        torch::autograd::variable_list grads(8);
+        const bool twice = torch::GradMode::is_enabled();
+        {
+            const torch::NoGradGuard guard;
+            std::tie(grads[0], grads[1], grads[2]) =
+                window_backward(saved[0], saved[1], saved[2], saved[3], saved[4], dout[0], ctx->saved_data["window"].toInt(),
+                                ctx->saved_data["sinks"].toInt(), given(saved[5]), given(saved[6]), ctx->saved_data["scale"].toDouble(),
+                                ctx->needs_input_grad(1) || ctx->needs_input_grad(2));
+        }
+        if (twice) {  // the gradients themselves have none: an error when somebody asks for it
+            torch::autograd::variable_list some;
+            for (int i = 0; i < 3; ++i)
+                if (grads[i].defined()) some.push_back(grads[i].detach().set_requires_grad(true));
+            auto error = std::make_shared<torch::autograd::DelayedError>("rode_window_attention can be differentiated once only",
+                                                                         static_cast<int64_t>(some.size()));
+            some = (*error)(std::move(some));
+            for (size_t i = 0, n = 0; i < 3; ++i)
+                if (grads[i].defined()) grads[i] = some[n++];
+        }
+        return grads;
+    }
+};
+
+Tensor py_window_attention(const Tensor &q, const Tensor &k, const Tensor &v, int64_t window, int64_t sinks,
+                           const OptionalTensor &q_offsets, const OptionalTensor &k_offsets, double scale) {
+    if (torch::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad()))
+        return WindowAttention::apply(q, k, v, window, sinks, q_offsets, k_offsets, scale);
+    return std::get<0>(window_forward(q, k, v, window, sinks, q_offsets, k_offsets, scale, false));
 }
 
 // Caches are read where they lie: a copy would cost more than the call.
@@ -267,12 +305,9 @@ Tensor py_shared_prefix(const Tensor &q_in, const Tensor &prefix_k, const Tensor
 
 void bind_attention(pybind11::module_ &m) {
     namespace py = pybind11;
-    m.def("window_attention_forward", &py_window_forward, "Window-and-sinks attention over packed sequences (CUDA)", py::arg("q"),
-          py::arg("k"), py::arg("v"), py::arg("window"), py::arg("sinks"), py::arg("q_offsets"), py::arg("k_offsets"),
-          py::arg("scale"), py::arg("want_lse"));
-    m.def("window_attention_backward", &py_window_backward, "Its gradients (CUDA)", py::arg("q"), py::arg("k"), py::arg("v"),
-          py::arg("out"), py::arg("lse"), py::arg("dout"), py::arg("window"), py::arg("sinks"), py::arg("q_offsets"),
-          py::arg("k_offsets"), py::arg("scale"), py::arg("want_keys"));
+    m.def("window_attention", &py_window_attention, "Window-and-sinks attention over packed sequences, differentiable (CUDA)",
+          py::arg("q"), py::arg("k"), py::arg("v"), py::arg("window"), py::arg("sinks"), py::arg("q_offsets"), py::arg("k_offsets"),
+          py::arg("scale"));
     m.def("window_attention_step", &py_window_step, "Window-and-sinks attention of one token per sequence (CUDA)", py::arg("q"),
           py::arg("k_cache"), py::arg("v_cache"), py::arg("lengths"), py::arg("window"), py::arg("sinks"), py::arg("scale"));
     m.def("shared_prefix_attention", &py_shared_prefix, "Attention of one token per request behind a shared prefix (CUDA)",

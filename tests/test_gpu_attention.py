@@ -234,6 +234,18 @@ def test_only_some_gradients():
     assert torch.equal(b.grad, full["dv"])
 
 
+def test_second_derivative_is_refused():
+    from rode_b200.rode_attention import rode_window_attention
+
+    q, k, v, dout = _make([50], [50], 4, 2, 64, torch.float32, seed=13)
+    full = _run(q, k, v, dout, 20, 2)
+    leaf = q.clone().requires_grad_()
+    grad, = torch.autograd.grad(rode_window_attention(leaf, k, v, 20, 2), leaf, dout, create_graph=True)
+    assert torch.equal(grad.detach(), full["dq"])
+    with pytest.raises(RuntimeError, match="once"):
+        grad.sum().backward()
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_captured_and_on_another_stream(dtype):
     from rode_b200.rode_attention import rode_window_attention
