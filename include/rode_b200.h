@@ -335,8 +335,8 @@ int rode_window_attention(int dtype, int n_seq, const int *q_offsets, const int 
 /* Its gradients: dq [q_rows, heads, dim], dk and dv [k_rows, kv_heads, dim] contiguous, dk and dv both or neither (null).
  * out and lse are what the forward call wrote.  workspace: rode_window_attention_backward_workspace_bytes() bytes,
  * 16-byte aligned, not shared by calls that may overlap in time. */
-int rode_window_attention_backward_workspace_bytes(int n_seq, int q_rows, int heads, int kv_heads, int dim, int window,
-                                                   int sinks, size_t *bytes);
+int rode_window_attention_backward_workspace_bytes(int dtype, int n_seq, int q_rows, int k_rows, int heads, int kv_heads,
+                                                   int dim, int window, int sinks, size_t *bytes);
 int rode_window_attention_backward(int dtype, int n_seq, const int *q_offsets, const int *k_offsets, int q_rows,
                                    int k_rows, int heads, int kv_heads, int dim, int window, int sinks, float scale,
                                    int clear, const rode_heads_t *q, const rode_heads_t *k, const rode_heads_t *v,

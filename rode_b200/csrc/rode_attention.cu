@@ -179,16 +179,19 @@ int rode_window_attention(int dtype, int n_seq, const int *q_offsets, const int 
     return tiles_take_prompt(dtype, p) ? tiles_prompt(dtype, p, stream) : simple_prompt(dtype, p, stream);
 }
 
-int rode_window_attention_backward_workspace_bytes(int n_seq, int q_rows, int heads, int kv_heads, int dim, int window, int sinks,
-                                                   size_t *bytes) {
+int rode_window_attention_backward_workspace_bytes(int dtype, int n_seq, int q_rows, int k_rows, int heads, int kv_heads, int dim,
+                                                   int window, int sinks, size_t *bytes) {
     const char *what = "rode_window_attention_backward_workspace_bytes";
     if (bytes == nullptr) return fail(RODE_ERR_INVALID_ARGUMENT, "%s: null pointer bytes", what);
-    RODE_TRY(check_shape(what, RODE_F32, heads, kv_heads, dim, 1.f));
+    RODE_TRY(check_shape(what, dtype, heads, kv_heads, dim, 1.f));
     RODE_TRY(check_window(what, window, sinks));
-    if (q_rows < 0 || q_rows > kMaxRows || n_seq < 0 || n_seq > kMaxRows)
-        return fail(RODE_ERR_INVALID_ARGUMENT, "%s: q_rows = %d and n_seq = %d must be 0 to 2^30", what, q_rows, n_seq);
+    if (q_rows < 0 || q_rows > kMaxRows || k_rows < 0 || k_rows > kMaxRows || n_seq < 0 || n_seq > kMaxRows)
+        return fail(RODE_ERR_INVALID_ARGUMENT, "%s: q_rows = %d, k_rows = %d and n_seq = %d must be 0 to 2^30", what, q_rows, k_rows,
+                    n_seq);
     const FarPlan far = plan_far(n_seq, true, q_rows, kv_heads, dim, window, sinks);
-    *bytes = delta_bytes(q_rows, heads) + far.near_bytes + far.far_bytes;
+    // (fp32 never runs on the kernels that cut far queries off, nor 16-bit types on those that want the heads apart)
+    *bytes = delta_bytes(q_rows, heads) + (dtype == RODE_F32 ? simple_backward_bytes(dtype, n_seq, k_rows, heads, kv_heads, dim)
+                                                            : far.near_bytes + far.far_bytes);
     return RODE_OK;
 }
 
@@ -212,7 +215,7 @@ int rode_window_attention_backward(int dtype, int n_seq, const int *q_offsets, c
     RODE_TRY(check_result(what, "dv", dv, keys && k_rows > 0));
     if (q_rows > 0 && lse == nullptr) return fail(RODE_ERR_INVALID_ARGUMENT, "%s: null pointer lse", what);
     size_t need = 0;
-    RODE_TRY(rode_window_attention_backward_workspace_bytes(n_seq, q_rows, heads, kv_heads, dim, window, sinks, &need));
+    RODE_TRY(rode_window_attention_backward_workspace_bytes(dtype, n_seq, q_rows, k_rows, heads, kv_heads, dim, window, sinks, &need));
     RODE_TRY(check_workspace(what, workspace, workspace_bytes, need));
     if (q_rows == 0 && (k_rows == 0 || !keys)) return RODE_OK;
     Prompt p = {};
@@ -233,7 +236,11 @@ int rode_window_attention_backward(int dtype, int n_seq, const int *q_offsets, c
     p.dv = dv;
     p.delta = static_cast<float *>(workspace);
     p.clear = clear != 0;
-    if (!tiles_take_backward(dtype, p)) return simple_prompt_backward(dtype, p, stream);
+    if (!tiles_take_backward(dtype, p)) {
+        if (simple_backward_bytes(dtype, n_seq, k_rows, heads, kv_heads, dim) > 0 && keys)
+            p.head_part = p.delta + delta_bytes(q_rows, heads) / sizeof(float);
+        return simple_prompt_backward(dtype, p, stream);
+    }
     const FarPlan far = plan_far(n_seq, q_offsets != nullptr, q_rows, kv_heads, dim, window, sinks);
     if (keys) {
         p.far_chunk = far.chunk;

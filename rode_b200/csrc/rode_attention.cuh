@@ -45,6 +45,7 @@ struct Prompt {
     // Chunks of the queries that see sinks only (key_gradient_tiles); far_slots == 0: none
     int far_chunk, far_slots;
     float *near_part, *far_part;
+    float *head_part;  // fp32 sums of dK and dV by query head, [2, k_rows, heads, dim] (key_gradients); null: not apart
     bool clear;  // rows of no sequence become zero (else they are left as they were)
 };
 
@@ -84,6 +85,8 @@ struct FarPlan {
     int chunk, slots;
     size_t near_bytes, far_bytes;
 };
+// Bytes of Prompt::head_part, 0 where the heads of a group need not be apart.
+size_t simple_backward_bytes(int dtype, int n_seq, int k_rows, int heads, int kv_heads, int dim);
 FarPlan plan_far(int n_seq, bool packed, int q_rows, int kv_heads, int dim, int window, int sinks);
 int tiles_backward(int dtype, const Prompt &p, cudaStream_t stream);
 int tiles_shared(int dtype, const Cached &c, cudaStream_t stream);

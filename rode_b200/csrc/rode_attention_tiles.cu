@@ -906,7 +906,7 @@ __device__ __forceinline__ bool far_chunks(const Prompt &p, int near, int querie
 // that they never wait for it; what they wait for is dP^T, which must wait for dV and dK of the tile before.
 //
 // The first tile of a sequence has the sinks, which all later queries see: as one CTA it took 4 times as long as the others on 8192 positions with a
-// window of 2048, and the grid waited for it (1436 us instead of RODE_KEYS).  So queries behind the window of the first tile's keys ("far" ones) are cut into chunks of
+// window of 2048, and the grid waited for it (train_long 1436 us, 923 without it).  So queries behind the window of the first tile's keys ("far" ones) are cut into chunks of
 // p.far_chunk for CTAs of their own, which come first in the grid; these and the first tile leave their sums in 32 bits, and add_far_gradients adds
 // them up in order.
 template <typename T, int kDim>

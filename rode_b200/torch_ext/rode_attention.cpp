@@ -163,8 +163,9 @@ std::tuple<Tensor, Tensor, Tensor> window_backward(const Tensor &q_in, const Ten
         dv = empty_on(k.sizes(), q.scalar_type(), q.device());
     }
     size_t bytes = 0;
-    check_status(rode_window_attention_backward_workspace_bytes(s.n, rows, heads, to_int(k.size(1), "key heads"), dim, window_of(window),
-                                                                sinks_of(sinks), &bytes));
+    check_status(rode_window_attention_backward_workspace_bytes(dtype, s.n, rows, to_int(k.size(0), "rows of k"), heads,
+                                                                to_int(k.size(1), "key heads"), dim, window_of(window), sinks_of(sinks),
+                                                                &bytes));
     Tensor ws = empty_on({static_cast<int64_t>(bytes)}, torch::kUInt8, q.device());
     const rode_heads_t qh = rows_heads(q), kh = rows_heads(k), vh = rows_heads(v), gh = rows_heads(dout);
     check_status(rode_window_attention_backward(

@@ -41,7 +41,7 @@ def test_nothing_to_do_needs_no_device(built_library):
 def test_workspaces(built_library):
     lib, need = capi.load(), ctypes.c_size_t(0)
     backward = lambda n_seq, q_rows, out=ctypes.byref(need): lib.rode_window_attention_backward_workspace_bytes(
-        n_seq, q_rows, 4, 2, 64, 4, 1, out)
+        0, n_seq, q_rows, 10, 4, 2, 64, 4, 1, out)
     assert backward(1, 10) == 0 and need.value >= 4 * 10 * 4
     assert backward(1, -1) == BAD and backward(-1, 10) == BAD and backward(1, 10, None) == BAD
     assert backward(0, 10**6) == 0
