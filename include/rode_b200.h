@@ -306,6 +306,8 @@ int rode_sddmm_f32_ordered(int M, int m1, int m2, int n, int k, long long nnz, c
  * whose bases and strides are multiples of 16 bytes, with dim a multiple of 8 up to 128, run on the tensor cores, which round the softmax weights (and,
  * backward, the scores' gradients) to dtype before they multiply.  Rows of an operand at most 2^30.
  *
+ * fp16: scores' gradients beyond 65504 become infinite and those below 2^-25 zero, as gradients in fp16 do; scale the loss.
+ *
  * A query that sees no key gets a zero row.  A non-finite key or value reaches the queries that see it, and may reach other
  * queries of the same sequence (whose weight for it is 0), never another sequence; nothing behind lengths[b] is read.
  * Results do not depend on the order in which thread blocks run.

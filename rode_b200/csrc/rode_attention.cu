@@ -206,8 +206,8 @@ int rode_window_attention_backward(int dtype, int n_seq, const int *q_offsets, c
     RODE_TRY(check_packed(what, n_seq, q_offsets, k_offsets, q_rows, k_rows));
     const bool both = q_rows > 0 && k_rows > 0, keys = dk != nullptr || dv != nullptr;
     RODE_TRY(check_operand(what, "q", q, dtype, q_rows > 0));
-    RODE_TRY(check_operand(what, "k", k, dtype, both));
-    RODE_TRY(check_operand(what, "v", v, dtype, both));
+    RODE_TRY(check_operand(what, "k", k, dtype, both || (keys && k_rows > 0)));
+    RODE_TRY(check_operand(what, "v", v, dtype, both || (keys && k_rows > 0)));
     RODE_TRY(check_operand(what, "dout", dout, dtype, q_rows > 0));
     RODE_TRY(check_result(what, "out", out, q_rows > 0));
     RODE_TRY(check_result(what, "dq", dq, q_rows > 0));
@@ -251,10 +251,12 @@ int rode_window_attention_backward(int dtype, int n_seq, const int *q_offsets, c
     return tiles_backward(dtype, p, stream);
 }
 
-static int check_cached_sizes(const char *what, int batch, int prefix, int capacity) {
+static int check_cached_sizes(const char *what, int batch, int heads, int prefix, int capacity) {
     if (batch < 0 || batch > kMaxRows || prefix < 0 || prefix > kMaxRows || capacity < 0 || capacity > kMaxRows)
         return fail(RODE_ERR_INVALID_ARGUMENT, "%s: batch = %d, prefix = %d and capacity = %d must be 0 to 2^30", what, batch, prefix,
                     capacity);
+    if (static_cast<long long>(batch) * heads > 2147483647ll)
+        return fail(RODE_ERR_INVALID_ARGUMENT, "%s: batch * heads = %lld must be less than 2^31", what, static_cast<long long>(batch) * heads);
     return RODE_OK;
 }
 
@@ -269,7 +271,7 @@ int rode_window_attention_step_workspace_bytes(int dtype, int batch, int capacit
     if (bytes == nullptr) return fail(RODE_ERR_INVALID_ARGUMENT, "%s: null pointer bytes", what);
     RODE_TRY(check_shape(what, dtype, heads, kv_heads, dim, 1.f));
     RODE_TRY(check_window(what, window, sinks));
-    RODE_TRY(check_cached_sizes(what, batch, 0, capacity));
+    RODE_TRY(check_cached_sizes(what, batch, heads, 0, capacity));
     *bytes = plan_parts(dtype, batch, 0, seen_at_most(capacity, window, sinks), heads, kv_heads, dim).bytes;
     return RODE_OK;
 }
@@ -281,7 +283,7 @@ int rode_window_attention_step(int dtype, int batch, int capacity, int heads, in
     const char *what = "rode_window_attention_step";
     RODE_TRY(check_shape(what, dtype, heads, kv_heads, dim, scale));
     RODE_TRY(check_window(what, window, sinks));
-    RODE_TRY(check_cached_sizes(what, batch, 0, capacity));
+    RODE_TRY(check_cached_sizes(what, batch, heads, 0, capacity));
     RODE_TRY(check_operand(what, "q", q, dtype, batch > 0));
     RODE_TRY(check_operand(what, "k_cache", k_cache, dtype, batch > 0 && capacity > 0));
     RODE_TRY(check_operand(what, "v_cache", v_cache, dtype, batch > 0 && capacity > 0));
@@ -308,7 +310,7 @@ int rode_shared_prefix_attention_workspace_bytes(int dtype, int batch, int prefi
     const char *what = "rode_shared_prefix_attention_workspace_bytes";
     if (bytes == nullptr) return fail(RODE_ERR_INVALID_ARGUMENT, "%s: null pointer bytes", what);
     RODE_TRY(check_shape(what, dtype, heads, kv_heads, dim, 1.f));
-    RODE_TRY(check_cached_sizes(what, batch, prefix, capacity));
+    RODE_TRY(check_cached_sizes(what, batch, heads, prefix, capacity));
     *bytes = plan_parts(dtype, batch, prefix, capacity, heads, kv_heads, dim).bytes;
     return RODE_OK;
 }
@@ -320,7 +322,7 @@ int rode_shared_prefix_attention(int dtype, int batch, int prefix, int capacity,
                                  rode_stream_t stream) {
     const char *what = "rode_shared_prefix_attention";
     RODE_TRY(check_shape(what, dtype, heads, kv_heads, dim, scale));
-    RODE_TRY(check_cached_sizes(what, batch, prefix, capacity));
+    RODE_TRY(check_cached_sizes(what, batch, heads, prefix, capacity));
     RODE_TRY(check_operand(what, "q", q, dtype, batch > 0));
     RODE_TRY(check_operand(what, "prefix_k", prefix_k, dtype, batch > 0 && prefix > 0));
     RODE_TRY(check_operand(what, "prefix_v", prefix_v, dtype, batch > 0 && prefix > 0));

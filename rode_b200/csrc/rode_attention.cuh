@@ -2,6 +2,8 @@
 //
 // Query i of a sequence with nq queries and nk keys stands at position p = i + nk - nq (the queries are the last nq positions).
 // It sees key j when j <= p and either j > p - window or j < sinks.
+//
+// Times beside the kernels are of the cases of perf/operators.py that they name, in us a pass or a kernel.
 #pragma once
 
 #include <cuda_bf16.h>

@@ -34,7 +34,9 @@ def rode_window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, win
     positions: with n keys and m queries, query i stands at position ``i + n - m``.  ``window`` at least the longest
     sequence: causal attention.  Rows that belong to no sequence get zeros, in the result and in the gradients.
 
-    ``scale`` multiplies the scores, ``dim ** -0.5`` by default.  Operands whose strides the kernels cannot take are copied."""
+    ``scale`` multiplies the scores, ``dim ** -0.5`` by default.  Operands whose strides the kernels cannot take are copied.
+    In a graph that is being captured, take gradients by ``torch.autograd.grad``, or with leaves that no eager graph holds: torch ties the
+    accumulation into a leaf to the stream of the graph that has seen it first, whatever the operators between."""
     return rode_sddmm_cuda.window_attention(q, k, v, window, sinks, q_offsets, k_offsets, _scale(scale, q))
 
 

@@ -60,6 +60,9 @@ def test_workspaces(built_library):
     assert lib.rode_shared_prefix_attention_workspace_bytes(0, 2, 500, 8, 8, 2, 64, ctypes.byref(need)) == 0 and need.value > 0
     assert lib.rode_shared_prefix_attention(0, 2, 500, 8, 8, 2, 64, 1.0, _heads(), _heads(), _heads(), _heads(), _heads(), 256, 256, 256,
                                             need.value - 1, None) == WS
+    assert lib.rode_window_attention_backward(0, 1, None, None, 0, 8, 4, 2, 64, 4, 0, 1.0, 1, None, None, None, None, None, None, None, 256, 256,
+                                              None, 0, None) == BAD  # keys without queries still need their operands
+    assert lib.rode_window_attention_step_workspace_bytes(0, 2**29, 8, 8, 2, 64, 8, 0, ctypes.byref(need)) == BAD
     assert lib.rode_shared_prefix_attention_workspace_bytes(0, 2, -1, 8, 8, 2, 64, ctypes.byref(need)) == BAD
 
 

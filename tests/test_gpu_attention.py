@@ -234,6 +234,46 @@ def test_only_some_gradients():
     assert torch.equal(b.grad, full["dv"])
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 1e-30])
+def test_scales(scale, dtype):
+    """Scores turned round (the smallest counts most) and all alike."""
+    q_lens = [100, 30]
+    q, k, v, dout = _make(q_lens, q_lens, 4, 2, 64, dtype, seed=14)
+    want = R.packed(q, k, v, q_lens, q_lens, 40, 3, scale, dout)
+    _check(_run(q, k, v, dout, 40, 3, q_offsets=_offsets(q_lens), scale=scale), want)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_rows_of_no_sequence_stay_as_they_were(dtype):
+    """The C entry points with clear = 0: results in front of the first and behind the last sequence keep what they held."""
+    import ctypes
+
+    from rode_b200 import capi
+
+    lib, kind = capi.load(), {torch.float32: capi.RODE_F32, torch.float16: capi.RODE_F16, torch.bfloat16: capi.RODE_BF16}[dtype]
+    q_lens, heads, kv_heads, dim = [50, 90], 4, 2, 64
+    q, k, v, dout = _make(q_lens, q_lens, heads, kv_heads, dim, dtype, seed=15, more_q=37, more_k=37)
+    rows = q.shape[0]
+    want = R.packed(q, k, v, q_lens, q_lens, 30, 2, 0.1, dout, 20, 20)
+    offsets = _offsets(q_lens, 20)
+    out, dq = (torch.full_like(q, 7.0) for _ in range(2))
+    dk, dv = (torch.full_like(k, 7.0) for _ in range(2))
+    lse = torch.empty(heads, rows, device="cuda")
+    need = ctypes.c_size_t(0)
+    capi.check(lib.rode_window_attention_backward_workspace_bytes(kind, 2, rows, rows, heads, kv_heads, dim, 30, 2, ctypes.byref(need)))
+    ws = torch.empty(need.value, dtype=torch.uint8, device="cuda")
+    h = lambda x: ctypes.byref(capi.Heads(x.data_ptr(), 0, x.stride(0), x.stride(1)))
+    stream = torch.cuda.current_stream().cuda_stream or None
+    common = (kind, 2, offsets.data_ptr(), offsets.data_ptr(), rows, rows, heads, kv_heads, dim, 30, 2, 0.1, 0, h(q), h(k), h(v))
+    capi.check(lib.rode_window_attention(*common, out.data_ptr(), lse.data_ptr(), stream))
+    capi.check(lib.rode_window_attention_backward(*common, out.data_ptr(), lse.data_ptr(), h(dout), dq.data_ptr(), dk.data_ptr(),
+                                                  dv.data_ptr(), ws.data_ptr(), need.value, stream))
+    for name, x in (("out", out), ("dq", dq), ("dk", dk), ("dv", dv)):
+        assert bool((x[:20] == 7).all()) and bool((x[160:] == 7).all()), name
+        R.check(x[20:160], tuple(y[20:160] for y in want[name]), name)
+
+
 def test_second_derivative_is_refused():
     from rode_b200.rode_attention import rode_window_attention
 

@@ -191,6 +191,40 @@ def test_prompt_then_tokens_then_samples(dtype):
     R.check(got, _want(sq, sk, sv, lengths, lambda n: list(range(n)), dim ** -0.5, (k, v)))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("scale", [-0.2, 0.0])
+def test_scales(scale, dtype):
+    from rode_b200.rode_attention import rode_shared_prefix_attention, rode_window_attention_step
+
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    lengths = [0, 5, 400]
+    q = _normal(gen, 3, 4, 64, dtype=dtype)
+    k, v = _caches(gen, 3, 400, 2, 64, dtype, "rows")
+    pk, pv = (_normal(gen, 300, 2, 64, dtype=dtype) for _ in range(2))
+    ints = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    R.check(rode_window_attention_step(q, k, v, ints, 90, 3, scale=scale), _want(q, k, v, lengths, _keys(90, 3), scale))
+    R.check(rode_shared_prefix_attention(q, pk, pv, k, v, ints, scale=scale),
+            _want(q, k, v, lengths, lambda n: list(range(n)), scale, (pk, pv)))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("batch,capacity", [(700, 300), (150, 3000), (129, 1000)])
+def test_ragged_batches(batch, capacity, dtype):
+    """Many requests, some without a token, whose blocks are dealt out in equal shares across their borders."""
+    from rode_b200.rode_attention import rode_window_attention_step
+
+    gen = torch.Generator(device="cuda").manual_seed(10)
+    lengths = [(b * 7919) % (capacity + 1) if b % 5 else 0 for b in range(batch)]
+    q = _normal(gen, batch, 6, 64, dtype=dtype)
+    k, v = _caches(gen, batch, capacity, 2, 64, dtype, "rows")
+    ints = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    for window, sinks in ((capacity, 0), (200, 20)):
+        got = rode_window_attention_step(q, k, v, ints, window, sinks)
+        R.check(got, _want(q, k, v, lengths, _keys(window, sinks), 0.125), (window, sinks))
+    short = torch.zeros_like(ints)
+    assert not rode_window_attention_step(q, k, v, short, capacity).any()
+
+
 def test_captured_replayed_and_on_two_streams():
     from rode_b200.rode_attention import rode_shared_prefix_attention, rode_window_attention_step
 
