@@ -6,9 +6,10 @@
 // folded into the queries' products), m' = max(m, max s), the accumulator times 2^(m - m'), plus 2^(s - m') V.
 //
 // A CTA of 256 threads works on 64 rows x 64 keys (32 x 32 at head dimensions above 128, where the operands' tiles would not fit
-// the shared memory); a thread holds 4 x 4 scores and 4 rows x dim / 16 columns of the result, so that eight 16-byte
-// loads from shared memory feed 64 FMAs.  Rows of shared memory are 4 floats longer than the tile: eight threads that read one
-// column of eight keys hit different banks.
+// the shared memory; at all of them, cases of fewer tiles than SMs gain 10 to 25 %, larger ones lose up to 16 %); a thread holds 4 x 4 scores and 4 rows x
+// dim / 16 columns of the result, so that eight 16-byte loads from shared memory feed 64 FMAs (32 instructions, two at once).  Rows of shared memory are 4
+// floats longer than the tile: eight threads that read one column of eight keys hit different banks.  Bound by the loads from shared memory (7600
+// wavefronts per block of 64 x 64 x 80, forward) and, in small cases, by the SMs that get two tiles.
 #include <algorithm>
 #include <type_traits>
 
@@ -661,7 +662,7 @@ __device__ __forceinline__ void join_parts_of_row(T *out, int dim, int parts, Ls
 // the result, most of which have no pieces, took 13 us behind step_batch.)
 template <typename T>
 __global__ void __launch_bounds__(128) join_pieces(Cached c) {
-    const int group = c.win.heads / c.win.kv_heads, chunks = (group + c.chunk - 1) / c.chunk, per = c.win.kv_heads * chunks;
+    const int group = c.win.heads / c.win.kv_heads, chunks = (group + c.chunk - 1) / c.chunk;
     const Share share = find_share(c, true);
     const float *piece_lse = after_chain(c.piece_lse), *piece_out = after_chain(c.piece_out);
     if (share.begin >= share.end) return;
