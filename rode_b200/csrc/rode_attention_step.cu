@@ -19,7 +19,7 @@
 namespace rode {
 namespace {
 
-constexpr int kWarps = 4, kQueries = kTensorCoreChunk, kKeys = 16;
+constexpr int kWarps = 4, kQueries = kTensorCoreChunk;
 
 template <typename T>
 __device__ __forceinline__ void small_product(float (&d)[4], const uint32_t a0, const uint32_t a1, const uint32_t a2, const uint32_t a3,

@@ -107,7 +107,8 @@ def test_sinks_seen_from_far(case, dim, dtype):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("heads,kv_heads,dim", [(1, 1, 4), (3, 1, 20), (6, 3, 40), (8, 1, 80), (5, 5, 96), (4, 2, 100), (2, 2, 16),
-                                                (16, 2, 120), (2, 1, 132), (4, 2, 256)])
+                                                (16, 2, 120), (2, 1, 132), (4, 2, 256), (128, 1, 64), (130, 1, 64), (48, 1, 128),
+                                                (65, 1, 88)])
 def test_head_layouts(heads, kv_heads, dim, dtype):
     q_lens = [70, 200]
     q, k, v, dout = _make(q_lens, q_lens, heads, kv_heads, dim, dtype, seed=1)
@@ -369,3 +370,29 @@ def test_from_a_thread_without_a_context():
         t.join()
     torch.cuda.synchronize()
     assert len(got) == 2 and all(torch.equal(x, want["out"]) for x in got)
+
+
+def test_two_host_threads_at_once():
+    """Calls from two host threads, each on a stream of its own."""
+    import threading
+
+    q_lens = [300, 200]
+    sets = [_make(q_lens, q_lens, 4, 2, dim, torch.bfloat16, seed=16 + dim) for dim in (64, 128)]
+    offsets = _offsets(q_lens)
+    want = [_run(*x, 100, 4, q_offsets=offsets) for x in sets]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got = _run(*sets[i], 100, 4, q_offsets=offsets)
+                torch.cuda.current_stream().synchronize()
+                bad.extend(n for n in got if not torch.equal(got[n], want[i][n]))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad

@@ -62,7 +62,7 @@ def _keys(window, sinks):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("layout", ["rows", "heads_first", "tokens_first", "gaps", "odd_rows"])
-@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 2, 64), (8, 8, 128), (16, 1, 128), (12, 4, 96), (33, 3, 64), (2, 1, 20), (4, 2, 256)])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 2, 64), (8, 8, 128), (16, 1, 128), (12, 4, 96), (33, 3, 64), (130, 1, 64), (2, 1, 20), (4, 2, 256)])
 def test_step(heads, kv_heads, dim, layout, dtype):
     gen = torch.Generator(device="cuda").manual_seed(1)
     capacity, lengths = 300, [0, 1, 2, 31, 32, 33, 100, 299, 300, 64, 7, 250]
@@ -137,7 +137,7 @@ def test_lengths_that_lie():
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("batch,prefix,heads,kv_heads,dim", [(1, 1, 4, 2, 64), (3, 777, 8, 2, 64), (40, 300, 8, 2, 128), (5, 0, 4, 4, 64),
                                                              (130, 129, 4, 4, 96), (2, 5000, 12, 1, 128), (7, 100, 6, 2, 20), (3, 130, 2, 1, 256),
-                                                             (17, 2500, 24, 3, 72)])
+                                                             (17, 2500, 24, 3, 72), (2, 400, 130, 1, 64), (3, 1000, 128, 1, 128)])
 def test_shared_prefix(batch, prefix, heads, kv_heads, dim, dtype):
     from rode_b200.rode_attention import rode_shared_prefix_attention
 
