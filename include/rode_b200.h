@@ -326,24 +326,27 @@ typedef struct {
  * when j <= p and (p - j < window or j < sinks).
  *   q [q_rows, heads, dim], k and v [k_rows, kv_heads, dim]   .batch is not used
  *   out  [q_rows, heads, dim] contiguous
+ *   out_rest  what rounding to dtype took from out, in dtype and of out's shape, for the backward call; may be null (fp32 has none)
  *   lse  float[heads, q_rows], natural logarithm of the softmax sums (-inf for a query that sees no key); may be null
  *   clear  1: rows of out (of the gradients) that belong to no sequence become zero; 0: they are left as they were
  */
 int rode_window_attention(int dtype, int n_seq, const int *q_offsets, const int *k_offsets, int q_rows, int k_rows,
                           int heads, int kv_heads, int dim, int window, int sinks, float scale, int clear,
-                          const rode_heads_t *q, const rode_heads_t *k, const rode_heads_t *v, void *out, float *lse,
-                          rode_stream_t stream);
+                          const rode_heads_t *q, const rode_heads_t *k, const rode_heads_t *v, void *out, void *out_rest,
+                          float *lse, rode_stream_t stream);
 
 /* Its gradients: dq [q_rows, heads, dim], dk and dv [k_rows, kv_heads, dim] contiguous, dk and dv both or neither (null).
- * out and lse are what the forward call wrote.  workspace: rode_window_attention_backward_workspace_bytes() bytes,
+ * out, out_rest and lse are what the forward call wrote; without out_rest (null) dq and dk are less exact where queries see few keys.
+ *  workspace: rode_window_attention_backward_workspace_bytes() bytes,
  * 16-byte aligned, not shared by calls that may overlap in time. */
 int rode_window_attention_backward_workspace_bytes(int dtype, int n_seq, int q_rows, int k_rows, int heads, int kv_heads,
                                                    int dim, int window, int sinks, size_t *bytes);
 int rode_window_attention_backward(int dtype, int n_seq, const int *q_offsets, const int *k_offsets, int q_rows,
                                    int k_rows, int heads, int kv_heads, int dim, int window, int sinks, float scale,
                                    int clear, const rode_heads_t *q, const rode_heads_t *k, const rode_heads_t *v,
-                                   const void *out, const float *lse, const rode_heads_t *dout, void *dq, void *dk,
-                                   void *dv, void *workspace, size_t workspace_bytes, rode_stream_t stream);
+                                   const void *out, const void *out_rest, const float *lse, const rode_heads_t *dout,
+                                   void *dq, void *dk, void *dv, void *workspace, size_t workspace_bytes,
+                                   rode_stream_t stream);
 
 /* The same pattern for one new token per sequence against a cache: request b's query (q [batch, heads, dim], .row is not
  * used) stands at position lengths[b] - 1 of its cache (k_cache, v_cache [batch, capacity, kv_heads, dim]), whose rows from

@@ -109,9 +109,9 @@ def load() -> ctypes.CDLL:
     lib.rode_sddmm_workspace_bytes.argtypes = [ci, ci, ctypes.c_longlong, ctypes.POINTER(sz)]
     lib.rode_sddmm_f32_ordered.argtypes = [ci, ci, ci, ci, ci, ctypes.c_longlong] + [vp] * 10 + [sz, vp, vp]
     cf, heads = ctypes.c_float, ctypes.POINTER(Heads)
-    lib.rode_window_attention.argtypes = [ci, ci, vp, vp] + [ci] * 7 + [cf, ci] + [heads] * 3 + [vp] * 3
+    lib.rode_window_attention.argtypes = [ci, ci, vp, vp] + [ci] * 7 + [cf, ci] + [heads] * 3 + [vp] * 4
     lib.rode_window_attention_backward_workspace_bytes.argtypes = [ci] * 9 + [ctypes.POINTER(sz)]
-    lib.rode_window_attention_backward.argtypes = ([ci, ci, vp, vp] + [ci] * 7 + [cf, ci] + [heads] * 3 + [vp, vp, heads]
+    lib.rode_window_attention_backward.argtypes = ([ci, ci, vp, vp] + [ci] * 7 + [cf, ci] + [heads] * 3 + [vp] * 3 + [heads]
                                                    + [vp] * 4 + [sz, vp])
     lib.rode_window_attention_step_workspace_bytes.argtypes = [ci] * 8 + [ctypes.POINTER(sz)]
     lib.rode_window_attention_step.argtypes = [ci] * 8 + [cf] + [heads] * 3 + [vp] * 3 + [sz, vp]

@@ -154,8 +154,8 @@ extern "C" {
 
 int rode_window_attention(int dtype, int n_seq, const int *q_offsets, const int *k_offsets, int q_rows, int k_rows,
                           int heads, int kv_heads, int dim, int window, int sinks, float scale, int clear,
-                          const rode_heads_t *q, const rode_heads_t *k, const rode_heads_t *v, void *out, float *lse,
-                          rode_stream_t stream) {
+                          const rode_heads_t *q, const rode_heads_t *k, const rode_heads_t *v, void *out, void *out_rest,
+                          float *lse, rode_stream_t stream) {
     const char *what = "rode_window_attention";
     RODE_TRY(check_shape(what, dtype, heads, kv_heads, dim, scale));
     RODE_TRY(check_window(what, window, sinks));
@@ -164,6 +164,7 @@ int rode_window_attention(int dtype, int n_seq, const int *q_offsets, const int 
     RODE_TRY(check_operand(what, "k", k, dtype, q_rows > 0 && k_rows > 0));
     RODE_TRY(check_operand(what, "v", v, dtype, q_rows > 0 && k_rows > 0));
     RODE_TRY(check_result(what, "out", out, q_rows > 0));
+    RODE_TRY(check_result(what, "out_rest", out_rest, out_rest != nullptr));
     if (q_rows == 0) return RODE_OK;
     Prompt p = {};
     p.seqs = {q_offsets, k_offsets, n_seq, q_rows, k_rows};
@@ -174,6 +175,7 @@ int rode_window_attention(int dtype, int n_seq, const int *q_offsets, const int 
         p.v = *v;
     }
     p.out = out;
+    p.rest = dtype == RODE_F32 ? nullptr : out_rest;
     p.lse = lse;
     p.clear = clear != 0;
     return tiles_take_prompt(dtype, p) ? tiles_prompt(dtype, p, stream) : simple_prompt(dtype, p, stream);
@@ -198,8 +200,9 @@ int rode_window_attention_backward_workspace_bytes(int dtype, int n_seq, int q_r
 int rode_window_attention_backward(int dtype, int n_seq, const int *q_offsets, const int *k_offsets, int q_rows,
                                    int k_rows, int heads, int kv_heads, int dim, int window, int sinks, float scale,
                                    int clear, const rode_heads_t *q, const rode_heads_t *k, const rode_heads_t *v,
-                                   const void *out, const float *lse, const rode_heads_t *dout, void *dq, void *dk,
-                                   void *dv, void *workspace, size_t workspace_bytes, rode_stream_t stream) {
+                                   const void *out, const void *out_rest, const float *lse, const rode_heads_t *dout,
+                                   void *dq, void *dk, void *dv, void *workspace, size_t workspace_bytes,
+                                   rode_stream_t stream) {
     const char *what = "rode_window_attention_backward";
     RODE_TRY(check_shape(what, dtype, heads, kv_heads, dim, scale));
     RODE_TRY(check_window(what, window, sinks));
@@ -210,6 +213,7 @@ int rode_window_attention_backward(int dtype, int n_seq, const int *q_offsets, c
     RODE_TRY(check_operand(what, "v", v, dtype, both || (keys && k_rows > 0)));
     RODE_TRY(check_operand(what, "dout", dout, dtype, q_rows > 0));
     RODE_TRY(check_result(what, "out", out, q_rows > 0));
+    RODE_TRY(check_result(what, "out_rest", out_rest, out_rest != nullptr));
     RODE_TRY(check_result(what, "dq", dq, q_rows > 0));
     RODE_TRY(check_result(what, "dk", dk, keys && k_rows > 0));
     RODE_TRY(check_result(what, "dv", dv, keys && k_rows > 0));
@@ -230,6 +234,7 @@ int rode_window_attention_backward(int dtype, int n_seq, const int *q_offsets, c
         p.v = *v;
     }
     p.out = const_cast<void *>(out);
+    p.rest = dtype == RODE_F32 ? nullptr : const_cast<void *>(out_rest);
     p.lse = const_cast<float *>(lse);
     p.dq = dq;
     p.dk = dk;

@@ -41,6 +41,7 @@ struct Prompt {
     Window win;
     rode_heads_t q, k, v, dout;
     void *out;
+    void *rest;  // what rounding took from out, in the same type; may be null
     float *lse;
     void *dq, *dk, *dv;
     float *delta;

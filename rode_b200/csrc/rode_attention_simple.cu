@@ -210,8 +210,13 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_rows(Prompt p) {
 #pragma unroll
         for (int c = 0; c < kDim / 64; ++c) {
             const int d = (tx + 16 * c) * 4;
-            if (d < w.dim)
-                store4(out + d, make_float4(acc[i][c].x * inv, acc[i][c].y * inv, acc[i][c].z * inv, acc[i][c].w * inv));
+            if (d >= w.dim) continue;
+            const float4 x = make_float4(acc[i][c].x * inv, acc[i][c].y * inv, acc[i][c].z * inv, acc[i][c].w * inv);
+            store4(out + d, x);
+            if (p.rest != nullptr)
+                store4(static_cast<T *>(p.rest) + ((row0 + r) * w.heads + head) * w.dim + d,
+                       make_float4(x.x - to_float(from_float<T>(x.x)), x.y - to_float(from_float<T>(x.y)),
+                                   x.z - to_float(from_float<T>(x.z)), x.w - to_float(from_float<T>(x.w))));
         }
         if (tx == 0 && p.lse != nullptr)
             p.lse[static_cast<long long>(head) * p.seqs.q_rows + row0 + r] = m[i] == -INFINITY ? -INFINITY : (m[i] + log2f(l[i])) * kLn2;
@@ -326,7 +331,9 @@ __global__ void __launch_bounds__(kThreads) query_gradients(Prompt p) {
         if (r < have) {
             const T *o = static_cast<const T *>(p.out) + ((row0 + r) * w.heads + head) * w.dim;
             for (int d = tx * 4; d < w.dim; d += 64) {
-                const float4 x = load4(o + d), g = *reinterpret_cast<const float4 *>(gs + r * (kDim + 4) + d);
+                float4 x = load4(o + d);
+                const float4 g = *reinterpret_cast<const float4 *>(gs + r * (kDim + 4) + d);
+                if (p.rest != nullptr) vadd(x, load4(static_cast<const T *>(p.rest) + ((row0 + r) * w.heads + head) * w.dim + d));
                 sum += x.x * g.x + x.y * g.y + x.z * g.z + x.w * g.w;
             }
         }

@@ -181,6 +181,13 @@ constexpr int kTileThreads = 384;
 __device__ __forceinline__ void take_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 216;"); }
 __device__ __forceinline__ void give_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 72;"); }
 
+// What rounding to `rounded` took from two numbers.
+template <typename T>
+__device__ __forceinline__ uint32_t rest2(float a, float b, uint32_t rounded) {
+    const T *t = reinterpret_cast<const T *>(&rounded);
+    return pack2<T>(a - to_float(t[0]), b - to_float(t[1]));
+}
+
 // kShared: rows are requests, keys a part of the prefix, results go to the parts; else prompts.
 template <typename T, int kDim, bool kShared>
 __global__ void __launch_bounds__(kTileThreads, 1)
@@ -523,6 +530,16 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                             y.w = pack2<T>(__uint_as_float(o[j + 6]) * inv, __uint_as_float(o[j + 7]) * inv);
                         }
                         if (mine && x + j < w.dim) *reinterpret_cast<uint4 *>(out + x + j) = y;
+                        if (p.rest != nullptr) {
+                            uint4 z = make_uint4(0, 0, 0, 0);
+                            if (done > 0) {
+                                z.x = rest2<T>(__uint_as_float(o[j]) * inv, __uint_as_float(o[j + 1]) * inv, y.x);
+                                z.y = rest2<T>(__uint_as_float(o[j + 2]) * inv, __uint_as_float(o[j + 3]) * inv, y.y);
+                                z.z = rest2<T>(__uint_as_float(o[j + 4]) * inv, __uint_as_float(o[j + 5]) * inv, y.z);
+                                z.w = rest2<T>(__uint_as_float(o[j + 6]) * inv, __uint_as_float(o[j + 7]) * inv, y.w);
+                            }
+                            if (mine && x + j < w.dim) *reinterpret_cast<uint4 *>(static_cast<T *>(p.rest) + (out - static_cast<T *>(p.out)) + x + j) = z;
+                        }
                     }
                 }
             }
@@ -557,7 +574,9 @@ struct GradientMaps {
     CUtensorMap q, dout, k, v;
 };
 
-// delta = do . o of all rows, a lane per 16 bytes.  (By two spare warps of the kernel below it took as long as three blocks of keys, more than short windows
+// delta = do . o of all rows, a lane per 16 bytes, with what rounding took from o: in rows of few keys dP - delta cancels, and the rounding
+// of o counted as much as that of the result (fp16, sequences of some tens of rows: dQ 0.00042 off instead of 0.0003; writing and reading it costs 70 us of
+// train_long's 2430).  (By two spare warps of the kernel below it took as long as three blocks of keys, more than short windows
 // have; here 41 us of train_long's 2400.)
 template <typename T, int kDim>
 __global__ void __launch_bounds__(256) row_deltas(const Prompt p) {
@@ -571,9 +590,11 @@ __global__ void __launch_bounds__(256) row_deltas(const Prompt p) {
     if (i < rows && d < dim) {
         const uint4 x = __ldg(reinterpret_cast<const uint4 *>(row_of<T>(p.dout, 0, row, head) + d));
         const uint4 y = __ldg(reinterpret_cast<const uint4 *>(static_cast<const T *>(p.out) + i * dim + d));
-        const T *s = reinterpret_cast<const T *>(&x), *t = reinterpret_cast<const T *>(&y);
+        uint4 z = make_uint4(0, 0, 0, 0);
+        if (p.rest != nullptr) z = __ldg(reinterpret_cast<const uint4 *>(static_cast<const T *>(p.rest) + i * dim + d));
+        const T *s = reinterpret_cast<const T *>(&x), *t = reinterpret_cast<const T *>(&y), *rest = reinterpret_cast<const T *>(&z);
 #pragma unroll
-        for (int u = 0; u < 8; ++u) sum = fmaf(to_float(s[u]), to_float(t[u]), sum);
+        for (int u = 0; u < 8; ++u) sum = fmaf(to_float(s[u]), to_float(t[u]) + to_float(rest[u]), sum);
     }
 #pragma unroll
     for (int o = kLanes / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);

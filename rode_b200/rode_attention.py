@@ -35,6 +35,7 @@ def rode_window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, win
     sequence: causal attention.  Rows that belong to no sequence get zeros, in the result and in the gradients.
 
     ``scale`` multiplies the scores, ``dim ** -0.5`` by default.  Operands whose strides the kernels cannot take are copied.
+    For the backward pass a call keeps its operands, its result, in 16-bit types one more array of the result's size, and a float per row and head.
     In a graph that is being captured, take gradients by ``torch.autograd.grad``, or with leaves that no eager graph holds: torch ties the
     accumulation into a leaf to the stream of the graph that has seen it first, whatever the operators between."""
     return rode_sddmm_cuda.window_attention(q, k, v, window, sinks, q_offsets, k_offsets, _scale(scale, q))

@@ -124,7 +124,8 @@ void check_prompt(const Tensor &q, const Tensor &k, const Tensor &v) {
     TORCH_CHECK_VALUE(k.size(2) == q.size(2), "k must have the head dimension of q, got ", k.size(2), " and ", q.size(2));
 }
 
-std::tuple<Tensor, Tensor> window_forward(const Tensor &q_in, const Tensor &k_in, const Tensor &v_in, int64_t window,
+// With want_lse (for the backward call): the result, what rounding took from it (16-bit types), the logarithms of the sums.
+std::tuple<Tensor, Tensor, Tensor> window_forward(const Tensor &q_in, const Tensor &k_in, const Tensor &v_in, int64_t window,
                                                       int64_t sinks, const OptionalTensor &q_offsets,
                                                       const OptionalTensor &k_offsets, double scale, bool want_lse) {
     check_prompt(q_in, k_in, v_in);
@@ -134,20 +135,21 @@ std::tuple<Tensor, Tensor> window_forward(const Tensor &q_in, const Tensor &k_in
     const Tensor q = fitting(q_in), k = fitting(k_in), v = fitting(v_in);
     const int rows = to_int(q.size(0), "rows of q"), heads = to_int(q.size(1), "heads"), dim = to_int(q.size(2), "dim");
     Tensor out = empty_on(q.sizes(), q.scalar_type(), q.device());
-    Tensor lse;
+    Tensor lse, rest;
+    if (want_lse && dtype != RODE_F32) rest = empty_on(q.sizes(), q.scalar_type(), q.device());
     if (want_lse) lse = empty_on({heads, rows}, torch::kFloat32, q.device());
     const rode_heads_t qh = rows_heads(q), kh = rows_heads(k), vh = rows_heads(v);
     check_status(rode_window_attention(dtype, s.n, s.q, s.k, rows, to_int(k.size(0), "rows of k"), heads,
                                        to_int(k.size(1), "key heads"), dim, window_of(window), sinks_of(sinks),
                                        static_cast<float>(scale), 1, &qh, &kh, &vh, out.data_ptr(),
-                                       want_lse ? lse.data_ptr<float>() : nullptr,
+                                       rest.defined() ? rest.data_ptr() : nullptr, want_lse ? lse.data_ptr<float>() : nullptr,
                                        at::cuda::getCurrentCUDAStream(q.device().index()).stream()));
-    return {out, lse};
+    return {out, rest, lse};
 }
 
-// out and lse are window_forward's.
+// out, rest and lse are window_forward's.
 std::tuple<Tensor, Tensor, Tensor> window_backward(const Tensor &q_in, const Tensor &k_in, const Tensor &v_in, const Tensor &out,
-                                                    const Tensor &lse, const Tensor &dout_in, int64_t window, int64_t sinks,
+                                                    const Tensor &rest, const Tensor &lse, const Tensor &dout_in, int64_t window, int64_t sinks,
                                                     const OptionalTensor &q_offsets, const OptionalTensor &k_offsets, double scale,
                                                     bool want_keys) {
     const int dtype = dtype_of(q_in);
@@ -170,7 +172,8 @@ std::tuple<Tensor, Tensor, Tensor> window_backward(const Tensor &q_in, const Ten
     const rode_heads_t qh = rows_heads(q), kh = rows_heads(k), vh = rows_heads(v), gh = rows_heads(dout);
     check_status(rode_window_attention_backward(
         dtype, s.n, s.q, s.k, rows, to_int(k.size(0), "rows of k"), heads, to_int(k.size(1), "key heads"), dim, window_of(window),
-        sinks_of(sinks), static_cast<float>(scale), 1, &qh, &kh, &vh, out.data_ptr(), lse.data_ptr<float>(), &gh, dq.data_ptr(),
+        sinks_of(sinks), static_cast<float>(scale), 1, &qh, &kh, &vh, out.data_ptr(), rest.defined() ? rest.data_ptr() : nullptr,
+        lse.data_ptr<float>(), &gh, dq.data_ptr(),
         want_keys ? dk.data_ptr() : nullptr, want_keys ? dv.data_ptr() : nullptr, ws.data_ptr(), bytes,
         at::cuda::getCurrentCUDAStream(q.device().index()).stream()));
     return {dq, dk, dv};
@@ -182,8 +185,8 @@ OptionalTensor given(const Tensor &x) { return x.defined() ? OptionalTensor(x) :
 struct WindowAttention : torch::autograd::Function<WindowAttention> {
     static Tensor forward(torch::autograd::AutogradContext *ctx, const Tensor &q, const Tensor &k, const Tensor &v, int64_t window,
                           int64_t sinks, const OptionalTensor &q_offsets, const OptionalTensor &k_offsets, double scale) {
-        auto [out, lse] = window_forward(q, k, v, window, sinks, q_offsets, k_offsets, scale, true);
-        ctx->save_for_backward({q, k, v, out, lse, q_offsets.value_or(Tensor()), k_offsets.value_or(Tensor())});
+        auto [out, rest, lse] = window_forward(q, k, v, window, sinks, q_offsets, k_offsets, scale, true);
+        ctx->save_for_backward({q, k, v, out, rest, lse, q_offsets.value_or(Tensor()), k_offsets.value_or(Tensor())});
         ctx->saved_data["window"] = window;
         ctx->saved_data["sinks"] = sinks;
         ctx->saved_data["scale"] = scale;
@@ -196,8 +199,8 @@ struct WindowAttention : torch::autograd::Function<WindowAttention> {
         {
             const torch::NoGradGuard guard;
             std::tie(grads[0], grads[1], grads[2]) =
-                window_backward(saved[0], saved[1], saved[2], saved[3], saved[4], dout[0], ctx->saved_data["window"].toInt(),
-                                ctx->saved_data["sinks"].toInt(), given(saved[5]), given(saved[6]), ctx->saved_data["scale"].toDouble(),
+                window_backward(saved[0], saved[1], saved[2], saved[3], saved[4], saved[5], dout[0], ctx->saved_data["window"].toInt(),
+                                ctx->saved_data["sinks"].toInt(), given(saved[6]), given(saved[7]), ctx->saved_data["scale"].toDouble(),
                                 ctx->needs_input_grad(1) || ctx->needs_input_grad(2));
         }
         if (twice) {  // the gradients themselves have none: an error when somebody asks for it

@@ -16,14 +16,14 @@ def _heads(data=256, batch=0, row=256, head=64):
 
 
 def _forward(lib, dtype=capi.RODE_F32, n_seq=1, qo=None, ko=None, q_rows=8, k_rows=8, heads=4, kv_heads=2, dim=64, window=4, sinks=0,
-             scale=1.0, q=None, k=None, out=256):
+             scale=1.0, q=None, k=None, out=256, rest=None):
     return lib.rode_window_attention(dtype, n_seq, qo, ko, q_rows, k_rows, heads, kv_heads, dim, window, sinks, scale, 1, q or _heads(),
-                                     k or _heads(), _heads(), out, None, None)
+                                     k or _heads(), _heads(), out, rest, None, None)
 
 
 @pytest.mark.parametrize("bad", [dict(dtype=7), dict(n_seq=2), dict(qo=256), dict(qo=256, ko=256, n_seq=-1), dict(q_rows=-1),
                                  dict(k_rows=2**30 + 1), dict(heads=3), dict(heads=0), dict(kv_heads=0), dict(dim=0), dict(dim=6),
-                                 dict(dim=260), dict(window=0), dict(sinks=-1), dict(scale=float("nan")), dict(out=None), dict(out=8),
+                                 dict(dim=260), dict(window=0), dict(sinks=-1), dict(scale=float("nan")), dict(out=None), dict(out=8), dict(rest=8),
                                  dict(q=_heads(data=None)), dict(q=_heads(data=8)), dict(k=_heads(row=-4)), dict(k=_heads(head=6)),
                                  dict(heads=70000, kv_heads=1)])
 def test_window_attention_refuses(built_library, bad):
@@ -46,7 +46,7 @@ def test_workspaces(built_library):
     assert backward(1, -1) == BAD and backward(-1, 10) == BAD and backward(1, 10, None) == BAD
     assert backward(0, 10**6) == 0
     back = lambda ws, n, dk=256, dv=256: lib.rode_window_attention_backward(
-        0, 1, None, None, 8, 8, 4, 2, 64, 4, 0, 1.0, 1, _heads(), _heads(), _heads(), 256, 256, _heads(), 256, dk, dv, ws, n, None)
+        0, 1, None, None, 8, 8, 4, 2, 64, 4, 0, 1.0, 1, _heads(), _heads(), _heads(), 256, None, 256, _heads(), 256, dk, dv, ws, n, None)
     assert back(None, 0) == WS and back(256, 8) == WS and back(264, 1 << 20) == WS
     assert back(256, 1 << 20, dk=None) == BAD and back(256, 1 << 20, dv=None) == BAD
     for batch, capacity, window, sinks in ((1, 100000, 100000, 0), (2, 5000, 3000, 4)):
@@ -60,7 +60,7 @@ def test_workspaces(built_library):
     assert lib.rode_shared_prefix_attention_workspace_bytes(0, 2, 500, 8, 8, 2, 64, ctypes.byref(need)) == 0 and need.value > 0
     assert lib.rode_shared_prefix_attention(0, 2, 500, 8, 8, 2, 64, 1.0, _heads(), _heads(), _heads(), _heads(), _heads(), 256, 256, 256,
                                             need.value - 1, None) == WS
-    assert lib.rode_window_attention_backward(0, 1, None, None, 0, 8, 4, 2, 64, 4, 0, 1.0, 1, None, None, None, None, None, None, None, 256, 256,
+    assert lib.rode_window_attention_backward(0, 1, None, None, 0, 8, 4, 2, 64, 4, 0, 1.0, 1, None, None, None, None, None, None, None, None, 256, 256,
                                               None, 0, None) == BAD  # keys without queries still need their operands
     assert lib.rode_window_attention_step_workspace_bytes(0, 2**29, 8, 8, 2, 64, 8, 0, ctypes.byref(need)) == BAD
     assert lib.rode_shared_prefix_attention_workspace_bytes(0, 2, -1, 8, 8, 2, 64, ctypes.byref(need)) == BAD

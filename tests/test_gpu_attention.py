@@ -258,7 +258,7 @@ def test_rows_of_no_sequence_stay_as_they_were(dtype):
     rows = q.shape[0]
     want = R.packed(q, k, v, q_lens, q_lens, 30, 2, 0.1, dout, 20, 20)
     offsets = _offsets(q_lens, 20)
-    out, dq = (torch.full_like(q, 7.0) for _ in range(2))
+    out, dq, rest = (torch.full_like(q, 7.0) for _ in range(3))
     dk, dv = (torch.full_like(k, 7.0) for _ in range(2))
     lse = torch.empty(heads, rows, device="cuda")
     need = ctypes.c_size_t(0)
@@ -267,12 +267,21 @@ def test_rows_of_no_sequence_stay_as_they_were(dtype):
     h = lambda x: ctypes.byref(capi.Heads(x.data_ptr(), 0, x.stride(0), x.stride(1)))
     stream = torch.cuda.current_stream().cuda_stream or None
     common = (kind, 2, offsets.data_ptr(), offsets.data_ptr(), rows, rows, heads, kv_heads, dim, 30, 2, 0.1, 0, h(q), h(k), h(v))
-    capi.check(lib.rode_window_attention(*common, out.data_ptr(), lse.data_ptr(), stream))
-    capi.check(lib.rode_window_attention_backward(*common, out.data_ptr(), lse.data_ptr(), h(dout), dq.data_ptr(), dk.data_ptr(),
+    capi.check(lib.rode_window_attention(*common, out.data_ptr(), rest.data_ptr(), lse.data_ptr(), stream))
+    capi.check(lib.rode_window_attention_backward(*common, out.data_ptr(), rest.data_ptr(), lse.data_ptr(), h(dout), dq.data_ptr(), dk.data_ptr(),
                                                   dv.data_ptr(), ws.data_ptr(), need.value, stream))
     for name, x in (("out", out), ("dq", dq), ("dk", dk), ("dv", dv)):
         assert bool((x[:20] == 7).all()) and bool((x[160:] == 7).all()), name
         R.check(x[20:160], tuple(y[20:160] for y in want[name]), name)
+    assert bool((rest[:20] == 7).all()) and bool((rest[160:] == 7).all())
+    if dtype != torch.float32:  # the rest: at most half a step of the result
+        step = torch.finfo(dtype).eps * out[20:160].double().abs() + 2.0 ** -24
+        assert bool((rest[20:160].double().abs() <= step).all()) and bool(rest[20:160].any())
+    else:
+        assert bool((rest == 7).all())
+    capi.check(lib.rode_window_attention_backward(*common, out.data_ptr(), None, lse.data_ptr(), h(dout), dq.data_ptr(), dk.data_ptr(),
+                                                  dv.data_ptr(), ws.data_ptr(), need.value, stream))
+    R.check(dq[20:160], tuple(y[20:160] for y in want["dq"]), "dq without the rest")
 
 
 def test_second_derivative_is_refused():
