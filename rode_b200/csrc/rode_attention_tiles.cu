@@ -576,8 +576,8 @@ struct GradientMaps {
 
 // delta = do . o of all rows, a lane per 16 bytes, with what rounding took from o: in rows of few keys dP - delta cancels, and the rounding
 // of o counted as much as that of the result (fp16, sequences of some tens of rows: dQ 0.00042 off instead of 0.0003; writing and reading it costs 70 us of
-// train_long's 2430).  (By two spare warps of the kernel below it took as long as three blocks of keys, more than short windows
-// have; here 41 us of train_long's 2400.)
+// train_long's 2459).  (By two spare warps of the kernel below it took as long as three blocks of keys, more than short windows
+// have.)
 template <typename T, int kDim>
 __global__ void __launch_bounds__(256) row_deltas(const Prompt p) {
     constexpr int kLanes = kDim / 8;
