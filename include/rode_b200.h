@@ -324,6 +324,7 @@ typedef struct {
  * k_offsets[s] .. k_offsets[s+1] of k and v (int32[n_seq+1] on the device, not decreasing; both null: one sequence of all
  * rows).  Its queries are its last positions: query i stands at p = i + keys - queries and sees key j
  * when j <= p and (p - j < window or j < sinks).
+ *   window at least 1, sinks at least 0, each up to INT_MAX (no window; all keys)
  *   q [q_rows, heads, dim], k and v [k_rows, kv_heads, dim]   .batch is not used
  *   out  [q_rows, heads, dim] contiguous
  *   out_rest  what rounding to dtype took from out, in dtype and of out's shape, for the backward call; may be null (fp32 has none)

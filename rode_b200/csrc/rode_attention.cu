@@ -28,6 +28,12 @@ int check_window(const char *what, int window, int sinks) {
     return RODE_OK;
 }
 
+// No operand has more rows than this, so that larger windows (INT_MAX for "no window") and more sinks say the same; and a position (at most 2^30 on either
+// side of 0) plus or minus a window stays within 32 bits, as the kernels need it.
+Window window_of(int window, int sinks, int heads, int kv_heads, int dim, float scale) {
+    return {std::min(window, kMaxRows), std::min(sinks, kMaxRows), heads, kv_heads, dim, scale};
+}
+
 size_t element_bytes(int dtype) { return dtype == RODE_F32 ? 4 : 2; }
 
 // Elements (of a power of two) that the base and all strides are multiples of, at most `most`.
@@ -168,7 +174,7 @@ int rode_window_attention(int dtype, int n_seq, const int *q_offsets, const int 
     if (q_rows == 0) return RODE_OK;
     Prompt p = {};
     p.seqs = {q_offsets, k_offsets, n_seq, q_rows, k_rows};
-    p.win = {window, sinks, heads, kv_heads, dim, scale};
+    p.win = window_of(window, sinks, heads, kv_heads, dim, scale);
     p.q = *q;
     if (k_rows > 0) {
         p.k = *k;
@@ -224,7 +230,7 @@ int rode_window_attention_backward(int dtype, int n_seq, const int *q_offsets, c
     if (q_rows == 0 && (k_rows == 0 || !keys)) return RODE_OK;
     Prompt p = {};
     p.seqs = {q_offsets, k_offsets, n_seq, q_rows, k_rows};
-    p.win = {window, sinks, heads, kv_heads, dim, scale};
+    p.win = window_of(window, sinks, heads, kv_heads, dim, scale);
     if (q_rows > 0) {
         p.q = *q;
         p.dout = *dout;
@@ -298,7 +304,7 @@ int rode_window_attention_step(int dtype, int batch, int capacity, int heads, in
     Cached c = {};
     c.batch = batch;
     c.capacity = capacity;
-    c.win = {window, sinks, heads, kv_heads, dim, scale};
+    c.win = window_of(window, sinks, heads, kv_heads, dim, scale);
     c.q = *q;
     if (capacity > 0) {
         c.k = *k_cache;
@@ -341,7 +347,7 @@ int rode_shared_prefix_attention(int dtype, int batch, int prefix, int capacity,
     c.capacity = capacity;
     c.prefix = prefix;
     // every row of the own cache up to the length
-    c.win = {kMaxRows, 0, heads, kv_heads, dim, scale};
+    c.win = window_of(kMaxRows, 0, heads, kv_heads, dim, scale);
     c.q = *q;
     if (prefix > 0) {
         c.pk = *prefix_k;
