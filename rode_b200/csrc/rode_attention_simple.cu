@@ -119,6 +119,7 @@ __device__ __forceinline__ float row_sum(float x) {
 }
 
 // The running softmax of one tile's scores: s becomes the weights, which go to `weights` for weigh_rows.
+// m + log2 l is -inf for a row that has seen no key (m = -inf, l = 0), and NaN for one whose scores are NaN (l is; m need not be).
 template <int kDim, int R>
 __device__ __forceinline__ void softmax_tile(float (&s)[R][R], float (&m)[R], float (&l)[R], float4 (&acc)[R][kDim / 64],
                                              float *weights) {
@@ -219,7 +220,7 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_rows(Prompt p) {
                                    x.z - to_float(from_float<T>(x.z)), x.w - to_float(from_float<T>(x.w))));
         }
         if (tx == 0 && p.lse != nullptr)
-            p.lse[static_cast<long long>(head) * p.seqs.q_rows + row0 + r] = m[i] == -INFINITY ? -INFINITY : (m[i] + log2f(l[i])) * kLn2;
+            p.lse[static_cast<long long>(head) * p.seqs.q_rows + row0 + r] = (m[i] + log2f(l[i])) * kLn2;
     }
 }
 
@@ -281,7 +282,7 @@ __global__ void __launch_bounds__(kThreads, 2) shared_rows(Cached c) {
                 store4(c.prefix_out + at * w.dim + d,
                        make_float4(acc[i][d4].x * inv, acc[i][d4].y * inv, acc[i][d4].z * inv, acc[i][d4].w * inv));
         }
-        if (tx == 0) c.prefix_lse[at] = m[i] == -INFINITY ? -INFINITY : m[i] + log2f(l[i]);
+        if (tx == 0) c.prefix_lse[at] = m[i] + log2f(l[i]);
     }
 }
 
@@ -609,7 +610,7 @@ __global__ void __launch_bounds__(kStepThreads) step_rows(Cached c) {
             if (r >= have || d0 >= w.dim) continue;
             const float inv = sums[r] > 0.f || sums[r] != sums[r] ? 1.f / sums[r] : 0.f;
             result.store<T>(c, r, d0, make_float4(acc[i].x * inv, acc[i].y * inv, acc[i].z * inv, acc[i].w * inv));
-            if (d0 == 0) result.store_lse(r, tops[r] == -INFINITY ? -INFINITY : tops[r] + log2f(sums[r]));
+            if (d0 == 0) result.store_lse(r, tops[r] + log2f(sums[r]));
         }
         if (c.whole) break;
         first += seen.blocks;

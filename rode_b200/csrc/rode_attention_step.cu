@@ -212,7 +212,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) step_tiles(const Cached c) {
             acc.z *= inv;
             acc.w *= inv;
             if (d < w.dim) result.store<T>(c, r, d, acc);
-            if (d == 0) result.store_lse(r, top == -INFINITY ? -INFINITY : top + log2f(sum));
+            if (d == 0) result.store_lse(r, top + log2f(sum));
         }
         if (c.whole) break;
         first += seen.blocks;

@@ -493,7 +493,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 tmem_fence_after();
             }
             const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-            const float lse2 = m == -INFINITY ? -INFINITY : m * s2 + log2f(l);
+            const float lse2 = m * s2 + log2f(l);  // -inf for a row that has seen no key, NaN for one whose scores are
             if (kShared) {
                 const long long at = (wk.part * static_cast<long long>(c.batch) + wk.row0 + t * per_tile + query) * w.heads + head;
                 if (mine) c.prefix_lse[at] = lse2;
@@ -513,7 +513,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             } else {
                 const long long row = wk.row0 + t * per_tile + query;
                 if (mine && p.lse != nullptr)
-                    p.lse[static_cast<long long>(head) * p.seqs.q_rows + row] = lse2 == -INFINITY ? -INFINITY : lse2 * kLn2;
+                    p.lse[static_cast<long long>(head) * p.seqs.q_rows + row] = lse2 * kLn2;
                 T *out = static_cast<T *>(p.out) + (row * w.heads + head) * w.dim;
 #pragma unroll
                 for (int x = 0; x < kDim; x += 32) {
@@ -1143,7 +1143,6 @@ __global__ void __launch_bounds__(kTileThreads, 1) key_gradient_tiles(const __gr
             tmem_wait_load32<32>(s);
             tmem_fence_before();
             barrier_arrive(s_read);
-            if (!whole) hide(s, range, 0xff800000u);
             const auto weight_off = [&](int j) { return load_pair(off_at + j * 4); };
             uint32_t packed[32];
             if (whole) {
@@ -1152,6 +1151,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) key_gradient_tiles(const __gr
             } else {
                 weights_in_place<0, 0>(s, s2, weight_off);
                 weights_in_place<32, 0>(s, s2, weight_off);
+                hide(s, range, 0u);  // (the weights, not the scores: a query whose lse is NaN leaves the keys alone that it does not see)
             }
 #pragma unroll
             for (int j = 0; j < 64; j += 2) packed[j / 2] = pack2<T>(__uint_as_float(s[j]), __uint_as_float(s[j + 1]));
