@@ -68,25 +68,24 @@ __device__ __forceinline__ Pair load_pair(uint32_t shared) {
     return r;
 }
 
-// 2^x by additions and products, for x <= 128 (below -125: as -125): x = n + f with f in [-1/2, 1/2], 2^f by the polynomial of degree 4
-// with the least relative error there (Remez' exchange, 2.7e-6 after rounding its coefficients, far below the rounding of the weights to 16 bits), n
-// added to its exponent.  Adding 1.5 * 2^23 rounds to an integer, whose bits shifted by 23 are n alone.  NaN gives something not finite in 16 bits.
+// 2^x by additions and products, for x < 128: x = n + f with f in [-1/2, 1/2], 2^f by the polynomial of degree 4 with the least relative
+// error there (Remez' exchange, 2.7e-6 after rounding its coefficients, far below the rounding of the weights to 16 bits), times 2^n.  Adding 1.5 * 2^23 + 127
+// rounds to an integer, whose bits shifted by 23 are those of 2^n alone, or of 0 for n = -127: so x below -126.5, -infinity too, gives 0.  NaN gives NaN, by
+// the product (n added to p's exponent made NaN a finite number, and ended at 2^-125, which bf16 holds, without being faster).
 __device__ __forceinline__ void exp2_by_fma(Pair x, float &a, float &b) {
     split(x, a, b);
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(-125.f));
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(b) : "f"(-125.f));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(-127.f));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(b) : "f"(-127.f));
     x = pair_of(a, b);
-    const Pair t = add2(x, pair_of(12582912.f, 12582912.f));
-    const Pair f = fma2(add2(t, pair_of(-12582912.f, -12582912.f)), pair_of(-1.f, -1.f), x);
+    const Pair t = add2(x, pair_of(12583039.f, 12583039.f));
+    const Pair f = fma2(add2(t, pair_of(-12583039.f, -12583039.f)), pair_of(-1.f, -1.f), x);
     Pair p = fma2(f, pair_of(0x1.3997d6p-7f, 0x1.3997d6p-7f), pair_of(0x1.ca1440p-5f, 0x1.ca1440p-5f));
     p = fma2(f, p, pair_of(0x1.ec06dap-3f, 0x1.ec06dap-3f));
     p = fma2(f, p, pair_of(0x1.62e0dcp-1f, 0x1.62e0dcp-1f));
     p = fma2(f, p, pair_of(0x1.ffffe8p-1f, 0x1.ffffe8p-1f));
     float na, nb;
     split(t, na, nb);
-    split(p, a, b);
-    a = __uint_as_float(__float_as_uint(a) + (__float_as_uint(na) << 23));
-    b = __uint_as_float(__float_as_uint(b) + (__float_as_uint(nb) << 23));
+    split(mul2(p, pair_of(__uint_as_float(__float_as_uint(na) << 23), __uint_as_float(__float_as_uint(nb) << 23))), a, b);
 }
 __device__ __forceinline__ float exp2_fast(float x) {
     asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(x));
