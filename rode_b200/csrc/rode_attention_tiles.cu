@@ -1400,6 +1400,7 @@ int tiles_shared(int dtype, const Cached &c, cudaStream_t stream) {
 }
 
 int tiles_waits_failed(int *failed) {
+    RODE_CUDA_TRY(cudaDeviceSynchronize());  // (the copy alone does not wait for streams that do not block, as torch's do not)
     RODE_CUDA_TRY(cudaMemcpyFromSymbol(failed, waits_failed, sizeof(int)));
     return RODE_OK;
 }

@@ -2,7 +2,7 @@
 
 On a CSR pattern, attention is an SDDMM (scores at the stored entries), a softmax per row and an SpMM (their product with the
 values).  The patterns here need not be stored: a sliding window with first tokens that stay visible, and a prefix that a
-batch of requests shares.  Scores, softmax and product run in one pass; all entry points launch on torch's current stream and do
+batch of requests shares.  Scores, softmax and product run in one pass; the operators launch on torch's current stream and do
 not block the host.  No counterpart in the reference.
 
 Types: float32, float16, bfloat16 (all operands of a call alike), sums and softmax in float32.  Head dimension: any multiple of 4
@@ -11,7 +11,7 @@ that sees no key gets zeros.
 """
 from __future__ import annotations
 
-from typing import Optional
+from typing import Optional, Union
 
 import torch
 
@@ -60,3 +60,15 @@ def rode_shared_prefix_attention(q: torch.Tensor, prefix_k: torch.Tensor, prefix
     ``rode_window_attention_step``, for the tokens behind the prefix (a length of 0 is a request that has none yet).  Request b
     sees the whole prefix and the first ``lengths[b]`` rows of its cache.  Not differentiable."""
     return rode_sddmm_cuda.shared_prefix_attention(q, prefix_k, prefix_v, k_cache, v_cache, lengths, _scale(scale, q))
+
+
+def rode_attention_waits_failed(device: Union[torch.device, str, None] = None) -> bool:
+    """Whether a kernel of this module on ``device`` (None: the current one) ever gave up a wait between its warps.
+
+    The tensor-core kernels bound such waits to some seconds instead of hanging.  A call has long returned by then, so nothing raises: where this is
+    True (an error of this library), the results of at least one call so far are wrong or were not written.  Waits for everything that runs on the
+    device; not for every step, but once behind a run whose results count."""
+    device = torch.device("cuda" if device is None else device)
+    if device.type != "cuda":
+        raise ValueError(f"device must be a CUDA device, got {device}")
+    return rode_sddmm_cuda.attention_waits_failed(torch.cuda.current_device() if device.index is None else device.index)

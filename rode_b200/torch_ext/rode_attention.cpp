@@ -305,6 +305,13 @@ Tensor py_shared_prefix(const Tensor &q_in, const Tensor &prefix_k, const Tensor
     return out;
 }
 
+bool py_waits_failed(int64_t device) {
+    const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(device));
+    int failed = 0;
+    check_status(rode_attention_waits_failed(&failed));
+    return failed != 0;
+}
+
 }  // namespace
 
 void bind_attention(pybind11::module_ &m) {
@@ -317,4 +324,6 @@ void bind_attention(pybind11::module_ &m) {
     m.def("shared_prefix_attention", &py_shared_prefix, "Attention of one token per request behind a shared prefix (CUDA)",
           py::arg("q"), py::arg("prefix_k"), py::arg("prefix_v"), py::arg("k_cache"), py::arg("v_cache"), py::arg("lengths"),
           py::arg("scale"));
+    m.def("attention_waits_failed", &py_waits_failed, "Whether a kernel on the device gave up a wait (synchronises)", py::arg("device"),
+          py::call_guard<py::gil_scoped_release>());
 }
