@@ -26,7 +26,7 @@ def rode_window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, win
                           q_offsets: Optional[torch.Tensor] = None, k_offsets: Optional[torch.Tensor] = None,
                           scale: Optional[float] = None) -> torch.Tensor:
     """Attention in which a query sees the ``window`` keys up to its own position and the first ``sinks`` keys of its sequence;
-    differentiable with respect to q, k and v, once.
+    differentiable with respect to q, k and v, once, in reverse mode.
 
     q [q_rows, heads, dim], k and v [k_rows, kv_heads, dim] hold sequences one behind the other: sequence s is rows
     ``q_offsets[s]`` to ``q_offsets[s + 1]`` of q and ``k_offsets[s]`` to ``k_offsets[s + 1]`` of k and v (int32 on the device, not
@@ -48,7 +48,9 @@ def rode_window_attention_step(q: torch.Tensor, k_cache: torch.Tensor, v_cache: 
     q [batch, heads, dim]; k_cache and v_cache [batch, capacity, kv_heads, dim] in any order of the first three dimensions (a
     transposed view of a cache that lies head by head); lengths int32 [batch] on the device: the tokens in each cache, the new
     one among them, taken as at most ``capacity``; a length of 0 gives zeros.  Nothing behind a sequence's length, and nothing
-    between its sinks and its window, is read.  Not differentiable."""
+    between its sinks and its window, is read.
+
+    Not differentiable: operands that require gradients are refused, unless gradients are off (``torch.no_grad()``)."""
     return rode_sddmm_cuda.window_attention_step(q, k_cache, v_cache, lengths, window, sinks, _scale(scale, q))
 
 
@@ -58,7 +60,9 @@ def rode_shared_prefix_attention(q: torch.Tensor, prefix_k: torch.Tensor, prefix
 
     q [batch, heads, dim]; prefix_k and prefix_v [prefix, kv_heads, dim]; k_cache, v_cache and lengths as in
     ``rode_window_attention_step``, for the tokens behind the prefix (a length of 0 is a request that has none yet).  Request b
-    sees the whole prefix and the first ``lengths[b]`` rows of its cache.  Not differentiable."""
+    sees the whole prefix and the first ``lengths[b]`` rows of its cache.
+
+    Not differentiable: operands that require gradients are refused, unless gradients are off (``torch.no_grad()``)."""
     return rode_sddmm_cuda.shared_prefix_attention(q, prefix_k, prefix_v, k_cache, v_cache, lengths, _scale(scale, q))
 
 

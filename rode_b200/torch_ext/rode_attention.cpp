@@ -217,8 +217,21 @@ struct WindowAttention : torch::autograd::Function<WindowAttention> {
     }
 };
 
+// Derivatives that an operator does not have are refused: a result that silently has none would train on nothing.
+void refuse_tangents(const char *what, std::initializer_list<const Tensor *> operands) {
+    for (const Tensor *x : operands)
+        TORCH_CHECK_NOT_IMPLEMENTED(!x->_fw_grad(/*level=*/0).defined(), what, " has no derivative in forward mode");
+}
+void refuse_gradients(const char *what, std::initializer_list<const Tensor *> operands) {
+    refuse_tangents(what, operands);
+    if (!torch::GradMode::is_enabled()) return;
+    for (const Tensor *x : operands)
+        TORCH_CHECK_NOT_IMPLEMENTED(!x->requires_grad(), what, " is not differentiable and an operand requires gradients; call it under torch.no_grad()");
+}
+
 Tensor py_window_attention(const Tensor &q, const Tensor &k, const Tensor &v, int64_t window, int64_t sinks,
                            const OptionalTensor &q_offsets, const OptionalTensor &k_offsets, double scale) {
+    refuse_tangents("rode_window_attention", {&q, &k, &v});
     if (torch::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad()))
         return WindowAttention::apply(q, k, v, window, sinks, q_offsets, k_offsets, scale);
     return std::get<0>(window_forward(q, k, v, window, sinks, q_offsets, k_offsets, scale, false));
@@ -263,6 +276,7 @@ Caches check_caches(const Tensor &q, const Tensor &k_cache, const Tensor &v_cach
 
 Tensor py_window_step(const Tensor &q_in, const Tensor &k_cache, const Tensor &v_cache, const Tensor &lengths, int64_t window,
                       int64_t sinks, double scale) {
+    refuse_gradients("rode_window_attention_step", {&q_in, &k_cache, &v_cache});
     const Caches c = check_caches(q_in, k_cache, v_cache, lengths);
     const c10::cuda::CUDAGuard guard(q_in.device());
     const Tensor q = fitting(q_in);
@@ -282,6 +296,7 @@ Tensor py_window_step(const Tensor &q_in, const Tensor &k_cache, const Tensor &v
 
 Tensor py_shared_prefix(const Tensor &q_in, const Tensor &prefix_k, const Tensor &prefix_v, const Tensor &k_cache,
                         const Tensor &v_cache, const Tensor &lengths, double scale) {
+    refuse_gradients("rode_shared_prefix_attention", {&q_in, &prefix_k, &prefix_v, &k_cache, &v_cache});
     const Caches c = check_caches(q_in, k_cache, v_cache, lengths);
     check_cache(prefix_k, "prefix_k", q_in, 3);
     check_cache(prefix_v, "prefix_v", q_in, 3);
