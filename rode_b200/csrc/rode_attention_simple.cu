@@ -305,8 +305,11 @@ constexpr int backward_shared() {
     return 4 * (4 * tile_rows<kDim>() * (kDim + 4) + 2 * tile_rows<kDim>() * (tile_rows<kDim>() + 4) + 2 * tile_rows<kDim>());
 }
 
-// Weights P and score gradients dS = P (dP - delta) of a tile from s = q.k and dp = do.v.  Rows that saw no key have lse = -inf, but
-// no visible key either.
+// Base-2 logarithm of a row's sum of weights, for the weights 2^(s - it).  -inf (all visible scores were -inf, if there were any) as 0, for the weights to
+// be 0 then, not 2^(-inf + inf).
+__device__ __forceinline__ float sum_log2(float lse) { return lse == -INFINITY ? 0.f : lse * kLog2e; }
+
+// Weights P and score gradients dS = P (dP - delta) of a tile from s = q.k and dp = do.v.
 template <int R>
 __device__ __forceinline__ void score_gradients(float (&s)[R][R], float (&dp)[R][R], const float *lse2, const float *delta, int pos0,
                                                 int have, int k0, const Window &w) {
@@ -356,7 +359,7 @@ __global__ void __launch_bounds__(kThreads) query_gradients(Prompt p) {
         if (tx == 0) {
             const long long at = static_cast<long long>(head) * p.seqs.q_rows + row0 + r;
             delta[r] = sum;
-            lse2[r] = r < have ? p.lse[at] * kLog2e : 0.f;
+            lse2[r] = r < have ? sum_log2(p.lse[at]) : 0.f;
             if (r < have) p.delta[at] = sum;
         }
     }
@@ -439,7 +442,7 @@ __global__ void __launch_bounds__(kThreads) key_gradients(Prompt p) {
             if (threadIdx.x < kRows) {
                 const long long at = static_cast<long long>(h) * p.seqs.q_rows + q0 + threadIdx.x;
                 const bool in = static_cast<int>(threadIdx.x) < n;
-                lse2[threadIdx.x] = in ? p.lse[at] * kLog2e : 0.f;
+                lse2[threadIdx.x] = in ? sum_log2(p.lse[at]) : 0.f;
                 delta[threadIdx.x] = in ? p.delta[at] : 0.f;
             }
             __syncthreads();

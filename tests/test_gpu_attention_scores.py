@@ -73,3 +73,23 @@ def test_scores_far_below_the_largest(dtype):
     keys[far], values[far] = 0.0, 0.0
     seen = R.visible(300, 900, 2000, 0, "cuda") & ~far
     R.check(prompt(q, k, v, dout, 2000, 0, 0.125)["out"], R.one_sequence(q, keys, values, seen, 0.125)["out"])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [64, 128, 20])
+def test_gradients_where_all_scores_are_minus_infinity(dim, dtype):
+    """Weights of 0: no gradient of those keys and values, and none of the others is lost."""
+    q, k, v, dout = _make(300, 300, dim, dtype, 54)
+    q[..., 0], k[..., 0] = 1.0, 0.0
+    k[100:200, :, 0] = -float("inf")
+    off = torch.zeros(300, dtype=torch.bool, device="cuda")
+    off[100:200] = True
+    keys = k.clone()
+    keys[off] = 0.0
+    seen = R.visible(300, 300, 40, 0, "cuda") & ~off            # queries 139 to 199 see keys of no weight alone
+    want = R.one_sequence(q, keys, v, seen, 0.125, dout)
+    got = prompt(q, k, v, dout, 40, 0, 0.125)
+    assert not got["out"][139:200].any() and bool((got["lse"][:, 139:200] == -float("inf")).all())
+    for name in ("out", "dk", "dv"):
+        R.check(got[name], want[name], name)
+    assert not got["dk"][off].any() and not got["dv"][off].any()
