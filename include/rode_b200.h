@@ -302,14 +302,17 @@ int rode_sddmm_f32_ordered(int M, int m1, int m2, int n, int k, long long nnz, c
  *   dim        head dimension: any multiple of 4 up to 256
  *   heads      query heads, a multiple of kv_heads; query head h reads key head h / (heads / kv_heads)
  *   scale      of the scores (usually 1 / sqrt(dim))
- * Strides are in elements, the last dimension is contiguous.  Bases and strides must be multiples of 4 elements; 16-bit operands
- * whose bases and strides are multiples of 16 bytes, with dim a multiple of 8 up to 128, run on the tensor cores, which round the softmax weights (and,
- * backward, the scores' gradients) to dtype before they multiply.  Rows of an operand at most 2^30.
+ * Strides are in elements, the last dimension is contiguous.  Bases and strides must be multiples of 4 elements.  16-bit operands
+ * whose bases and strides are multiples of 16 bytes, with dim a multiple of 8 up to 128, run on the tensor cores: single tokens on their own caches
+ * always, prompts, gradients and shared prefixes where besides scale > 0, heads / kv_heads <= 128 and no stride is 0.  The tensor cores round the softmax
+ * weights (and, backward, the scores' gradients) to dtype before they multiply.  All other operands run on fused multiply-adds in 32 bits, prompts and
+ * gradients tens of times slower where sequences are long.  Rows of an operand at most 2^30.
  *
  * fp16: scores' gradients beyond 65504 become infinite and those below 2^-25 zero, as gradients in fp16 do; scale the loss.
  *
- * A query that sees no key gets a zero row.  A non-finite key or value reaches the queries that see it, and may reach other
- * queries of the same sequence (whose weight for it is 0), never another sequence; nothing behind lengths[b] is read.
+ * A query that sees no key gets a zero row, and so does one whose scores are all -inf.  A non-finite key or value reaches the queries that see it, and
+ * may reach other queries of the same sequence (whose weight for it is 0), never another sequence; a query that is NaN gets a row of NaN.  Gradients
+ * likewise: a non-finite query may reach other keys of its sequence.  Nothing behind lengths[b] is read.
  * Results do not depend on the order in which thread blocks run.
  */
 enum rode_dtype { RODE_F32 = 0, RODE_F16 = 1, RODE_BF16 = 2 };
@@ -338,7 +341,7 @@ int rode_window_attention(int dtype, int n_seq, const int *q_offsets, const int 
 
 /* Its gradients: dq [q_rows, heads, dim], dk and dv [k_rows, kv_heads, dim] contiguous, dk and dv both or neither (null).
  * out, out_rest and lse are what the forward call wrote; without out_rest (null) dq and dk are less exact where queries see few keys.
- *  workspace: rode_window_attention_backward_workspace_bytes() bytes,
+ *  workspace: rode_window_attention_backward_workspace_bytes() bytes (they depend on the current device),
  * 16-byte aligned, not shared by calls that may overlap in time. */
 int rode_window_attention_backward_workspace_bytes(int dtype, int n_seq, int q_rows, int k_rows, int heads, int kv_heads,
                                                    int dim, int window, int sinks, size_t *bytes);

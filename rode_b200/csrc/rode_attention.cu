@@ -94,8 +94,9 @@ struct Parts {
 // at most 256 keys stay whole and save the joining, and so do they behind a prefix where there are enough of them, for there CTAs must be free to go
 // to the SMs that the prefix leaves.
 // Prefix, 16-bit operands: CTAs of 256 rows of queries, one per SM, which the tensor cores bound, while the own keys' are bound by memory and take
-// whatever SMs are left; so the prefix gets the SMs in proportion to its time (blocks of 128 keys at 1.75 us, own keys at 5.4 TB/s with caches half
-// full).  fp32: CTAs of 64 rows, parts down to 64 keys.
+// whatever SMs are left; so the prefix gets the SMs in proportion to its time (own keys at 5.4 TB/s with caches half full; blocks of 128 keys at
+// 1.75 us, as measured at head dimension 128 with two tiles of requests in a CTA: smaller heads and CTAs with one tile are faster, and the prefix is then done
+// before the own keys are).  fp32: CTAs of 64 rows, parts down to 64 keys.
 Parts plan_parts(int dtype, int batch, int prefix, long long seen, int heads, int kv_heads, int dim) {
     Parts p = {};
     p.whole = true;

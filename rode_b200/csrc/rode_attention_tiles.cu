@@ -575,7 +575,7 @@ struct GradientMaps {
 
 // delta = do . o of all rows, a lane per 16 bytes, with what rounding took from o: in rows of few keys dP - delta cancels, and the rounding
 // of o counted as much as that of the result (fp16, sequences of some tens of rows: dQ 0.00042 off instead of 0.0003; writing and reading it costs 70 us of
-// train_long's 2459).  (By two spare warps of the kernel below it took as long as three blocks of keys, more than short windows
+// train_long's 2396).  (By two spare warps of the kernel below it took as long as three blocks of keys, more than short windows
 // have.)
 template <typename T, int kDim>
 __global__ void __launch_bounds__(256) row_deltas(const Prompt p) {
@@ -1329,7 +1329,8 @@ int tiles_prompt(int dtype, const Prompt &p, cudaStream_t stream) {
 }
 
 // Chunks of about a tile's own work, and only where the sequences are long on average: the first tile is then at least three times the work
-// of the others.
+// of the others.  (One long sequence among many short ones, and more sinks than a tile has keys, are left whole: the same results, but the grid waits for the
+// tiles of the sinks.)
 FarPlan plan_far(int n_seq, bool packed, int q_rows, int kv_heads, int dim, int window, int sinks) {
     FarPlan f = {0, 0, 0, 0};
     if (sinks <= 0 || sinks > kRows || n_seq <= 0 || window > (1 << 29)) return f;
