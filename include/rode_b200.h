@@ -376,7 +376,8 @@ int rode_shared_prefix_attention(int dtype, int batch, int prefix, int capacity,
 
 /* The tensor-core kernels give up a wait between their warps after some seconds instead of hanging; the call itself returns RODE_OK all the same, before
  * they run.  *failed (host) becomes 1 if that ever happened on the current device (an error of this library; the results of that call are
- * wrong or were not written), else 0.  Waits for everything that runs on the device, on all streams. */
+ * wrong or were not written), else 0.  Waits for everything that runs on the device, on all streams, so not to be
+ * called while a stream of it is being captured. */
 int rode_attention_waits_failed(int *failed);
 
 #ifdef __cplusplus

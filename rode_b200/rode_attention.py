@@ -71,7 +71,7 @@ def rode_attention_waits_failed(device: Union[torch.device, str, None] = None) -
 
     The tensor-core kernels bound such waits to some seconds instead of hanging.  A call has long returned by then, so nothing raises: where this is
     True (an error of this library), the results of at least one call so far are wrong or were not written.  Waits for everything that runs on the
-    device; not for every step, but once behind a run whose results count."""
+    device (and so cannot be called while a graph is captured); not for every step, but once behind a run whose results count."""
     device = torch.device("cuda" if device is None else device)
     if device.type != "cuda":
         raise ValueError(f"device must be a CUDA device, got {device}")
